@@ -1131,3 +1131,100 @@ def sum_f32(x):
     out = torch.empty(1, dtype=torch.float32, device=x.device)
     check(_abi.lib().dr_sum_f32(_ptr(x), x.numel(), _ptr(out), _stream()), "dr_sum_f32")
     return out
+
+
+# ------------------------------------------------------------------ mixed-precision operators
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # DR_F32, DR_F16, DR_BF16
+
+
+def _req_half(t, name, ndim=None, dtype=None):
+    """A tensor of one of DTYPES (or of exactly `dtype`): contiguous, on the current device."""
+    if dtype is None:
+        if isinstance(t, torch.Tensor) and t.dtype not in DTYPES:
+            raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+        dtype = t.dtype if isinstance(t, torch.Tensor) else None
+    return _req(t, dtype, name, ndim)
+
+
+# ------------------------------------------------------------------ global gradient norm and clipping
+def _norm_list(tensors, name):
+    tensors = list(tensors)
+    for i, t in enumerate(tensors):
+        _req_half(t, "%s[%d]" % (name, i))
+    n = len(tensors)
+    return tensors, (C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_int64 * n)(*[t.numel() for t in tensors]), \
+        (C.c_int32 * n)(*[DTYPES[t.dtype] for t in tensors])
+
+
+def _norm_ws(n, device):
+    return torch.empty(check(_abi.lib().dr_global_norm_bytes(n), "dr_global_norm_bytes"), dtype=torch.uint8, device=device)
+
+
+def global_norm(tensors):
+    """tf.global_norm: sqrt of the sum of all squared elements of a list of float32 / float16 / bfloat16 tensors, as a
+    float32 device tensor [1] (no host synchronisation)."""
+    tensors, ins, counts, dts = _norm_list(tensors, "tensors")
+    dev = tensors[0].device if tensors else torch.device("cuda", torch._C._cuda_getDevice())
+    norm = torch.empty(1, dtype=torch.float32, device=dev)
+    ws = _norm_ws(len(tensors), dev)
+    check(_abi.lib().dr_clip_global_norm(ins, None, counts, dts, len(tensors), 1.0, _ptr(norm), _ptr(ws), ws.numel(),
+                                         _stream()), "dr_clip_global_norm")
+    return norm
+
+
+def clip_by_global_norm(tensors, clip_norm, out=None):
+    """tf.clip_by_global_norm: (list of t * clip_norm / max(norm, clip_norm), norm [1] float32 on the device).  float32,
+    float16 and bfloat16 tensors may be mixed; each is read twice and written once.  out: the tensors to write (same
+    shapes and types; the list itself clips in place); None: new ones.  No host synchronisation."""
+    tensors, ins, counts, dts = _norm_list(tensors, "tensors")
+    if out is None:
+        out = [torch.empty_like(t) for t in tensors]
+    else:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError("clip_by_global_norm: %d tensors but %d outputs" % (len(tensors), len(out)))
+        for i, (o, t) in enumerate(zip(out, tensors)):
+            if _req_half(o, "out[%d]" % i, dtype=t.dtype).shape != t.shape:
+                raise ValueError("clip_by_global_norm: out[%d] must be shaped like tensor %d" % (i, i))
+    dev = tensors[0].device if tensors else torch.device("cuda", torch._C._cuda_getDevice())
+    norm = torch.empty(1, dtype=torch.float32, device=dev)
+    ws = _norm_ws(len(tensors), dev)
+    outs = (C.c_void_p * len(out))(*[o.data_ptr() for o in out])
+    check(_abi.lib().dr_clip_global_norm(ins, outs, counts, dts, len(tensors), float(clip_norm), _ptr(norm), _ptr(ws),
+                                         ws.numel(), _stream()), "dr_clip_global_norm")
+    return out, norm
+
+
+# ------------------------------------------------------------------ embedding lookup with scaling
+def embed_forward(table, ids, scale=1.0):
+    """scale * table[ids]: table [rows, d] float32 / float16 / bfloat16, ids of any shape (int32 or int64), result in the
+    table's type, rounded once.  Ids outside the table give zero rows, as gather() does."""
+    table = _req_half(table, "table", 2)
+    ids, bits = _ids(ids, "ids")
+    if table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError("embed_forward: the table is empty")
+    out = torch.empty(tuple(ids.shape) + (table.shape[1],), dtype=table.dtype, device=table.device)
+    check(_abi.lib().dr_embed_forward(_ptr(table), table.shape[0], table.shape[1], DTYPES[table.dtype], _ptr(ids),
+                                      ids.numel(), bits, float(scale), _ptr(out), _stream()), "dr_embed_forward")
+    return out
+
+
+def embed_backward(gout, ids, rows, scale=1.0, padding_idx=None):
+    """Gradient of embed_forward w.r.t. the table: [rows, d] in gout's type, grad[r] = scale * sum of the gout rows whose
+    id is r (0 where there is none).  Sums in float32, fixed order (bit-repeatable), rounded once.  Ids equal to
+    padding_idx or outside [0, rows) contribute nothing."""
+    gout = _req_half(gout, "gout")
+    ids, bits = _ids(ids, "ids")
+    if gout.dim() < 1 or tuple(gout.shape[:-1]) != tuple(ids.shape):
+        raise ValueError("embed_backward: gout must be shaped like ids plus one dim, got %s for ids %s"
+                         % (tuple(gout.shape), tuple(ids.shape)))
+    n, d, rows = ids.numel(), gout.shape[-1], int(rows)
+    pad = -1 if padding_idx is None else int(padding_idx)
+    if padding_idx is not None and not 0 <= pad < rows:
+        raise ValueError("embed_backward: padding_idx %d is outside the table of %d rows" % (pad, rows))
+    need = check(_abi.lib().dr_embed_backward_bytes(n, d), "dr_embed_backward_bytes")
+    grad = torch.empty((rows, d), dtype=gout.dtype, device=gout.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=gout.device)
+    check(_abi.lib().dr_embed_backward(_ptr(gout), n, d, DTYPES[gout.dtype], _ptr(ids), bits, rows, float(scale), pad,
+                                       _ptr(grad), _ptr(ws), ws.numel(), _stream()), "dr_embed_backward")
+    return grad

@@ -56,6 +56,11 @@ extern "C" {
 #define DR_SCORE_NEG_SQDIST 1 /* cml.py:151-153                                       */
 #define DR_SCORE_TWO_DIST 2   /* SeqRecMetrics.py:122-123 (AttRec / PRME)             */
 
+/* element types of the mixed-precision entry points (dr_embed_*, dr_clip_global_norm) */
+#define DR_F32 0
+#define DR_F16 1
+#define DR_BF16 2
+
 /* hyper-parameters of one optimizer application (all fp32) */
 typedef struct dr_opt_params {
     int32_t kind;    /* DR_OPT_*                                               */
@@ -540,6 +545,29 @@ int32_t dr_shard_bpr_finish(float* P, float* Pslot0, float* Pslot1, float* Q, fl
                             int32_t world, int32_t me, int64_t B, int64_t num_user, int64_t num_item, int32_t k,
                             int64_t cap_s, int64_t cap_g, const float* received, const dr_opt_params* opt, float* loss_out,
                             void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- global gradient norm over many tensors, and clipping -----------------------------------------------------------
+ * tf.clip_by_global_norm (the reference clips rows only, cml.py:80-81): norm = sqrt(sum over the n tensors of the sum of
+ * their squared elements), out[i] = in[i] * clip_norm / max(norm, clip_norm); a norm that is not finite makes every output
+ * NaN.  in / out / count / dtype are HOST arrays of n device pointers, element counts and DR_F32 / DR_F16 / DR_BF16; every
+ * tensor is contiguous, out[i] has in[i]'s type.  out[i] == in[i] clips in place; any other overlap of an output is
+ * refused.  out NULL: only the norm.  norm_out: fp32 device scalar (NULL: not wanted).  Sums in fp64, in a fixed order.
+ * Recorded gradient rows of a table count row by row, duplicates not combined, as TensorFlow's IndexedSlices do. */
+int64_t dr_global_norm_bytes(int32_t n);
+int32_t dr_clip_global_norm(const void* const* in, void* const* out, const int64_t* count, const int32_t* dtype, int32_t n,
+                            float clip_norm, float* norm_out, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- embedding lookup with scaling, and its gradient by sorted ids ----------------------------------------------------
+ * forward: out[e, :] = scale * table[ids[e], :], table [rows, d] and out [n, d] of one type (DR_F32 / DR_F16 / DR_BF16),
+ * rounded once; an id outside [0, rows) gives a zero row (as dr_gather_f32).  1 <= d <= 32768.
+ * backward: grad [rows, d] (overwritten, every row; 16-byte aligned) = scale * sum over the e with ids[e] == r of
+ * gout[e, :], summed in fp32 in a fixed order and rounded once; ids that equal `padding` (-1: none) or lie outside
+ * [0, rows) contribute nothing.  ws: dr_embed_backward_bytes(n, d), 256-byte aligned. */
+int32_t dr_embed_forward(const void* table, int64_t rows, int32_t d, int32_t dtype, const void* ids, int64_t n,
+                         int32_t id_bits, float scale, void* out, void* stream);
+int64_t dr_embed_backward_bytes(int64_t n, int32_t d);
+int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype, const void* ids, int32_t id_bits,
+                          int64_t rows, float scale, int64_t padding, void* grad, void* ws, int64_t ws_bytes, void* stream);
 
 /* ---- measurement hooks (no counterpart in the reference) ---------------------------------------------
  * dr_profile_enable(1): from now on every instrumented kernel launch of this library (the gather kernel, the fused step's forward

@@ -1,0 +1,261 @@
+"""Scaled embedding lookup, its gradient by sorted ids, and global-norm clipping against plain 64-bit restatements.
+
+Tolerances.  eps = finfo(t).eps / 2 is the largest relative error of one rounding to t.
+  lookup           one fp32 product, one rounding: |err| <= (eps + 2^-24 + tiny) |ref|, plus half the smallest subnormal of t
+  lookup gradient  a row that sums m terms of absolute sum A: fp32 sums in any order err by at most (m + 1) 2^-24 A, then
+                   one product and one rounding
+  norm             fp64 sums: the final rounding to fp32 only;  clipped values: fp32 factor, fp32 product, one rounding"""
+import math
+
+import pytest
+import torch
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+gpu = pytest.mark.gpu
+
+
+def _eps(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def _sub(dt):
+    return torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+
+
+def _within(got, ref, bound):
+    got, ref = got.detach().cpu().double(), ref.cpu()
+    err = (got - ref).abs()
+    bad = ~(err <= bound.cpu())
+    assert not bool(bad.any()), (int(bad.sum()), float(err[bad].max()), got[bad][:4], ref[bad][:4])
+
+
+def _ids(n, rows, idt, g, bad=False):
+    ids = (torch.rand(n, generator=g) ** 4 * rows).long().clamp_(0, rows - 1)
+    if bad and n > 3:
+        ids[1], ids[n // 2] = -1, rows
+    return ids.to(idt)
+
+
+# ---- embedding -------------------------------------------------------------------------------------------------------
+EMBED = [(1, 1, 1), (7, 3, 5), (1683, 150, 5000), (50, 128, 4096), (50, 128, 4097), (300, 256, 9000), (9, 100, 20000),
+         (100001, 64, 70001), (5, 1030, 300), (70000, 7, 33)]
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,d,n", EMBED)
+def test_embed_forward(dev, rows, d, n, dt):
+    from deeprec_amd import kernels as K
+    g = torch.Generator().manual_seed(rows * 7 + d + n)
+    table = torch.randn((rows, d), generator=g).to(dt)
+    for idt in (torch.int32, torch.int64):
+        ids = _ids(n, rows, idt, g, bad=True)
+        scale = math.sqrt(d)
+        out = K.embed_forward(table.to(dev), ids.to(dev), scale=scale)
+        ok = (ids >= 0) & (ids < rows)
+        ref = table.double()[ids.long().clamp(0, rows - 1)] * scale * ok[:, None]
+        assert out.dtype == dt and out.shape == (n, d)
+        _within(out, ref, (_eps(dt) + 2.0 ** -23) * ref.abs() + _sub(dt))
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,d,n", EMBED + [(400, 32, 0)])
+def test_embed_backward(dev, rows, d, n, dt):
+    from deeprec_amd import kernels as K
+    g = torch.Generator().manual_seed(rows + 3 * d + n)
+    gout = torch.randn((n, d), generator=g).to(dt)
+    scale = 0.7
+    for idt, pad in ((torch.int32, None), (torch.int64, 0)):
+        ids = _ids(n, rows, idt, g, bad=True)
+        grad = K.embed_backward(gout.to(dev), ids.to(dev), rows, scale=scale, padding_idx=pad)
+        again = K.embed_backward(gout.to(dev), ids.to(dev), rows, scale=scale, padding_idx=pad)
+        assert torch.equal(grad, again)                                   # fixed order
+        ok = (ids >= 0) & (ids < rows)
+        if pad is not None:
+            ok &= ids != pad
+        i = ids.long()[ok]
+        ref = torch.zeros((rows, d), dtype=torch.float64).index_add_(0, i, gout.double()[ok]) * scale
+        A = torch.zeros((rows, d), dtype=torch.float64).index_add_(0, i, gout.double().abs()[ok]) * scale
+        m = torch.zeros(rows, dtype=torch.float64).index_add_(0, i, torch.ones(len(i), dtype=torch.float64))
+        _within(grad, ref, _eps(dt) * (ref.abs() + (m[:, None] + 3) * 2.0 ** -24 * A) + (m[:, None] + 3) * 2.0 ** -24 * A + _sub(dt))
+        assert not bool(grad[m.to(dev) == 0].any())
+
+
+@gpu
+@pytest.mark.parametrize("n", [31, 64, 4096, 40000])
+def test_embed_backward_one_id(dev, n):
+    """Every entry the same row; integers, so that any order gives the exact sum."""
+    from deeprec_amd import kernels as K
+    ids = torch.full((n,), 3, dtype=torch.int32, device=dev)
+    gout = torch.randint(-4, 5, (n, 20), generator=torch.Generator().manual_seed(n)).float().to(dev)
+    grad = K.embed_backward(gout, ids, 5)
+    assert torch.equal(grad[3].cpu(), gout.cpu().double().sum(0).float())
+    assert not bool(grad[[0, 1, 2, 4]].any())
+    assert not bool(K.embed_backward(gout, ids, 5, padding_idx=3).any())
+
+
+@gpu
+def test_embed_unaligned_views_and_shapes(dev):
+    """Contiguous tensors whose first element is not on a 16-byte border; ids of several dims; no ids."""
+    from deeprec_amd import kernels as K
+    for dt in DTYPES:
+        base = torch.randn(1 + 40 * 16, device=dev).to(dt)
+        table = base[1:].view(40, 16)
+        ids = torch.randint(0, 40, (6, 7), device=dev)
+        assert torch.equal(K.embed_forward(table, ids), table[ids])
+        gb = torch.randint(-3, 4, (1 + 42 * 16,), device=dev).to(dt)
+        gout = gb[1:].view(6, 7, 16)
+        ref = torch.zeros((40, 16), dtype=torch.float64, device=dev).index_add_(0, ids.reshape(-1), gout.reshape(42, 16).double())
+        assert torch.equal(K.embed_backward(gout, ids, 40).double(), ref)
+        none = torch.empty((0,), dtype=torch.int32, device=dev)
+        assert K.embed_forward(table, none).shape == (0, 16)
+
+
+@gpu
+def test_embed_graph_replay(dev):
+    from deeprec_amd import kernels as K
+    ids = torch.randint(0, 500, (6000,), device=dev, dtype=torch.int32)
+    table, gout = torch.randn(500, 48, device=dev), torch.randn(6000, 48, device=dev)
+    K.embed_backward(gout, ids, 500), K.embed_forward(table, ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, gr = K.embed_forward(table, ids, 2.0), K.embed_backward(gout, ids, 500, 2.0)
+    for seed in range(3):
+        ids.copy_(torch.randint(0, 500, (6000,), generator=torch.Generator().manual_seed(seed)))
+        gout.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, K.embed_forward(table, ids, 2.0)) and torch.equal(gr, K.embed_backward(gout, ids, 500, 2.0))
+
+
+def test_embed_refusals_cpu():
+    import ctypes as C
+    from deeprec_amd import _abi, kernels as K
+    lib = _abi.lib()
+    with pytest.raises(TypeError):
+        K.embed_forward(torch.zeros(4, 4), torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(TypeError):
+        K.embed_backward(torch.zeros(4, 4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32), 3)
+    p = C.c_void_p(4096)
+    assert lib.dr_embed_forward(p, 4, 4, 3, p, 2, 32, 1.0, p, None) == -1 and b"dtype" in lib.dr_last_error()
+    assert lib.dr_embed_forward(p, 4, 4, 0, p, 2, 16, 1.0, p, None) == -1 and b"id_bits" in lib.dr_last_error()
+    assert lib.dr_embed_forward(p, 0, 4, 0, p, 2, 32, 1.0, p, None) == -1 and b"bad sizes" in lib.dr_last_error()
+    assert lib.dr_embed_forward(p, 4, 40000, 0, p, 2, 32, 1.0, p, None) == -1
+    assert lib.dr_embed_forward(C.c_void_p(4097), 4, 4, 0, p, 2, 32, 1.0, p, None) == -1 and b"aligned" in lib.dr_last_error()
+    assert lib.dr_embed_backward_bytes(-1, 4) < 0 and lib.dr_embed_backward_bytes(4, 0) < 0
+    assert lib.dr_embed_backward(p, 5000, 4, 0, p, 32, 9, 1.0, -1, p, p, 16, None) == -2
+    assert lib.dr_embed_backward(p, 5, 4, 0, p, 32, 9, 1.0, -1, C.c_void_p(4100), p, 1 << 20, None) == -1
+
+
+# ---- clipping --------------------------------------------------------------------------------------------------------
+def _grads(shapes, dts, std, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=g) * std).to(dts[i % len(dts)]) for i, s in enumerate(shapes)]
+
+
+SHAPES = [[(1,)], [(0,), (3, 5), (0, 7)], [(8192,), (8191,), (8193,), (1, 2, 3)], [(257, 129), (64,), (40000, 3), (5,)],
+          [(i + 1, 3) for i in range(300)]]
+
+
+@gpu
+@pytest.mark.parametrize("std", [0.001, 2.0])
+@pytest.mark.parametrize("dts", [[torch.float32], [torch.bfloat16, torch.float32, torch.float16]])
+@pytest.mark.parametrize("shapes", SHAPES)
+def test_clip_by_global_norm(dev, shapes, dts, std):
+    from deeprec_amd import kernels as K
+    host = _grads(shapes, dts, std, len(shapes))
+    ts = [t.to(dev) for t in host]
+    total = math.sqrt(sum(float(t.double().pow(2).sum()) for t in host))
+    clip = 1.5
+    out, norm = K.clip_by_global_norm(ts, clip)
+    assert abs(float(norm) - total) <= 2.0 ** -23 * total
+    assert torch.equal(K.global_norm(ts), norm)
+    c = clip / max(total, clip)
+    for o, t, h in zip(out, ts, host):
+        assert torch.equal(t.cpu(), h)                                     # inputs stay
+        ref = h.double() * c
+        _within(o, ref, (_eps(h.dtype) + 2.0 ** -22) * ref.abs() + _sub(h.dtype))
+    inplace, n2 = K.clip_by_global_norm(ts, clip, out=ts)                  # in place: the same bits
+    assert torch.equal(n2, norm)
+    for o, t in zip(out, ts):
+        assert torch.equal(o, t)
+
+
+@gpu
+def test_clip_extremes(dev):
+    from deeprec_amd import kernels as K
+    big = torch.tensor([3e30, -4e30], device=dev)                          # squares overflow fp32
+    out, norm = K.clip_by_global_norm([big], 1.0)
+    assert abs(float(norm) - 5e30) < 1e24 and torch.allclose(out[0].cpu(), torch.tensor([0.6, -0.8]))
+    tiny = torch.tensor([3e-30, 4e-30], device=dev)                        # squares underflow fp32
+    assert abs(float(K.global_norm([tiny])) - 5e-30) < 1e-36
+    for bad in (math.inf, math.nan):
+        out, norm = K.clip_by_global_norm([torch.ones(5, device=dev), torch.tensor([bad], device=dev)], 1.0)
+        assert bool(torch.isnan(out[0]).all()) and bool(torch.isnan(out[1]).all()) and not math.isfinite(float(norm))
+    out, norm = K.clip_by_global_norm([], 1.0)
+    assert out == [] and float(norm) == 0.0
+    zero = torch.zeros(9, device=dev)
+    out, norm = K.clip_by_global_norm([zero], 1.0)
+    assert float(norm) == 0.0 and not bool(out[0].any())
+    base = torch.randn(1001, device=dev)                                   # views off the 16-byte border
+    out, norm = K.clip_by_global_norm([base[1:], base[:1]], 1.0)
+    ref = base.double() / base.double().norm().clamp_min(1.0)
+    assert torch.allclose(out[0].double(), ref[1:], rtol=1e-6) and torch.allclose(out[1].double(), ref[:1], rtol=1e-6)
+
+
+@gpu
+def test_clip_refusals(dev):
+    from deeprec_amd import kernels as K
+    from deeprec_amd._abi import DeepRecError
+    t = torch.ones(100, device=dev)
+    for bad in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(DeepRecError, match="clip_norm"):
+            K.clip_by_global_norm([t], bad)
+    with pytest.raises(DeepRecError, match="overlaps"):
+        K.clip_by_global_norm([t, t], 1.0, out=[t, t])                     # the same tensor twice, in place
+    with pytest.raises(DeepRecError, match="overlaps"):
+        K.clip_by_global_norm([t[:60], t[40:]], 1.0, out=[t[:60], torch.empty(60, device=dev)])
+    K.clip_by_global_norm([t, t], 1.0)                                     # fresh outputs: fine
+    with pytest.raises(ValueError):
+        K.clip_by_global_norm([t], 1.0, out=[])
+    with pytest.raises(ValueError):
+        K.clip_by_global_norm([t.view(10, 10).t()], 1.0)
+    with pytest.raises(TypeError):
+        K.clip_by_global_norm([t.double()], 1.0)
+
+
+@gpu
+def test_clip_graph_replay(dev):
+    from deeprec_amd import kernels as K
+    ts = [torch.randn(s, device=dev) for s in ((3000, 7), (11,), (129, 65))]
+    K.clip_by_global_norm(ts, 1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, norm = K.clip_by_global_norm(ts, 1.0)
+    for _ in range(3):
+        for t in ts:
+            t.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        o2, n2 = K.clip_by_global_norm(ts, 1.0)
+        assert torch.equal(norm, n2) and all(torch.equal(a, b) for a, b in zip(out, o2))
+
+
+def test_clip_refusals_cpu():
+    import ctypes as C
+    from deeprec_amd import _abi
+    lib = _abi.lib()
+    n = lib.dr_global_norm_bytes(1)
+    assert n > 0 and lib.dr_global_norm_bytes(129) == 2 * n and lib.dr_global_norm_bytes(-1) < 0
+    one = (C.c_void_p * 1)(4096)
+    cnt, dt = (C.c_int64 * 1)(10), (C.c_int32 * 1)(0)
+    w = C.c_void_p(8192)
+    assert lib.dr_clip_global_norm(one, None, cnt, dt, 1, 1.0, None, w, n, None) == -1
+    assert lib.dr_clip_global_norm(one, one, cnt, dt, 1, 1.0, None, w, n - 1, None) == -2
+    assert lib.dr_clip_global_norm(one, one, cnt, (C.c_int32 * 1)(5), 1, 1.0, None, w, n, None) == -1
+    assert lib.dr_clip_global_norm(one, one, (C.c_int64 * 1)(-1), dt, 1, 1.0, None, w, n, None) == -1
+    odd = (C.c_void_p * 1)(4098)
+    assert lib.dr_clip_global_norm(odd, one, cnt, dt, 1, 1.0, None, w, n, None) == -1 and b"aligned" in lib.dr_last_error()
