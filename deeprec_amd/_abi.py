@@ -105,6 +105,9 @@ SIGNATURES = {
     "dr_embed_forward": (_i32, [_p, _i64, _i32, _i32, _p, _i64, _i32, _f, _p, _p]),
     "dr_embed_backward_bytes": (_i64, [_i64, _i32]),
     "dr_embed_backward": (_i32, [_p, _i64, _i32, _i32, _p, _i32, _i64, _f, _i64, _p, _p, _i64, _p]),
+    "dr_item_logprobs_bytes": (_i64, [_i64, _i64, _i32]),
+    "dr_item_logprobs_forward": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dr_item_logprobs_backward": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p]),
     "dr_profile_enable": (_i32, [_i32]),
     "dr_profile_collect": (_i32, [C.c_char_p, _i64, C.POINTER(C.c_float), _i32]),
     "dr_profile_collect_timeline": (_i32, [C.c_char_p, _i64, _p, _p, _i32]),

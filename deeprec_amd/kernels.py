@@ -3,6 +3,7 @@
 Every function takes CUDA(HIP) tensors, validates shapes / dtypes / contiguity on the host
 (the kernels assume them), and enqueues on torch's current stream.
 """
+import collections
 import ctypes as C
 
 import torch
@@ -1228,3 +1229,74 @@ def embed_backward(gout, ids, rows, scale=1.0, padding_idx=None):
     check(_abi.lib().dr_embed_backward(_ptr(gout), n, d, DTYPES[gout.dtype], _ptr(ids), bits, rows, float(scale), pad,
                                        _ptr(grad), _ptr(ws), ws.numel(), _stream()), "dr_embed_backward")
     return grad
+
+
+# ------------------------------------------------------------------ catalog log-probabilities
+LOGP_MAX_T, LOGP_MAX_K = 64, 64
+LogProbs = collections.namedtuple("LogProbs", "logp entropy lse top_idx top_logp")
+
+
+def _logits(t, targets):
+    """logits [N, V] with unit column stride (any row stride >= V); targets None, [N] or [N, T]."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("logits must be a CUDA/HIP tensor (deeprec_amd has no CPU path)")
+    _on_current_device(t, "logits")
+    if t.dtype not in DTYPES:
+        raise TypeError("logits must be float32, float16 or bfloat16, got %s" % t.dtype)
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError("logits must be [N, V] with V >= 1, got %s" % (tuple(t.shape),))
+    N, V = t.shape
+    ld = t.stride(0) if N > 1 else V
+    if (V > 1 and t.stride(1) != 1) or ld < V:
+        raise ValueError("logits must have unit column stride and rows that do not overlap")
+    if targets is None:
+        return N, V, ld, None, 32, 0
+    targets, bits = _ids(targets, "targets")
+    if targets.dim() not in (1, 2) or targets.shape[0] != N:
+        raise ValueError("targets must be [N] or [N, T], got %s" % (tuple(targets.shape),))
+    T = targets.shape[1] if targets.dim() == 2 else 1
+    if T > LOGP_MAX_T:
+        raise ValueError("at most %d targets a row" % LOGP_MAX_T)
+    return N, V, ld, targets, bits, T
+
+
+def item_logprobs_forward(logits, targets=None, K=0):
+    """Log-probabilities under softmax(logits) over the catalog: LogProbs(logp, entropy, lse, top_idx, top_logp).
+    logits [N, V] float32 / float16 / bfloat16 (-inf: not offered), targets [N] or [N, T] ids (outside [0, V): missing,
+    logp 0).  logp is shaped like targets (None without), entropy [N], lse [N, 2] = (maximum, log sum exp(x - maximum)),
+    top_idx int32 / top_logp [N, K]: the K largest, ties by lower index, -1 / -inf behind the last one offered (None with
+    K = 0).  Everything float32."""
+    N, V, ld, targets, bits, T = _logits(logits, targets)
+    K = int(K)
+    if not 0 <= K <= LOGP_MAX_K:
+        raise ValueError("K must be 0..%d" % LOGP_MAX_K)
+    dev = logits.device
+    logp = torch.empty(targets.shape, dtype=torch.float32, device=dev) if targets is not None else None
+    ent = torch.empty(N, dtype=torch.float32, device=dev)
+    lse = torch.empty((N, 2), dtype=torch.float32, device=dev)
+    idx = torch.empty((N, K), dtype=torch.int32, device=dev) if K else None
+    top = torch.empty((N, K), dtype=torch.float32, device=dev) if K else None
+    ws = torch.empty(check(_abi.lib().dr_item_logprobs_bytes(N, V, K), "dr_item_logprobs_bytes"), dtype=torch.uint8, device=dev)
+    check(_abi.lib().dr_item_logprobs_forward(_ptr(logits), N, V, ld, DTYPES[logits.dtype], _ptr(targets), bits, T, K,
+                                              _ptr(logp), _ptr(ent), _ptr(lse), _ptr(idx), _ptr(top), _ptr(ws), ws.numel(),
+                                              _stream()), "dr_item_logprobs_forward")
+    return LogProbs(logp, ent, lse, idx, top)
+
+
+def item_logprobs_backward(logits, targets, lse, entropy, g_logp, g_entropy=None):
+    """d loss / d logits [N, V] (contiguous, the logits' type) of item_logprobs_forward's logp and entropy: g_logp shaped
+    like targets (None without targets), g_entropy [N] or None; lse and entropy as the forward returned them."""
+    N, V, ld, targets, bits, T = _logits(logits, targets)
+    if tuple(_req(lse, torch.float32, "lse", 2).shape) != (N, 2):
+        raise ValueError("lse must be [N, 2] as item_logprobs_forward returns it")
+    if targets is not None and _req(g_logp, torch.float32, "g_logp").shape != targets.shape:
+        raise ValueError("g_logp must be shaped like targets")
+    if g_entropy is not None and (tuple(_req(g_entropy, torch.float32, "g_entropy", 1).shape) != (N,)
+                                  or tuple(_req(entropy, torch.float32, "entropy", 1).shape) != (N,)):
+        raise ValueError("g_entropy and entropy must be [N]")
+    out = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
+    check(_abi.lib().dr_item_logprobs_backward(_ptr(logits), N, V, ld, DTYPES[logits.dtype], _ptr(targets), bits, T,
+                                               _ptr(lse), _ptr(entropy) if g_entropy is not None else None,
+                                               _ptr(g_logp) if targets is not None else None, _ptr(g_entropy), _ptr(out),
+                                               _stream()), "dr_item_logprobs_backward")
+    return out

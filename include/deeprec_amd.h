@@ -56,7 +56,7 @@ extern "C" {
 #define DR_SCORE_NEG_SQDIST 1 /* cml.py:151-153                                       */
 #define DR_SCORE_TWO_DIST 2   /* SeqRecMetrics.py:122-123 (AttRec / PRME)             */
 
-/* element types of the mixed-precision entry points (dr_embed_*, dr_clip_global_norm) */
+/* element types of the mixed-precision entry points (dr_embed_*, dr_item_logprobs_*, dr_clip_global_norm) */
 #define DR_F32 0
 #define DR_F16 1
 #define DR_BF16 2
@@ -568,6 +568,27 @@ int32_t dr_embed_forward(const void* table, int64_t rows, int32_t d, int32_t dty
 int64_t dr_embed_backward_bytes(int64_t n, int32_t d);
 int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype, const void* ids, int32_t id_bits,
                           int64_t rows, float scale, int64_t padding, void* grad, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- log-probabilities of given items over the catalog, entropy and best items ----------------------------------------
+ * logits [N, V] (DR_F32 / DR_F16 / DR_BF16, row stride ld >= V elements): -inf marks an item that is not offered.
+ * targets [N, T] int32 / int64 (T <= 64; NULL with T = 0); an entry outside [0, V) is missing: its logp is 0 and it has no
+ * gradient.  forward, all fp32 / int32:
+ *   logp [N, T]     log softmax(logits)[target]
+ *   entropy [N]     -sum p log p
+ *   lse [N, 2]      the row's maximum M and log sum exp(x - M) (what the backward needs; their sum is the log-sum-exp)
+ *   top_idx, top_logp [N, K]   the K (<= 64; 0: not wanted) largest logits' items and log-probabilities, by value and then
+ *                   by lower index; -1 / -inf behind the last item offered
+ * A row without any offered item: logp -inf, entropy 0, lse (-inf, 0), no best items, gradient 0.  A NaN or +inf logit makes
+ * the row's logp, entropy and gradients NaN (NaN is never among the best).  ws: dr_item_logprobs_bytes(N, V, K), 256-byte
+ * aligned.  backward: g_logp [N, T] and g_entropy [N] (NULL: none) fp32 -> glogits [N, V] contiguous, in the logits' type:
+ *   sum_t g_t [v = target_t] - p_v (sum_t g_t + g_entropy (log p_v + entropy)), rounded once. */
+int64_t dr_item_logprobs_bytes(int64_t N, int64_t V, int32_t K);
+int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64_t V, int64_t ld, int32_t dtype, const void* targets,
+                                 int32_t id_bits, int32_t T, int32_t K, float* logp, float* entropy, float* lse,
+                                 int32_t* top_idx, float* top_logp, void* ws, int64_t ws_bytes, void* stream);
+int32_t dr_item_logprobs_backward(const void* logits, int64_t N, int64_t V, int64_t ld, int32_t dtype, const void* targets,
+                                  int32_t id_bits, int32_t T, const float* lse, const float* entropy, const float* g_logp,
+                                  const float* g_entropy, void* glogits, void* stream);
 
 /* ---- measurement hooks (no counterpart in the reference) ---------------------------------------------
  * dr_profile_enable(1): from now on every instrumented kernel launch of this library (the gather kernel, the fused step's forward
