@@ -108,6 +108,14 @@ SIGNATURES = {
     "dr_item_logprobs_bytes": (_i64, [_i64, _i64, _i32]),
     "dr_item_logprobs_forward": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "dr_item_logprobs_backward": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p]),
+    "dr_window_attn_forward": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _f, _p, _p, _p, _p,
+                                      _p]),
+    "dr_window_attn_backward_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i64, _i32]),
+    "dr_window_attn_backward": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _f,
+                                       _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dr_window_attn_token_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i64, _i32]),
+    "dr_window_attn_token": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _f, _p, _p, _p, _p,
+                                    _i64, _p]),
     "dr_profile_enable": (_i32, [_i32]),
     "dr_profile_collect": (_i32, [C.c_char_p, _i64, C.POINTER(C.c_float), _i32]),
     "dr_profile_collect_timeline": (_i32, [C.c_char_p, _i64, _p, _p, _i32]),

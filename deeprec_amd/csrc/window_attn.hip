@@ -1,0 +1,1095 @@
+// Causal attention over a sliding window and the first few items of a history:
+//   key j is visible to query i iff begin <= j <= i < end and (i - j < window or j - begin < sinks)
+//   out_i = sum_j p_ij v_j,  p_i = softmax_j(scale <q_i, k_j>) over the visible j;   lse_i = log sum_j exp(scale <q_i, k_j>)
+// [begin, end) is the part of the row that holds the history (padding on either side); a query outside it gets zeros and
+// lse = -inf, keys and values outside it are never read.  Hq query heads share Hkv key / value heads in groups.
+//
+// Tiles of 16 queries x 16 keys on the matrix cores.  The contraction is laid out so that nothing moves between lanes: with
+// S^T = K Q^T a lane holds, for ONE query, four keys of each 16-key tile (rows 4 g + i of lane group g), and that is already
+// the B operand of O^T = V^T P^T if slot (g, e) of the 32-long contraction means key 4 g + e (e < 4) or 16 + 4 g + e - 4:
+// the order of a sum is free as long as A uses the same one, and A = V^T is read from LDS by that rule (two transposing
+// 8-byte reads for 16-bit types, eight 4-byte reads for fp32).  Running maximum and sum are one scalar per lane.
+// fp32 runs the same code: a 16x16x32 step is eight v_mfma_f32_16x16x4_f32, element e of every lane's eight in step e.
+// Scores, statistics and sums are fp32; P and dS are rounded to the storage type for the second product, as its operands
+// are (fp32: not at all).
+#include <initializer_list>
+#include <type_traits>
+
+#include "dr_types.h"
+
+namespace dr {
+
+constexpr int WA_MAX_D = 256, WA_MAX_SINKS = 64;
+constexpr int WA_BK = 32;              // keys (queries in the dK / dV kernels) per tile
+constexpr float WA_LOG2E = 1.44269504088896340736f;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <class T>
+using Oct = typename VecType<T, 8>::type;
+
+__device__ __forceinline__ f32x4 mma(const Oct<bf16>& a, const Oct<bf16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Oct<f16>& a, const Oct<f16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Oct<float>& a, const Oct<float>& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+// LDS row length: rows of a 16-lane read start 4 banks apart
+template <class T, int DP>
+constexpr int lds_ld() {
+    return DP + (sizeof(T) == 2 ? 8 : 4);
+}
+
+// 8 elements at p of which the first n exist (the rest: 0); al = bytes that every row start is aligned to
+template <class T>
+__device__ __forceinline__ Oct<T> load_oct(const T* p, int n, int al) {
+    Oct<T> r;
+    if (n >= 8 && al >= 16) {
+        if constexpr (sizeof(T) == 2) {
+            r = *reinterpret_cast<const Oct<T>*>(p);
+        } else {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                r[e] = x[e];
+                r[4 + e] = y[e];
+            }
+        }
+    } else if (n >= 8 && al >= 4) {
+        typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        typename std::conditional<sizeof(T) == 2, u32x4, u32x8>::type w;
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(T) * 2; ++e) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+        r = __builtin_bit_cast(Oct<T>, w);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = e < n ? p[e] : (T)0.0f;
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ Oct<T> zero_oct() {
+    Oct<T> r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (T)0.0f;
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void lds_store_oct(T* p, const Oct<T>& r) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<Oct<T>*>(p) = r;
+    } else {
+        *reinterpret_cast<f32x4*>(p) = f32x4{r[0], r[1], r[2], r[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{r[4], r[5], r[6], r[7]};
+    }
+}
+// 8 consecutive elements of a row (operand whose contraction runs along the row)
+template <class T>
+__device__ __forceinline__ Oct<T> row_frag(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+        return *reinterpret_cast<const Oct<T>*>(p);
+    } else {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+        Oct<T> r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r[e] = x[e];
+            r[4 + e] = y[e];
+        }
+        return r;
+    }
+}
+// column col0 + (lane & 15) at the 8 rows of lane group g = lane / 16: 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3
+template <class T, int LD>
+__device__ __forceinline__ Oct<T> col_frag(const T* tile, int col0) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    if constexpr (sizeof(T) == 2) {
+        // the transposing read: of the 16 lanes of a group, lanes 4 r .. 4 r + 3 name row r's 16 columns, lane i gets
+        // column i of the four rows
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const T* p = tile + (4 * g + (i >> 2)) * LD + col0 + 4 * (i & 3);
+        struct {
+            s16x4 a, b;
+        } r;
+        r.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+        r.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 16 * LD));
+        return __builtin_bit_cast(Oct<T>, r);
+    } else {
+        Oct<T> r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r[e] = tile[(4 * g + e) * LD + col0 + i];
+            r[4 + e] = tile[(16 + 4 * g + e) * LD + col0 + i];
+        }
+        return r;
+    }
+}
+template <class T>
+__device__ __forceinline__ Oct<T> to_oct(const f32x4& a, const f32x4& b) {
+    Oct<T> r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        r[e] = (T)a[e];
+        r[4 + e] = (T)b[e];
+    }
+    return r;
+}
+
+struct WinStride {
+    int64_t b, l, h;
+};
+struct WinArgs {
+    const void *q, *k, *v, *out, *gout;
+    WinStride qs, ks, vs;      // elements; out and gout are contiguous [B, L, Hq, D]
+    int B, L, Hq, Hkv, D, W, S;
+    int tiles;                 // workgroups along the sequence
+    float scale;
+    const int32_t *begin, *end;
+    int al, alg;               // alignment in bytes of the rows of q, k, v / of out, gout
+    float *lse, *delta;        // [B, Hq, L]
+    float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
+    int chunks;
+};
+// [begin[b], end[b]) cut to the row, whatever the arrays hold
+__device__ __forceinline__ void history(const int32_t* begin, const int32_t* end, int b, int L, int& lo, int& hi) {
+    lo = begin ? begin[b] : 0;
+    hi = end ? end[b] : L;
+    lo = lo < 0 ? 0 : (lo > L ? L : lo);
+    hi = hi < 0 ? 0 : (hi > L ? L : hi);
+}
+__device__ __forceinline__ void win_range(const WinArgs& a, int b, int& lo, int& hi) {
+    history(a.begin, a.end, b, a.L, lo, hi);
+}
+__device__ __forceinline__ bool win_visible(const WinArgs& a, int q, int k, int lo) {
+    return k >= lo && k <= q && (q - k < a.W || k - lo < a.S);
+}
+
+// ---- staging of a 32-row tile by 256 threads: rows row0 .. row0 + 31 of the sequence, those outside [lo, hi) as zeros ----
+template <class T, int DP>
+struct Stage {
+    static constexpr int OCTS = WA_BK * DP / 8, N = (OCTS + 255) / 256, LD = lds_ld<T, DP>();
+    Oct<T> r[N];
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int lo, int hi, int D, int al) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int o = (int)threadIdx.x + n * 256, row = row0 + o / (DP / 8), c = o % (DP / 8) * 8;
+            if ((OCTS % 256 == 0 || o < OCTS) && row >= lo && row < hi && c < D)
+                r[n] = load_oct<T>(base + row * ld + c, D - c, al);
+            else
+                r[n] = zero_oct<T>();
+        }
+    }
+    __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int o = (int)threadIdx.x + n * 256;
+            if (OCTS % 256 == 0 || o < OCTS) lds_store_oct<T>(tile + o / (DP / 8) * LD + o % (DP / 8) * 8, r[n]);
+        }
+    }
+};
+// the row fragments of 16 rows (lane & 15) straight from memory
+template <class T, int DP>
+__device__ __forceinline__ void load_frags(Oct<T> (&f)[DP / 32], const T* row, bool ok, int D, int al) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+        const int c = 32 * s + 8 * g;
+        f[s] = ok && c < D ? load_oct<T>(row + c, D - c, al) : zero_oct<T>();
+    }
+}
+// which key tiles a block of queries [qlo, qhi] needs: the tiles of the first items, then those of the window
+struct KeyTiles {
+    int s0, ns, w0, n;
+    __device__ __forceinline__ void set(const WinArgs& a, int qlo, int qhi, int lo) {
+        ns = n = 0;
+        s0 = w0 = 0;
+        if (qlo > qhi) return;
+        const int first = qlo - a.W + 1 > lo ? qlo - a.W + 1 : lo;      // W <= L: no overflow
+        w0 = first / WA_BK;
+        if (a.S > 0) {
+            s0 = lo / WA_BK;
+            int s1 = (lo + a.S - 1) / WA_BK;
+            if (s1 >= w0) s1 = w0 - 1;
+            ns = s1 >= s0 ? s1 - s0 + 1 : 0;
+        }
+        n = ns + qhi / WA_BK - w0 + 1;
+    }
+    __device__ __forceinline__ int row0(int i) const { return (i < ns ? s0 + i : w0 + i - ns) * WA_BK; }
+};
+
+// ---- forward ---------------------------------------------------------------------------------------------------------------
+// A workgroup of 4 wavefronts takes 64 queries of one head; the key and value tiles it needs go through LDS, the next
+// tile's loads in flight while one is used (two buffers; one where two would not leave room for a second workgroup).
+template <class T, int DP>
+constexpr int fwd_buffers() {
+    return DP * (int)sizeof(T) <= 512 ? 2 : 1;
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__ out, float* __restrict__ lse) {
+    constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
+    extern __shared__ char smem[];
+    T* kt = reinterpret_cast<T*>(smem);
+    T* vt = kt + NB * TILE;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const int q0 = (int)(blockIdx.x % a.tiles) * 64, h = (int)(blockIdx.x / a.tiles % a.Hq);
+    const int b = (int)(blockIdx.x / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
+    int lo, hi;
+    win_range(a, b, lo, hi);
+    const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
+    const T* vp = (const T*)a.v + b * a.vs.b + hk * a.vs.h;
+    const int qw = q0 + wave * 16, qi = qw + c16;
+    const bool q_ok = qi >= lo && qi < hi;
+    const int qlo = qw > lo ? qw : lo, qhi = qw + 15 < hi - 1 ? qw + 15 : hi - 1;      // this wavefront's queries
+    Oct<T> qf[DP / 32];
+    load_frags<T, DP>(qf, (const T*)a.q + b * a.qs.b + qi * a.qs.l + h * a.qs.h, q_ok, a.D, a.al);
+    KeyTiles kts;
+    kts.set(a, q0 > lo ? q0 : lo, q0 + 63 < hi - 1 ? q0 + 63 : hi - 1, lo);
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
+    float m = -__builtin_inff(), l = 0.0f;
+    const float c = a.scale * WA_LOG2E;
+    Stage<T, DP> ks, vs;
+    if (kts.n > 0) {
+        ks.load(kp, a.ks.l, kts.row0(0), lo, hi, a.D, a.al);
+        vs.load(vp, a.vs.l, kts.row0(0), lo, hi, a.D, a.al);
+        ks.store(kt);
+        vs.store(vt);
+    }
+    __syncthreads();
+    for (int n = 0; n < kts.n; ++n) {
+        const int t0 = kts.row0(n);
+        const T* kc = kt + (NB == 2 ? (n & 1) * TILE : 0);
+        const T* vc = vt + (NB == 2 ? (n & 1) * TILE : 0);
+        if (n + 1 < kts.n) {
+            ks.load(kp, a.ks.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+            vs.load(vp, a.vs.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+        }
+        if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x) {
+                s[0] = mma(row_frag<T>(kc + c16 * LD + 32 * x + 8 * g), qf[x], s[0]);
+                s[1] = mma(row_frag<T>(kc + (16 + c16) * LD + 32 * x + 8 * g), qf[x], s[1]);
+            }
+            // a tile that all 16 queries see whole needs no mask
+            const bool whole = t0 >= lo && t0 + WA_BK - 1 <= qw && qw >= lo && qw + 15 < hi && qw + 15 - t0 < a.W;
+            if (!whole) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(q_ok && win_visible(a, qi, t0 + 16 * x + 4 * g + i, lo))) s[x][i] = -__builtin_inff();
+            }
+            float mt = s[0][0];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[x][i]);
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const float mn = fmaxf(m, mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
+            m = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[x][i] = __builtin_amdgcn_exp2f((s[x][i] - ms) * c);
+                    sum += s[x][i];
+                }
+            l = fmaf(l, alpha, sum);
+            if (__ballot(alpha != 1.0f) != 0) {
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) o[t] *= alpha;
+            }
+            const Oct<T> p = to_oct<T>(s[0], s[1]);
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) o[t] = mma(col_frag<T, LD>(vc, 16 * t), p, o[t]);
+        }
+        if (NB == 1) __syncthreads();
+        if (n + 1 < kts.n) {
+            ks.store(kt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
+            vs.store(vt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (qi >= a.L) return;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    T* op = out + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        const int d = 16 * t + 4 * g;
+        if (d + 4 <= a.D && a.alg >= 4 * (int)sizeof(T)) {
+            float r[4] = {o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv};
+            store_f32<T, 4>(op + d, r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (d + i < a.D) op[d + i] = (T)(o[t][i] * inv);
+        }
+    }
+    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l > 0.0f ? fmaf(m, a.scale, logf(l)) : -__builtin_inff();
+}
+
+// ---- backward: dQ ------------------------------------------------------------------------------------------------------------
+// delta_i = <dO_i, O_i>;  dS = P (dP - delta) scale;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the others.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void win_dq_kernel(WinArgs a, T* __restrict__ dq) {
+    constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
+    extern __shared__ char smem[];
+    T* kt = reinterpret_cast<T*>(smem);
+    T* vt = kt + NB * TILE;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const int q0 = (int)(blockIdx.x % a.tiles) * 64, h = (int)(blockIdx.x / a.tiles % a.Hq);
+    const int b = (int)(blockIdx.x / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
+    int lo, hi;
+    win_range(a, b, lo, hi);
+    const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
+    const T* vp = (const T*)a.v + b * a.vs.b + hk * a.vs.h;
+    const int qw = q0 + wave * 16, qi = qw + c16;
+    const bool q_ok = qi >= lo && qi < hi;
+    const int qlo = qw > lo ? qw : lo, qhi = qw + 15 < hi - 1 ? qw + 15 : hi - 1;
+    Oct<T> qf[DP / 32], gf[DP / 32];
+    load_frags<T, DP>(qf, (const T*)a.q + b * a.qs.b + qi * a.qs.l + h * a.qs.h, q_ok, a.D, a.al);
+    const int64_t orow = (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
+    load_frags<T, DP>(gf, (const T*)a.gout + orow, q_ok, a.D, a.alg);
+    float delta = 0.0f;
+    {
+        Oct<T> of[DP / 32];
+        load_frags<T, DP>(of, (const T*)a.out + orow, q_ok, a.D, a.alg);
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[s][e], delta);
+    }
+    delta += __shfl_xor(delta, 16, 64);
+    delta += __shfl_xor(delta, 32, 64);
+    const int64_t srow = ((int64_t)b * a.Hq + h) * a.L + qi;
+    float lse2 = 0.0f;                                       // in units of log 2
+    if (qi < a.L) {
+        if (q_ok) lse2 = a.lse[srow] * WA_LOG2E;
+        if (g == 0) a.delta[srow] = delta;
+    }
+    KeyTiles kts;
+    kts.set(a, q0 > lo ? q0 : lo, q0 + 63 < hi - 1 ? q0 + 63 : hi - 1, lo);
+    f32x4 acc[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
+    const float c = a.scale * WA_LOG2E;
+    Stage<T, DP> ks, vs;
+    if (kts.n > 0) {
+        ks.load(kp, a.ks.l, kts.row0(0), lo, hi, a.D, a.al);
+        vs.load(vp, a.vs.l, kts.row0(0), lo, hi, a.D, a.al);
+        ks.store(kt);
+        vs.store(vt);
+    }
+    __syncthreads();
+    for (int n = 0; n < kts.n; ++n) {
+        const int t0 = kts.row0(n);
+        const T* kc = kt + (NB == 2 ? (n & 1) * TILE : 0);
+        const T* vc = vt + (NB == 2 ? (n & 1) * TILE : 0);
+        if (n + 1 < kts.n) {
+            ks.load(kp, a.ks.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+            vs.load(vp, a.vs.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+        }
+        if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    s[y] = mma(row_frag<T>(kc + (16 * y + c16) * LD + 32 * x + 8 * g), qf[x], s[y]);
+                    dp[y] = mma(row_frag<T>(vc + (16 * y + c16) * LD + 32 * x + 8 * g), gf[x], dp[y]);
+                }
+            const bool whole = t0 >= lo && t0 + WA_BK - 1 <= qw && qw >= lo && qw + 15 < hi && qw + 15 - t0 < a.W;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -lse2));
+                    if (!whole && !(q_ok && win_visible(a, qi, t0 + 16 * y + 4 * g + i, lo))) p = 0.0f;
+                    s[y][i] = p == 0.0f ? 0.0f : p * (dp[y][i] - delta) * a.scale;
+                }
+            const Oct<T> ds = to_oct<T>(s[0], s[1]);
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) acc[t] = mma(col_frag<T, LD>(kc, 16 * t), ds, acc[t]);
+        }
+        if (NB == 1) __syncthreads();
+        if (n + 1 < kts.n) {
+            ks.store(kt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
+            vs.store(vt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
+        }
+        __syncthreads();
+    }
+    if (qi >= a.L) return;
+    T* op = dq + orow;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        const int d = 16 * t + 4 * g;
+        if (d + 4 <= a.D && a.alg >= 4 * (int)sizeof(T)) {
+            float r[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+            store_f32<T, 4>(op + d, r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (d + i < a.D) op[d + i] = (T)acc[t][i];
+        }
+    }
+}
+
+// ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
+// S = Q K^T here, so a lane holds one KEY and four queries of each 16: the A operand of dV = P^T dO and dK = dS^T Q.
+// one (32 queries x 16 keys) step: adds to dk, dv.  far: only what the sinks see beyond the window; else only the window.
+template <class T, int DP>
+__device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* lse2, const float* delta,
+                                          const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int ki, int lo,
+                                          int hi, bool far, bool whole, f32x4 (&dk)[DP / 16], f32x4 (&dv)[DP / 16]) {
+    constexpr int LD = lds_ld<T, DP>();
+    const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const float c = a.scale * WA_LOG2E;
+    f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            s[y] = mma(row_frag<T>(qc + (16 * y + c16) * LD + 32 * x + 8 * g), kf[x], s[y]);
+            dp[y] = mma(row_frag<T>(gc + (16 * y + c16) * LD + 32 * x + 8 * g), vf[x], dp[y]);
+        }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(lse2 + 16 * y + 4 * g);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 16 * y + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int qi = t0 + 16 * y + 4 * g + i, gap = qi - ki;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i]));
+            if (!whole) {
+                const bool seen = far ? (gap >= a.W && ki - lo < a.S) : (gap >= 0 && gap < a.W);
+                if (!(seen && ki >= lo && qi < hi)) p = 0.0f;
+            }
+            s[y][i] = p;
+            dp[y][i] = p == 0.0f ? 0.0f : p * (dp[y][i] - de[i]) * a.scale;
+        }
+    }
+    const Oct<T> pf = to_oct<T>(s[0], s[1]), df = to_oct<T>(dp[0], dp[1]);
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
+        dk[t] = mma(df, col_frag<T, LD>(qc, 16 * t), dk[t]);
+    }
+}
+
+// A workgroup takes 64 keys of one key head and walks the queries that see them through the window, head by head of the
+// group (so the group's sum needs no atomics); what the first items get from queries beyond the window comes from
+// win_sink_kernel's partial sums, added last and in order.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void win_dkdv_kernel(WinArgs a, T* __restrict__ dk_out, T* __restrict__ dv_out) {
+    constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
+    extern __shared__ char smem[];
+    T* qt = reinterpret_cast<T*>(smem);
+    T* gt = qt + NB * TILE;
+    float* st = reinterpret_cast<float*>(gt + NB * TILE);    // [NB][2][32]: lse2, delta
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const int k0 = (int)(blockIdx.x % a.tiles) * 64, hk = (int)(blockIdx.x / a.tiles % a.Hkv);
+    const int b = (int)(blockIdx.x / a.tiles / a.Hkv), G = a.Hq / a.Hkv;
+    int lo, hi;
+    win_range(a, b, lo, hi);
+    const int kw = k0 + wave * 16, ki = kw + c16;
+    const bool k_ok = ki >= lo && ki < hi;
+    Oct<T> kf[DP / 32], vf[DP / 32];
+    load_frags<T, DP>(kf, (const T*)a.k + b * a.ks.b + ki * a.ks.l + hk * a.ks.h, k_ok, a.D, a.al);
+    load_frags<T, DP>(vf, (const T*)a.v + b * a.vs.b + ki * a.vs.l + hk * a.vs.h, k_ok, a.D, a.al);
+    f32x4 dk[DP / 16], dv[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
+    const int klo = k0 > lo ? k0 : lo, khi = k0 + 63 < hi - 1 ? k0 + 63 : hi - 1;
+    const int qend = klo <= khi ? (khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1) : -1;   // last query
+    const int tq0 = klo / WA_BK, nt = klo <= khi ? qend / WA_BK - tq0 + 1 : 0, total = nt * G;
+    Stage<T, DP> qs, gs;
+    float stat = 0.0f;
+    auto load = [&](int n) {
+        const int h = hk * G + n / nt, t0 = (tq0 + n % nt) * WA_BK;
+        qs.load((const T*)a.q + b * a.qs.b + h * a.qs.h, a.qs.l, t0, lo, hi, a.D, a.al);
+        gs.load((const T*)a.gout + ((int64_t)b * a.L * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, t0, lo, hi, a.D, a.alg);
+        if (threadIdx.x < 64) {
+            const int qi = t0 + (int)(threadIdx.x & 31);
+            const int64_t row = ((int64_t)b * a.Hq + h) * a.L + qi;
+            stat = 0.0f;
+            if (qi >= lo && qi < hi) stat = threadIdx.x < 32 ? a.lse[row] * WA_LOG2E : a.delta[row];
+        }
+    };
+    auto store = [&](int buf) {
+        qs.store(qt + buf * TILE);
+        gs.store(gt + buf * TILE);
+        if (threadIdx.x < 64) st[buf * 64 + threadIdx.x] = stat;
+    };
+    if (total > 0) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int n = 0; n < total; ++n) {
+        const int t0 = (tq0 + n % nt) * WA_BK, buf = NB == 2 ? n & 1 : 0;
+        if (n + 1 < total) load(n + 1);
+        if (kw <= t0 + WA_BK - 1 && t0 - (kw + 15) < a.W && kw < hi && kw + 15 >= lo) {
+            const bool whole = kw >= lo && kw + 15 <= t0 && t0 + WA_BK - 1 < hi && t0 + WA_BK - 1 - kw < a.W;
+            dkdv_step<T, DP>(a, qt + buf * TILE, gt + buf * TILE, st + buf * 64, st + buf * 64 + 32, kf, vf, t0, ki, lo, hi,
+                             false, whole, dk, dv);
+        }
+        if (NB == 1) __syncthreads();
+        if (n + 1 < total) store(NB == 2 ? (n + 1) & 1 : 0);
+        __syncthreads();
+    }
+    // lane: column d = 16 t + c16 of keys kw + 4 g + i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int kk = kw + 4 * g + i;
+        if (kk >= a.L) continue;
+        const bool sink = a.chunks > 0 && kk >= lo && kk < hi && kk - lo < a.S;
+        T* ko = dk_out + (((int64_t)b * a.L + kk) * a.Hkv + hk) * a.D;
+        T* vo = dv_out + (((int64_t)b * a.L + kk) * a.Hkv + hk) * a.D;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            const int d = 16 * t + c16;
+            if (d >= a.D) continue;
+            float x = dk[t][i], y = dv[t][i];
+            if (sink) {
+                const int64_t step = 2 * (int64_t)a.S * a.D;
+                const float* p = a.part + ((int64_t)b * a.Hkv + hk) * a.chunks * step + (int64_t)(kk - lo) * a.D + d;
+                for (int q = 0; q < a.chunks; ++q) {
+                    x += p[q * step];
+                    y += p[q * step + (int64_t)a.S * a.D];
+                }
+            }
+            ko[d] = (T)x;
+            vo[d] = (T)y;
+        }
+    }
+}
+
+// ---- backward: what the first items get from queries beyond the window ----------------------------------------------------------
+// Every query of a long history sees them, so their sums are split over chunks of 256 queries: NW wavefronts, each with its
+// own tiles of 32 queries in LDS, all on the same 16 first items, added up over LDS in order.
+constexpr int WA_CHUNK = 256;
+template <class T, int DP>
+constexpr int sink_waves() {
+    return DP * (int)sizeof(T) <= 256 ? 4 : (DP * (int)sizeof(T) <= 512 ? 2 : 1);
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
+    constexpr int LD = lds_ld<T, DP>(), TILE = WA_BK * LD, NW = sink_waves<T, DP>();
+    extern __shared__ char smem[];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    T* qt = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
+    T* gt = qt + TILE;
+    float* st = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + NW * 2 * TILE) + wave * 64;
+    const int groups = (a.S + 15) / 16;
+    int id = (int)blockIdx.x;
+    const int grp = id % groups;
+    id /= groups;
+    const int chunk = id % a.chunks;
+    id /= a.chunks;
+    const int hk = id % a.Hkv, b = id / a.Hkv, G = a.Hq / a.Hkv;
+    int lo, hi;
+    win_range(a, b, lo, hi);
+    const int kw = lo + grp * 16, ki = kw + c16;
+    const bool k_ok = ki < hi && ki - lo < a.S;
+    Oct<T> kf[DP / 32], vf[DP / 32];
+    load_frags<T, DP>(kf, (const T*)a.k + b * a.ks.b + ki * a.ks.l + hk * a.ks.h, k_ok, a.D, a.al);
+    load_frags<T, DP>(vf, (const T*)a.v + b * a.vs.b + ki * a.vs.l + hk * a.vs.h, k_ok, a.D, a.al);
+    f32x4 dk[DP / 16], dv[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
+    const int first = chunk * WA_CHUNK, per = WA_CHUNK / WA_BK;
+    for (int n = wave; n < per * G; n += NW) {
+        const int h = hk * G + n / per, t0 = first + n % per * WA_BK;
+        // wavefront-uniform: no query of the tile is both in the history and beyond the window of the group's first key
+        if (t0 >= hi || t0 + WA_BK - 1 - kw < a.W) continue;
+        const T* qp = (const T*)a.q + b * a.qs.b + h * a.qs.h;
+        const T* gp = (const T*)a.gout + ((int64_t)b * a.L * a.Hq + h) * a.D;
+        for (int o = lane; o < WA_BK * DP / 8; o += 64) {
+            const int r = o / (DP / 8), cc = o % (DP / 8) * 8, row = t0 + r;
+            const bool ok = row >= lo && row < hi && cc < a.D;
+            lds_store_oct<T>(qt + r * LD + cc, ok ? load_oct<T>(qp + row * a.qs.l + cc, a.D - cc, a.al) : zero_oct<T>());
+            lds_store_oct<T>(gt + r * LD + cc, ok ? load_oct<T>(gp + (int64_t)row * a.Hq * a.D + cc, a.D - cc, a.alg) : zero_oct<T>());
+        }
+        {
+            const int qi = t0 + (lane & 31);
+            const int64_t row = ((int64_t)b * a.Hq + h) * a.L + qi;
+            float x = 0.0f;
+            if (qi >= lo && qi < hi) x = lane < 32 ? a.lse[row] * WA_LOG2E : a.delta[row];
+            st[lane] = x;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki, lo, hi, true, false, dk, dv);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the wavefronts' sums in order through LDS (the tiles are done with), then to this chunk's slot
+    const int64_t step = 2 * (int64_t)a.S * a.D;
+    float* part = a.part + (((int64_t)b * a.Hkv + hk) * a.chunks + chunk) * step;
+    float* red = reinterpret_cast<float*>(smem);             // [16][DP]
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        for (int w = 0; w < NW; ++w) {
+            __syncthreads();
+            if (wave == w) {
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float* r = red + (4 * g + i) * DP + 16 * t + c16;
+                        const float x = which ? dv[t][i] : dk[t][i];
+                        *r = w == 0 ? x : *r + x;
+                    }
+            }
+        }
+        __syncthreads();
+        for (int o = threadIdx.x; o < 16 * DP; o += NW * 64) {
+            const int r = o / DP, d = o % DP;
+            if (grp * 16 + r < a.S && d < a.D) part[(int64_t)which * a.S * a.D + (int64_t)(grp * 16 + r) * a.D + d] = red[o];
+        }
+    }
+}
+
+// ---- one new token per sequence over a cache -----------------------------------------------------------------------------------
+// The query stands at position end - 1 and sees the first items and the window before it.  A workgroup takes one key head
+// (its up to 16 query heads are the 16 columns of the tile) and a share of the visible keys; its wavefronts take 32 keys
+// in turn, keys straight into registers, values through their own LDS tile, and are joined at the end.  With few sequences
+// the keys are split over workgroups and win_join_kernel adds up.
+struct TokenArgs {
+    const void *q, *k, *v;
+    int64_t qb, qh;
+    WinStride ks, vs;
+    int B, L, Hq, Hkv, D, W, S, splits, per, hgroups;   // per: 32-key tiles of a workgroup
+    float scale;
+    const int32_t *begin, *end;
+    int al, alq;
+    void* out;                                          // [B, Hq, D]
+    float* part;                                        // [B, Hq, splits, D + 2]: sum, m, l
+};
+template <class T, int DP>
+constexpr int token_waves() {
+    return DP * (int)sizeof(T) <= 256 ? 4 : (DP * (int)sizeof(T) <= 512 ? 2 : 1);
+}
+template <class T, int DP>
+__global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
+    constexpr int LD = lds_ld<T, DP>(), TILE = WA_BK * LD, NW = token_waves<T, DP>();
+    __shared__ __attribute__((aligned(16))) T tiles[NW * TILE];
+    __shared__ float sm[NW][16], sl[NW][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    T* vt = tiles + wave * TILE;
+    int id = (int)blockIdx.x;
+    const int sp = id % a.splits;
+    id /= a.splits;
+    const int hg = id % a.hgroups;
+    id /= a.hgroups;
+    const int hk = id % a.Hkv, b = id / a.Hkv, G = a.Hq / a.Hkv;
+    int lo, hi;
+    history(a.begin, a.end, b, a.L, lo, hi);
+    const int first = hi - a.W > lo ? hi - a.W : lo;                       // window: [first, hi)
+    int ns = first - lo < a.S ? first - lo : a.S;                          // first items before it
+    if (hi <= lo) ns = 0;
+    const int total = hi > lo ? ns + hi - first : 0;
+    const int hq = hg * 16 + c16;                                          // query head inside the group
+    Oct<T> qf[DP / 32];
+    load_frags<T, DP>(qf, (const T*)a.q + b * a.qb + (hk * G + hq) * a.qh, hq < G && total > 0, a.D, a.alq);
+    const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
+    const T* vp = (const T*)a.v + b * a.vs.b + hk * a.vs.h;
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
+    float m = -__builtin_inff(), l = 0.0f;
+    const float c = a.scale * WA_LOG2E;
+    const int t_end = (sp + 1) * a.per;
+    for (int t = sp * a.per + wave; t < t_end && t * WA_BK < total; t += NW) {
+        const int n0 = t * WA_BK;
+        auto pos = [&](int n) { return (int64_t)(n < ns ? lo + n : first + n - ns); };
+        Oct<T> kf[2][DP / 32];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int n = n0 + 16 * y + c16;
+            load_frags<T, DP>(kf[y], kp + pos(n < total ? n : total - 1) * a.ks.l, n < total, a.D, a.al);
+        }
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+            const int oo = lane + 64 * x, r = oo / (DP / 8), cc = oo % (DP / 8) * 8, n = n0 + r;
+            const bool ok = n < total && cc < a.D;
+            lds_store_oct<T>(vt + r * LD + cc, ok ? load_oct<T>(vp + pos(n) * a.vs.l + cc, a.D - cc, a.al) : zero_oct<T>());
+        }
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) s[y] = mma(kf[y][x], qf[x], s[y]);
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (n0 + 16 * y + 4 * g + i >= total) s[y][i] = -__builtin_inff();
+                mt = fmaxf(mt, s[y][i]);
+            }
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        const float mn = fmaxf(m, mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
+        const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
+        m = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[y][i] = __builtin_amdgcn_exp2f((s[y][i] - ms) * c);
+                sum += s[y][i];
+            }
+        l = fmaf(l, alpha, sum);
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) o[x] *= alpha;
+        const Oct<T> p = to_oct<T>(s[0], s[1]);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) o[x] = mma(col_frag<T, LD>(vt, 16 * x), p, o[x]);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    // join the wavefronts: common maximum, then sums in order
+    if (g == 0) {
+        sm[wave][c16] = m;
+        sl[wave][c16] = l;
+    }
+    __syncthreads();
+    float mx = sm[0][c16];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, sm[w][c16]);
+    const float ms = mx == -__builtin_inff() ? 0.0f : mx;
+    const float f = __builtin_amdgcn_exp2f((m - ms) * c);
+    float lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) lt += sl[w][c16] * __builtin_amdgcn_exp2f((sm[w][c16] - ms) * c);
+    float* red = reinterpret_cast<float*>(tiles);                          // [16 heads][DP] fp32: 64 DP bytes of the tiles
+#pragma unroll 1
+    for (int w = 0; w < NW; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float* r = red + c16 * DP + 16 * x + 4 * g + i;
+                    *r = w == 0 ? o[x][i] * f : *r + o[x][i] * f;
+                }
+        }
+        __syncthreads();
+    }
+    if (wave == 0 && g == 0) {
+        sm[0][c16] = mx;
+        sl[0][c16] = lt;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * DP; e += NW * 64) {
+        const int r = e / DP, d = e % DP, hh = hg * 16 + r;
+        if (hh >= G || d >= a.D) continue;
+        const int64_t row = (int64_t)b * a.Hq + hk * G + hh;
+        const float lr = sl[0][r];
+        if (a.splits == 1) {
+            ((T*)a.out)[row * a.D + d] = (T)(lr > 0.0f ? red[e] / lr : 0.0f);
+        } else {
+            float* p = a.part + (row * a.splits + sp) * (a.D + 2);
+            p[d] = red[e];
+            if (d == 0) {
+                p[a.D] = sm[0][r];
+                p[a.D + 1] = lr;
+            }
+        }
+    }
+}
+template <class T>
+__global__ __launch_bounds__(64) void win_join_kernel(const float* __restrict__ part, int splits, int D, float scale,
+                                                      T* __restrict__ out) {
+    const float* p = part + (int64_t)blockIdx.x * splits * (D + 2);
+    const float c = scale * WA_LOG2E;
+    float m = -__builtin_inff();
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, p[s * (D + 2) + D]);
+    const float ms = m == -__builtin_inff() ? 0.0f : m;
+    for (int d = threadIdx.x; d < D; d += 64) {
+        float l = 0.0f, o = 0.0f;
+        for (int s = 0; s < splits; ++s) {
+            const float f = __builtin_amdgcn_exp2f((p[s * (D + 2) + D] - ms) * c);
+            l = fmaf(p[s * (D + 2) + D + 1], f, l);
+            o = fmaf(p[s * (D + 2) + d], f, o);
+        }
+        out[(int64_t)blockIdx.x * D + d] = (T)(l > 0.0f ? o / l : 0.0f);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------
+// largest of 16, 8, 4, 2 bytes that divides every row start
+static int row_alignment(int es, std::initializer_list<const void*> bases, std::initializer_list<int64_t> strides) {
+    uint64_t bits = 16;
+    for (const void* p : bases) bits |= (uint64_t)(uintptr_t)p;
+    for (int64_t s : strides) bits |= (uint64_t)(s * es);
+    return (int)(bits & (~bits + 1)) > 16 ? 16 : (int)(bits & (~bits + 1));
+}
+static int win_check(const char* who, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype, int64_t window,
+                     int32_t sinks, float scale) {
+    DR_REQUIRE(dtype_ok(dtype), "%s: dtype %d", who, dtype);
+    DR_REQUIRE(B >= 0 && L >= 1 && L < (1 << 30) && Hq >= 1 && Hkv >= 1 && Hq <= 65536 && Hq % Hkv == 0 && D >= 1 &&
+                   D <= WA_MAX_D && B < (1 << 30),
+               "%s: bad sizes (B=%lld L=%lld Hq=%d Hkv=%d D=%d)", who, (long long)B, (long long)L, Hq, Hkv, D);
+    DR_REQUIRE(window >= 1 && sinks >= 0 && sinks <= WA_MAX_SINKS, "%s: window=%lld (>= 1), sinks=%d (0..%d)", who,
+               (long long)window, sinks, WA_MAX_SINKS);
+    DR_REQUIRE(scale > 0.0f && scale <= 3.402823466e38f, "%s: scale must be positive and finite", who);
+    return DR_OK;
+}
+template <class Kernel>
+static int win_lds(Kernel k, size_t bytes) {
+    if (bytes > 65536)
+        DR_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return DR_OK;
+}
+static int64_t win_chunks(int64_t L, int64_t window, int32_t sinks) {
+    return sinks > 0 && L > window ? (L + WA_CHUNK - 1) / WA_CHUNK : 0;
+}
+
+template <class T, int DP>
+static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
+    const size_t lds = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
+    int rc = win_lds(win_fwd_kernel<T, DP>, lds);
+    if (rc != DR_OK) return rc;
+    DR_LAUNCH_NAMED("win_fwd_kernel", (win_fwd_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), lds, st, a,
+                    (T*)out, a.lse);
+    DR_CHECK_LAUNCH("win_fwd_kernel");
+    return DR_OK;
+}
+template <class T, int DP>
+static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStream_t st) {
+    const size_t tiles = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
+    const size_t lds = tiles + fwd_buffers<T, DP>() * 64 * sizeof(float);
+    int rc = win_lds(win_dq_kernel<T, DP>, tiles);
+    if (rc != DR_OK) return rc;
+    DR_LAUNCH_NAMED("win_dq_kernel", (win_dq_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), tiles, st, a,
+                    (T*)dq);
+    DR_CHECK_LAUNCH("win_dq_kernel");
+    if (a.chunks > 0) {
+        constexpr int NW = sink_waves<T, DP>();
+        const size_t sl = (size_t)NW * (2 * WA_BK * lds_ld<T, DP>() * sizeof(T) + 64 * sizeof(float));
+        rc = win_lds(win_sink_kernel<T, DP>, sl);
+        if (rc != DR_OK) return rc;
+        DR_LAUNCH_NAMED("win_sink_kernel", (win_sink_kernel<T, DP>), dim3((unsigned)((a.S + 15) / 16) * a.chunks * a.Hkv * a.B),
+                        dim3(NW * 64), sl, st, a);
+        DR_CHECK_LAUNCH("win_sink_kernel");
+    }
+    rc = win_lds(win_dkdv_kernel<T, DP>, lds);
+    if (rc != DR_OK) return rc;
+    DR_LAUNCH_NAMED("win_dkdv_kernel", (win_dkdv_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hkv * a.B), dim3(256), lds, st, a,
+                    (T*)dk, (T*)dv);
+    DR_CHECK_LAUNCH("win_dkdv_kernel");
+    return DR_OK;
+}
+template <class T, int DP>
+static int win_token_launch(const TokenArgs& a, hipStream_t st) {
+    DR_LAUNCH_NAMED("win_token_kernel", (win_token_kernel<T, DP>), dim3((unsigned)a.splits * a.hgroups * a.Hkv * a.B),
+                    dim3(64 * token_waves<T, DP>()), 0, st, a);
+    DR_CHECK_LAUNCH("win_token_kernel");
+    if (a.splits > 1) {
+        DR_LAUNCH_NAMED("win_join_kernel", (win_join_kernel<T>), dim3((unsigned)(a.B * a.Hq)), dim3(64), 0, st,
+                        (const float*)a.part, a.splits, a.D, a.scale, (T*)a.out);
+        DR_CHECK_LAUNCH("win_join_kernel");
+    }
+    return DR_OK;
+}
+// workgroups per sequence and key head, 32-key tiles each: 2 workgroups per CU, none below 128 keys
+static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int* splits, int* per) {
+    const int64_t tiles = (keys + WA_BK - 1) / WA_BK, rows = B * Hkv * hgroups;
+    int64_t s = (512 + rows - 1) / rows;
+    if (s > tiles / 4) s = tiles / 4;
+    if (s > 128) s = 128;
+    if (s < 1) s = 1;
+    *per = (int)((tiles + s - 1) / s);
+    *splits = (int)((tiles + *per - 1) / *per);
+}
+static int64_t token_keys(int64_t L, int64_t window, int32_t sinks) { return window >= L ? L : (window + sinks < L ? window + sinks : L); }
+
+#define WIN_BY_D(T, launch, ...)                                    \
+    return a.D <= 32    ? launch<T, 32>(__VA_ARGS__)                \
+           : a.D <= 64  ? launch<T, 64>(__VA_ARGS__)                \
+           : a.D <= 128 ? launch<T, 128>(__VA_ARGS__)               \
+                        : launch<T, 256>(__VA_ARGS__)
+}  // namespace dr
+
+extern "C" int32_t dr_window_attn_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                          const void* v, const int64_t* v_strides, int64_t B, int64_t L, int32_t Hq,
+                                          int32_t Hkv, int32_t D, int32_t dtype, int64_t window, int32_t sinks, float scale,
+                                          const int32_t* begin, const int32_t* end, void* out, float* lse, void* stream) {
+    using namespace dr;
+    int rc = win_check("dr_window_attn_forward", B, L, Hq, Hkv, D, dtype, window, sinks, scale);
+    if (rc != DR_OK) return rc;
+    if (B == 0) return DR_OK;
+    DR_REQUIRE(q && k && v && out && lse && q_strides && k_strides && v_strides, "dr_window_attn_forward: NULL pointer");
+    const int es = dtype_size(dtype);
+    WinArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.qs = WinStride{q_strides[0], q_strides[1], q_strides[2]};
+    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
+    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.B = (int)B;
+    a.L = (int)L;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.D = D;
+    a.W = (int)(window < L ? window : L);
+    a.S = sinks;
+    a.scale = scale;
+    a.begin = begin;
+    a.end = end;
+    a.lse = lse;
+    a.tiles = (int)((L + 63) / 64);
+    DR_REQUIRE((int64_t)a.tiles * Hq * B < (1ll << 31), "dr_window_attn_forward: too many workgroups");
+    a.al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    a.alg = row_alignment(es, {out}, {(int64_t)D});
+    DR_REQUIRE(a.al >= es && a.alg >= es, "dr_window_attn_forward: a pointer is not aligned to its element size");
+    hipStream_t st = (hipStream_t)stream;
+#define WIN_FWD(T) WIN_BY_D(T, win_fwd_launch, a, out, st)
+    DR_BY_DTYPE(dtype, WIN_FWD);
+#undef WIN_FWD
+}
+
+extern "C" int64_t dr_window_attn_backward_bytes(int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int64_t window,
+                                                 int32_t sinks) {
+    using namespace dr;
+    int rc = win_check("dr_window_attn_backward_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
+    if (rc != DR_OK) return rc;
+    return align_up(B * Hq * L * 4, 256) + align_up(B * Hkv * win_chunks(L, window, sinks) * 2 * sinks * D * 4, 256) + 256;
+}
+
+extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                           const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                           const void* gout, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D,
+                                           int32_t dtype, int64_t window, int32_t sinks, float scale, const int32_t* begin,
+                                           const int32_t* end, void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes,
+                                           void* stream) {
+    using namespace dr;
+    int rc = win_check("dr_window_attn_backward", B, L, Hq, Hkv, D, dtype, window, sinks, scale);
+    if (rc != DR_OK) return rc;
+    if (B == 0) return DR_OK;
+    DR_REQUIRE(q && k && v && out && lse && gout && dq && dk && dv && q_strides && k_strides && v_strides,
+               "dr_window_attn_backward: NULL pointer");
+    DR_REQUIRE(ws && aligned_to(ws, 256), "dr_window_attn_backward: workspace is NULL or not 256-byte aligned");
+    const int64_t need = dr_window_attn_backward_bytes(B, L, Hq, Hkv, D, window, sinks);
+    if (ws_bytes < need)
+        DR_FAIL(DR_ERR_WORKSPACE, "dr_window_attn_backward: workspace %lld < required %lld", (long long)ws_bytes, (long long)need);
+    const int es = dtype_size(dtype);
+    WinArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.gout = gout;
+    a.qs = WinStride{q_strides[0], q_strides[1], q_strides[2]};
+    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
+    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.B = (int)B;
+    a.L = (int)L;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.D = D;
+    a.W = (int)(window < L ? window : L);
+    a.S = sinks;
+    a.scale = scale;
+    a.begin = begin;
+    a.end = end;
+    a.lse = const_cast<float*>(lse);
+    a.delta = (float*)ws;
+    a.part = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
+    a.chunks = (int)win_chunks(L, window, sinks);
+    a.tiles = (int)((L + 63) / 64);
+    DR_REQUIRE((int64_t)a.tiles * Hq * B < (1ll << 31) && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < (1ll << 31),
+               "dr_window_attn_backward: too many workgroups");
+    a.al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    a.alg = row_alignment(es, {out, gout, dq}, {(int64_t)D});
+    DR_REQUIRE(a.al >= es && a.alg >= es && aligned_to(dk, es) && aligned_to(dv, es),
+               "dr_window_attn_backward: a pointer is not aligned to its element size");
+    hipStream_t st = (hipStream_t)stream;
+#define WIN_BWD(T) WIN_BY_D(T, win_bwd_launch, a, dq, dk, dv, st)
+    DR_BY_DTYPE(dtype, WIN_BWD);
+#undef WIN_BWD
+}
+
+extern "C" int64_t dr_window_attn_token_bytes(int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int64_t window,
+                                              int32_t sinks) {
+    using namespace dr;
+    int rc = win_check("dr_window_attn_token_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
+    if (rc != DR_OK) return rc;
+    if (B == 0) return 256;
+    int splits, per;
+    token_split(B, Hkv, (Hq / Hkv + 15) / 16, token_keys(L, window, sinks), &splits, &per);
+    return splits > 1 ? align_up(B * Hq * splits * ((int64_t)D + 2) * 4, 256) : 256;
+}
+
+extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                        const void* v, const int64_t* v_strides, int64_t B, int64_t L, int32_t Hq,
+                                        int32_t Hkv, int32_t D, int32_t dtype, int64_t window, int32_t sinks, float scale,
+                                        const int32_t* begin, const int32_t* end, void* out, void* ws, int64_t ws_bytes,
+                                        void* stream) {
+    using namespace dr;
+    int rc = win_check("dr_window_attn_token", B, L, Hq, Hkv, D, dtype, window, sinks, scale);
+    if (rc != DR_OK) return rc;
+    if (B == 0) return DR_OK;
+    DR_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides, "dr_window_attn_token: NULL pointer");
+    DR_REQUIRE(ws && aligned_to(ws, 256), "dr_window_attn_token: workspace is NULL or not 256-byte aligned");
+    const int64_t need = dr_window_attn_token_bytes(B, L, Hq, Hkv, D, window, sinks);
+    if (ws_bytes < need)
+        DR_FAIL(DR_ERR_WORKSPACE, "dr_window_attn_token: workspace %lld < required %lld", (long long)ws_bytes, (long long)need);
+    const int es = dtype_size(dtype);
+    TokenArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.qb = q_strides[0];
+    a.qh = q_strides[1];
+    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
+    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.B = (int)B;
+    a.L = (int)L;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.D = D;
+    a.W = (int)(window < L ? window : L);
+    a.S = sinks;
+    a.hgroups = (Hq / Hkv + 15) / 16;
+    token_split(B, Hkv, a.hgroups, token_keys(L, window, sinks), &a.splits, &a.per);
+    DR_REQUIRE((int64_t)a.splits * a.hgroups * Hkv * B < (1ll << 31) && B * Hq < (1ll << 31),
+               "dr_window_attn_token: too many workgroups");
+    a.scale = scale;
+    a.begin = begin;
+    a.end = end;
+    a.al = row_alignment(es, {k, v}, {a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    a.alq = row_alignment(es, {q}, {a.qb, a.qh});
+    DR_REQUIRE(a.al >= es && a.alq >= es && aligned_to(out, es), "dr_window_attn_token: a pointer is not aligned to its element size");
+    a.out = out;
+    a.part = (float*)ws;
+    hipStream_t st = (hipStream_t)stream;
+#define WIN_TOK(T) WIN_BY_D(T, win_token_launch, a, st)
+    DR_BY_DTYPE(dtype, WIN_TOK);
+#undef WIN_TOK
+}

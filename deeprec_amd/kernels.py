@@ -1300,3 +1300,111 @@ def item_logprobs_backward(logits, targets, lse, entropy, g_logp, g_entropy=None
                                                _ptr(g_logp) if targets is not None else None, _ptr(g_entropy), _ptr(out),
                                                _stream()), "dr_item_logprobs_backward")
     return out
+
+
+# ------------------------------------------------------------------ windowed attention with first items
+WIN_MAX_D, WIN_MAX_SINKS = 256, 64
+
+
+def _win_tensor(t, name, ndim, dtype=None):
+    """An attention operand: any strides, last dim contiguous."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("%s must be a CUDA/HIP tensor (deeprec_amd has no CPU path)" % name)
+    _on_current_device(t, name)
+    if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
+        raise TypeError("%s must be %s, got %s" % (name, dtype or "float32, float16 or bfloat16", t.dtype))
+    if t.dim() != ndim:
+        raise ValueError("%s must have %d dims, got shape %s" % (name, ndim, tuple(t.shape)))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("%s: the last dim must be contiguous" % name)
+    # the stride of a dim of one entry is never used and may be anything
+    return (C.c_int64 * (ndim - 1))(*[st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])])
+
+
+def _win_mask(B, window, sinks, scale, D, begin, end):
+    window, sinks = int(window), int(sinks)
+    if window < 1 or not 0 <= sinks <= WIN_MAX_SINKS:
+        raise ValueError("window must be >= 1 and sinks 0..%d, got %d and %d" % (WIN_MAX_SINKS, window, sinks))
+    for name, t in (("begin", begin), ("end", end)):
+        if t is not None and _req(t, torch.int32, name, 1).numel() != B:
+            raise ValueError("%s must hold one position per sequence" % name)
+    return min(window, 1 << 40), sinks, float(D ** -0.5 if scale is None else scale)
+
+
+def _win_shapes(q, k, v):
+    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[-1] != k.shape[-1]:
+        raise ValueError("q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if not 1 <= q.shape[-1] <= WIN_MAX_D:
+        raise ValueError("head dim must be 1..%d" % WIN_MAX_D)
+    Hq, Hkv = q.shape[-2], k.shape[-2]
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("%d query heads are no multiple of %d key heads" % (Hq, Hkv))
+    if k.shape[1] < 1:
+        raise ValueError("the sequence dim is empty")
+
+
+def window_attn_forward(q, k, v, window, sinks=0, scale=None, begin=None, end=None):
+    """Causal attention over the last `window` positions and the first `sinks` items of each history.  q [B, L, Hq, D],
+    k, v [B, L, Hkv, D] (float32 / float16 / bfloat16, any strides with the last dim contiguous), Hq a multiple of Hkv.
+    Key j is visible to query i iff begin <= j <= i < end and (i - j < window or j - begin < sinks); begin / end: int32 [B]
+    (None: the whole row), so padding may stand on either side; padded positions are never read and give zero rows.
+    scale None: D ** -0.5.  Returns (out [B, L, Hq, D], lse float32 [B, Hq, L])."""
+    sq = _win_tensor(q, "q", 4)
+    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
+    _win_shapes(q, k, v)
+    B, L, Hq, D = q.shape
+    if k.shape[1] != L:
+        raise ValueError("q and k must have the same length, got %d and %d" % (L, k.shape[1]))
+    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
+    out = torch.empty((B, L, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device)
+    check(_abi.lib().dr_window_attn_forward(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, B, L, Hq, k.shape[2], D, DTYPES[q.dtype],
+                                            window, sinks, scale, _ptr(begin), _ptr(end), _ptr(out), _ptr(lse), _stream()),
+          "dr_window_attn_forward")
+    return out, lse
+
+
+def window_attn_backward(q, k, v, out, lse, gout, window, sinks=0, scale=None, begin=None, end=None):
+    """(dq [B, L, Hq, D], dk, dv [B, L, Hkv, D]) of window_attn_forward for d loss / d out = gout; out and lse as it
+    returned them.  Bit-repeatable."""
+    sq = _win_tensor(q, "q", 4)
+    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
+    _win_shapes(q, k, v)
+    B, L, Hq, D = q.shape
+    if k.shape[1] != L:
+        raise ValueError("q and k must have the same length, got %d and %d" % (L, k.shape[1]))
+    for name, t in (("out", out), ("gout", gout)):
+        if _req(t, q.dtype, name, 4).shape != q.shape:
+            raise ValueError("%s must be shaped like q" % name)
+    if tuple(_req(lse, torch.float32, "lse", 3).shape) != (B, Hq, L):
+        raise ValueError("lse must be [B, Hq, L]")
+    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
+    Hkv = k.shape[2]
+    dq = torch.empty((B, L, Hq, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, L, Hkv, D), dtype=q.dtype, device=q.device)
+    dv = torch.empty((B, L, Hkv, D), dtype=q.dtype, device=q.device)
+    ws = torch.empty(check(_abi.lib().dr_window_attn_backward_bytes(B, L, Hq, Hkv, D, window, sinks),
+                           "dr_window_attn_backward_bytes"), dtype=torch.uint8, device=q.device)
+    check(_abi.lib().dr_window_attn_backward(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, _ptr(out), _ptr(lse), _ptr(gout), B, L, Hq,
+                                             Hkv, D, DTYPES[q.dtype], window, sinks, scale, _ptr(begin), _ptr(end), _ptr(dq),
+                                             _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream()), "dr_window_attn_backward")
+    return dq, dk, dv
+
+
+def window_attn_token(q, k, v, window, sinks=0, scale=None, begin=None, end=None):
+    """The serving form: one new token per sequence.  q [B, Hq, D] stands at position end - 1 of the caches k, v
+    [B, L, Hkv, D], which already hold its own key and value; it sees what window_attn_forward's last query sees.
+    Returns out [B, Hq, D] (zeros for an empty history)."""
+    sq = _win_tensor(q, "q", 3)
+    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
+    _win_shapes(q, k, v)
+    B, Hq, D = q.shape
+    L, Hkv = k.shape[1], k.shape[2]
+    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    ws = torch.empty(check(_abi.lib().dr_window_attn_token_bytes(B, L, Hq, Hkv, D, window, sinks),
+                           "dr_window_attn_token_bytes"), dtype=torch.uint8, device=q.device)
+    check(_abi.lib().dr_window_attn_token(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, B, L, Hq, Hkv, D, DTYPES[q.dtype], window,
+                                          sinks, scale, _ptr(begin), _ptr(end), _ptr(out), _ptr(ws), ws.numel(), _stream()),
+          "dr_window_attn_token")
+    return out

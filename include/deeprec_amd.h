@@ -56,7 +56,8 @@ extern "C" {
 #define DR_SCORE_NEG_SQDIST 1 /* cml.py:151-153                                       */
 #define DR_SCORE_TWO_DIST 2   /* SeqRecMetrics.py:122-123 (AttRec / PRME)             */
 
-/* element types of the mixed-precision entry points (dr_embed_*, dr_item_logprobs_*, dr_clip_global_norm) */
+/* element types of the mixed-precision entry points (dr_embed_*, dr_window_attn_*, dr_item_logprobs_*,
+ * dr_clip_global_norm) */
 #define DR_F32 0
 #define DR_F16 1
 #define DR_BF16 2
@@ -568,6 +569,35 @@ int32_t dr_embed_forward(const void* table, int64_t rows, int32_t d, int32_t dty
 int64_t dr_embed_backward_bytes(int64_t n, int32_t d);
 int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype, const void* ids, int32_t id_bits,
                           int64_t rows, float scale, int64_t padding, void* grad, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- causal attention over a sliding window and the first items of a history -------------------------------------------
+ * Beside AttRec's pooling attention (dr_attn_pool_*, AttRec.py:147-186): an output per position, for histories of any length.
+ * q [B, L, Hq, D], k, v [B, L, Hkv, D], Hq a multiple of Hkv (query head h reads key head h / (Hq / Hkv)), one type
+ * (DR_F32 / DR_F16 / DR_BF16), 1 <= D <= 256; the last dim is contiguous, *_strides = element strides {batch, position, head}.
+ * Key j is visible to query i iff begin[b] <= j <= i < end[b] and (i - j < window or j - begin[b] < sinks); window >= 1,
+ * 0 <= sinks <= 64; begin / end int32 [B] on the device (NULL: 0 / L), cut to [0, L].  scale > 0.
+ * forward: out [B, L, Hq, D] contiguous, lse [B, Hq, L] fp32 = log sum exp(scale <q, k>).  A position outside [begin, end)
+ * gives a zero row (lse -inf, gradients 0) and is never read.  backward: out, lse as written, gout [B, L, Hq, D]
+ * contiguous -> dq [B, L, Hq, D], dk, dv [B, L, Hkv, D] contiguous, overwritten; sums over a group's heads included; no
+ * atomics, bit-repeatable.  ws: dr_window_attn_backward_bytes(...), 256-byte aligned.
+ * token: ONE query per sequence, q [B, Hq, D] (strides {batch, head}), at position end[b] - 1 of a cache k, v [B, L, Hkv, D]
+ * that already holds its own key and value -> out [B, Hq, D] contiguous.  ws: dr_window_attn_token_bytes(...). */
+int32_t dr_window_attn_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, int64_t B, int64_t L, int32_t Hq, int32_t Hkv,
+                               int32_t D, int32_t dtype, int64_t window, int32_t sinks, float scale, const int32_t* begin,
+                               const int32_t* end, void* out, float* lse, void* stream);
+int64_t dr_window_attn_backward_bytes(int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int64_t window,
+                                      int32_t sinks);
+int32_t dr_window_attn_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, const void* out, const float* lse,
+                                const void* gout, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                                int64_t window, int32_t sinks, float scale, const int32_t* begin, const int32_t* end,
+                                void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes, void* stream);
+int64_t dr_window_attn_token_bytes(int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int64_t window, int32_t sinks);
+int32_t dr_window_attn_token(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D,
+                             int32_t dtype, int64_t window, int32_t sinks, float scale, const int32_t* begin,
+                             const int32_t* end, void* out, void* ws, int64_t ws_bytes, void* stream);
 
 /* ---- log-probabilities of given items over the catalog, entropy and best items ----------------------------------------
  * logits [N, V] (DR_F32 / DR_F16 / DR_BF16, row stride ld >= V elements): -inf marks an item that is not offered.
