@@ -4,6 +4,8 @@
 //             ids equal to padding, or outside [0, rows), contribute nothing.
 // HBM-bound both ways.  Sums are fp32 in a fixed order (sorted list cut into blocks of EMB_CHUNK entries, entries in list
 // order inside a block, a row's blocks in ascending order): the same ids and gradients give the same bits, with no atomics.
+#include <utility>
+
 #include "dr_lsd_sort.h"
 #include "dr_types.h"
 
@@ -11,8 +13,7 @@ namespace dr {
 
 constexpr int EMB_MAX_D = 32768;
 constexpr int EMB_CHUNK = 32;        // sorted entries a group of lanes sums
-constexpr int EMB_DEPTH = 8;         // gradient rows of a chunk in flight per lane group
-constexpr int64_t EMB_SMALL_N = 4096;   // lists the one-workgroup plan sorts in one launch (segment.hip)
+constexpr int EMB_DEPTH = 16;        // gradient rows of a chunk in flight per lane group
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 // A block owns R whole rows = R * cpr vectors of V elements, dealt to its threads in order, so every lane moves 16 bytes
@@ -52,6 +53,15 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict_
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
+// Stable sort of (id, list position), then the sums.  At 2 x 10^5 ids the sort is launches and latency, not bytes, so it
+// takes the fewest passes that cover the table's rows (digits of 8 to 11 bits: 2 passes up to 2^22 rows), and while it
+// runs most of the chip would idle: its launches carry extra workgroups that clear the gradient table (rows no id names
+// stay 0), which therefore costs next to nothing.
+constexpr int SRT_T = 512, SRT_WAVES = SRT_T / 64, SRT_IPT = 4, SRT_TILE = SRT_T * SRT_IPT;
+constexpr int SRT_MAX_TILES = 128;      // beyond, every workgroup would read too many tile histograms: lsd_sort
+constexpr int64_t SRT_MAX_N = SRT_MAX_TILES * SRT_TILE;
+constexpr int SRT_DIRECT_TILES = 8;     // up to here a workgroup counts all keys itself instead of a histogram launch
+
 template <class Id>
 struct EmbedKeys {  // ids -> sort keys; ids that contribute nothing sort behind every row
     const Id* ids;
@@ -63,134 +73,329 @@ struct EmbedKeys {  // ids -> sort keys; ids that contribute nothing sort behind
     __device__ __forceinline__ int32_t val(int64_t e) const { return (int32_t)e; }
 };
 
-template <class T>
-__global__ __launch_bounds__(256) void embed_zero_kernel(T* __restrict__ grad, int64_t count) {
-    constexpr int V = 16 / (int)sizeof(T);
-    typename VecType<T, V>::type z;
-#pragma unroll
-    for (int x = 0; x < V; ++x) z[x] = (T)0.0f;
-    const int64_t nv = count / V, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nv; i += step)
-        *reinterpret_cast<typename VecType<T, V>::type*>(grad + i * V) = z;
-    if (blockIdx.x == 0 && threadIdx.x < (unsigned)(count - nv * V)) grad[nv * V + threadIdx.x] = (T)0.0f;
-}
-
-struct EmbedArgs {
-    const uint32_t* keys;   // sorted keys (>= rows: contributes nothing), or NULL: looked up through ids
-    const int32_t* spos;    // sorted list positions
-    const void* ids;
-    int64_t n, rows, padding, chunks;
-    int d;
-    float scale;
-    float* part;            // [chunks, 2, d] sums of the runs that cross a chunk border: first run, last run
+struct EmbedPairs {  // a previous pass's output
+    const uint2* pairs;
+    __device__ __forceinline__ uint32_t key(int64_t e) const { return pairs[e].x; }
+    __device__ __forceinline__ int32_t val(int64_t e) const { return (int32_t)pairs[e].y; }
 };
 
-template <class Id>
-__device__ __forceinline__ int64_t embed_key(const EmbedArgs& a, int64_t s) {
-    if (a.keys) return (int64_t)a.keys[s];
-    const int64_t id = (int64_t)((const Id*)a.ids)[a.spos[s]];
-    return (id < 0 || id >= a.rows || id == a.padding) ? a.rows : id;
+// `count` 16-byte pieces of zeros from `base` on, written by workgroups first, first + 1, .. first + blocks - 1
+struct EmbedFill {
+    uint4* base;
+    int64_t count;
+    int first, blocks;
+};
+__device__ __forceinline__ void embed_fill(const EmbedFill& f, int block) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 z = {0, 0, 0, 0};
+    const int64_t per = (f.count + f.blocks - 1) / f.blocks, lo = block * per, hi = lo + per < f.count ? lo + per : f.count;
+#pragma unroll 4
+    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) reinterpret_cast<u32x4*>(f.base)[i] = z;
+}
+template <class T>
+__global__ __launch_bounds__(256) void embed_zero_kernel(EmbedFill f, T* __restrict__ tail, int n_tail) {
+    embed_fill(f, (int)blockIdx.x);
+    if (blockIdx.x == 0 && (int)threadIdx.x < n_tail) tail[threadIdx.x] = (T)0.0f;
 }
 
-// One group of LPR lanes per chunk.  A run (equal keys) that lies inside the chunk is finished here; the part of a run that
-// began in an earlier chunk goes to part[chunk][0], the part of one that goes on behind the chunk to part[chunk][1] (a run
-// that does both: [0]).
-template <class T, class Id, int V, int LPR>
-__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedArgs a, const T* __restrict__ gout, T* __restrict__ grad) {
-    const int64_t chunk = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
-    if (chunk >= a.chunks) return;
-    const int lane = threadIdx.x % LPR;
-    const int64_t s0 = chunk * EMB_CHUNK;
-    const int m = (int)(a.n - s0 < EMB_CHUNK ? a.n - s0 : EMB_CHUNK);
-    if (a.keys && a.keys[s0] >= (uint32_t)a.rows) return;    // sorted: nothing from here on contributes
-    const int64_t before = s0 > 0 ? embed_key<Id>(a, s0 - 1) : -1, behind = s0 + m < a.n ? embed_key<Id>(a, s0 + m) : -1;
-    for (int c = lane * V; c < a.d; c += LPR * V) {
-        float acc[V];
+// digit counts of every tile
+template <int BITS, class Src>
+__global__ __launch_bounds__(SRT_T) void embed_hist_kernel(Src src, int n, unsigned shift, uint16_t* __restrict__ hist,
+                                                           EmbedFill fill) {
+    constexpr int BINS = 1 << BITS;
+    __shared__ int bins[BINS];
+    if ((int)blockIdx.x >= fill.first) {
+        embed_fill(fill, (int)blockIdx.x - fill.first);
+        return;
+    }
+    const int base = (int)blockIdx.x * SRT_TILE + (int)threadIdx.x;
+    uint32_t key[SRT_IPT];
 #pragma unroll
-        for (int x = 0; x < V; ++x) acc[x] = 0.0f;
-        int64_t run = -1;                          // key of the run being summed
-        bool carried = false;                      // it began before this chunk
-        for (int q0 = 0; q0 < m; q0 += EMB_DEPTH) {
-            int64_t key[EMB_DEPTH];
-            float v[EMB_DEPTH][V];
+    for (int q = 0; q < SRT_IPT; ++q) key[q] = src.key(base + q * SRT_T < n ? base + q * SRT_T : n - 1);
+    for (int d = threadIdx.x; d < BINS; d += SRT_T) bins[d] = 0;
+    __syncthreads();
 #pragma unroll
-            for (int q = 0; q < EMB_DEPTH; ++q) {
-                const int64_t s = s0 + (q0 + q < m ? q0 + q : m - 1);
-                key[q] = embed_key<Id>(a, s);
-                load_f32<T, V>(v[q], gout + (int64_t)a.spos[s] * a.d + c);
-            }
+    for (int q = 0; q < SRT_IPT; ++q)
+        if (base + q * SRT_T < n) atomicAdd(&bins[(key[q] >> shift) & (BINS - 1)], 1);
+    __syncthreads();
+    for (int d = threadIdx.x; d < BINS; d += SRT_T) hist[(int64_t)blockIdx.x * BINS + d] = (uint16_t)bins[d];
+}
+
+// exclusive sum of one value per thread over the workgroup
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* red) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = x;
 #pragma unroll
-            for (int q = 0; q < EMB_DEPTH; ++q) {
-                if (q0 + q >= m || key[q] >= a.rows) continue;
-                if (key[q] != run) {
-                    if (run >= 0) {
-                        if (carried) {
-                            store_f32<float, V>(a.part + (chunk * 2) * a.d + c, acc);
-                        } else {
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t y = __shfl_up(s, off, 64);
+        if (lane >= off) s += y;
+    }
+    if (lane == 63) red[wave] = s;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int w = 0; w < wave; ++w) before += red[w];
+    __syncthreads();
+    return before + s - x;
+}
+
+// Places every key of a tile: keys with a smaller digit, equal digits in earlier tiles, equal digits earlier in the tile.
+// A wavefront takes 256 consecutive keys in four rounds of 64; lanes with equal digits find each other by one ballot per
+// bit, the first of them moves the wavefront's counter of that digit.  No atomics whose order matters.
+template <int BITS, class Src>
+__global__ __launch_bounds__(SRT_T) void embed_scatter_kernel(Src src, int n, unsigned shift, const uint16_t* __restrict__ hist,
+                                                              int ntiles, uint2* __restrict__ out, EmbedFill fill) {
+    constexpr int BINS = 1 << BITS, BPT = BINS > SRT_T ? BINS / SRT_T : 1;
+    __shared__ uint32_t cnt[SRT_WAVES][BINS];       // a wavefront's keys per digit, then where they go
+    __shared__ uint32_t red[SRT_WAVES];
+    if ((int)blockIdx.x >= fill.first) {
+        embed_fill(fill, (int)blockIdx.x - fill.first);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tile = (int)blockIdx.x;
+    // the tile's keys and payloads first: they arrive while the counts are put together
+    uint32_t key[SRT_IPT], rank[SRT_IPT];
+    int32_t val[SRT_IPT];
+    const int k0 = tile * SRT_TILE + wave * (64 * SRT_IPT) + lane;
 #pragma unroll
-                            for (int x = 0; x < V; ++x) acc[x] *= a.scale;
-                            store_f32<T, V>(grad + run * a.d + c, acc);
-                        }
+    for (int q = 0; q < SRT_IPT; ++q) {
+        const int e = k0 + q * 64 < n ? k0 + q * 64 : n - 1;
+        key[q] = src.key(e);
+        val[q] = src.val(e);
+    }
+    // cnt[0]: keys per digit in earlier tiles, cnt[1]: in this one and later ones
+    for (int d = tid; d < BINS; d += SRT_T) cnt[0][d] = cnt[1][d] = 0;
+    __syncthreads();
+    if (hist) {
+        // pairs of digits x parts of the tile list over the threads, 32 tiles of a part requested together: the table was
+        // written by other XCDs, a round trip to it is what this step costs
+        constexpr int PAIRS = BINS / 2, PARTS = PAIRS < SRT_T ? SRT_T / PAIRS : 1;
+        const uint32_t* h2 = reinterpret_cast<const uint32_t*>(hist);
+        const int per = (ntiles + PARTS - 1) / PARTS, t_lo = tid / PAIRS * per, t_hi = t_lo + per < ntiles ? t_lo + per : ntiles;
+        for (int p = tid % PAIRS; p < PAIRS; p += SRT_T) {
+            uint32_t e0 = 0, e1 = 0, r0 = 0, r1 = 0;
+            for (int t0 = t_lo; t0 < t_hi; t0 += 32) {
+                uint32_t h[32];
+#pragma unroll
+                for (int q = 0; q < 32; ++q) h[q] = h2[(int64_t)(t0 + q < t_hi ? t0 + q : t_lo) * PAIRS + p];
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                    const uint32_t v = t0 + q < t_hi ? h[q] : 0u;
+                    if (t0 + q < tile) {
+                        e0 += v & 0xFFFFu;
+                        e1 += v >> 16;
+                    } else {
+                        r0 += v & 0xFFFFu;
+                        r1 += v >> 16;
                     }
-                    run = key[q];
-                    carried = q0 + q == 0 && before == run;
-#pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] = 0.0f;
                 }
-#pragma unroll
-                for (int x = 0; x < V; ++x) acc[x] += v[q][x];
             }
+            atomicAdd(&cnt[0][2 * p], e0);
+            atomicAdd(&cnt[0][2 * p + 1], e1);
+            atomicAdd(&cnt[1][2 * p], r0);
+            atomicAdd(&cnt[1][2 * p + 1], r1);
         }
-        if (run < 0) continue;
-        if (carried) {
-            store_f32<float, V>(a.part + (chunk * 2) * a.d + c, acc);
-        } else if (behind == run) {
-            store_f32<float, V>(a.part + (chunk * 2 + 1) * a.d + c, acc);
-        } else {
+    } else {                                                     // few keys: count all of them here
+        uint32_t k[SRT_DIRECT_TILES][SRT_IPT];
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] *= a.scale;
-            store_f32<T, V>(grad + run * a.d + c, acc);
+        for (int t = 0; t < SRT_DIRECT_TILES; ++t)
+#pragma unroll
+            for (int q = 0; q < SRT_IPT; ++q) {
+                const int e = t * SRT_TILE + q * SRT_T + tid;
+                k[t][q] = src.key(e < n ? e : n - 1);
+            }
+#pragma unroll
+        for (int t = 0; t < SRT_DIRECT_TILES; ++t)
+#pragma unroll
+            for (int q = 0; q < SRT_IPT; ++q)
+                if (t * SRT_TILE + q * SRT_T + tid < n) atomicAdd(&cnt[t < tile ? 0 : 1][(k[t][q] >> shift) & (BINS - 1)], 1u);
+    }
+    __syncthreads();
+    uint32_t tot[BPT], pre[BPT];
+    const int d0 = tid * BPT;
+    const bool own = d0 < BINS;
+#pragma unroll
+    for (int x = 0; x < BPT; ++x) {
+        pre[x] = own ? cnt[0][d0 + x] : 0u;
+        tot[x] = own ? pre[x] + cnt[1][d0 + x] : 0u;
+    }
+    __syncthreads();
+    for (int d = tid; d < BINS * SRT_WAVES; d += SRT_T) (&cnt[0][0])[d] = 0;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int x = 0; x < BPT; ++x) mine += tot[x];
+    uint32_t base = block_exclusive(mine, red);                  // its barriers also order the clearing above
+    // rank inside the wavefront's 256 keys
+#pragma unroll
+    for (int q = 0; q < SRT_IPT; ++q) {
+        const bool in = k0 + q * 64 < n;
+        const uint32_t d = (key[q] >> shift) & (BINS - 1);
+        uint64_t same = __ballot(in);
+#pragma unroll
+        for (int b = 0; b < BITS; ++b) {
+            const uint64_t ones = __ballot((d >> b) & 1u);
+            same &= (d >> b) & 1u ? ones : ~ones;
+        }
+        const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0u));
+        uint32_t before = 0;
+        if (in) before = cnt[wave][d];
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (in && below == 0) cnt[wave][d] = before + (uint32_t)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        rank[q] = before + (uint32_t)below;
+    }
+    __syncthreads();
+    if (own) {
+#pragma unroll
+        for (int x = 0; x < BPT; ++x) {
+            uint32_t at = base + pre[x];
+#pragma unroll
+            for (int w = 0; w < SRT_WAVES; ++w) {
+                const uint32_t c = cnt[w][d0 + x];
+                cnt[w][d0 + x] = at;
+                at += c;
+            }
+            base += tot[x];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < SRT_IPT; ++q) {
+        if (k0 + q * 64 < n) {
+            const uint32_t pos = cnt[wave][(key[q] >> shift) & (BINS - 1)] + rank[q];
+            out[pos] = make_uint2(key[q], (uint32_t)val[q]);   // one scattered write of 8 bytes, not two of 4
         }
     }
 }
 
-// Joins the runs that cross chunk borders: one block per chunk in which such a run BEGINS; the 256 threads of the block
-// are 256 / LPR groups that take every (256 / LPR)-th of the run's chunks, the groups' sums are added in order.
-template <class T, class Id, int V, int LPR>
+struct EmbedArgs {
+    const uint32_t* keys;   // sorted keys (every step-th word); those >= rows contribute nothing and stand last
+    const uint32_t* spos;   // their list positions, likewise
+    int step;
+    int64_t n, rows, chunks;
+    int d;
+    float scale;
+    float* part;            // [chunks, 2, d] sums of the runs that cross a chunk border: first run, last run
+    uint8_t* state;         // [chunks] RUN_*
+};
+constexpr uint8_t RUN_BEGINS = 1;   // the last run of the chunk begins in it and goes on behind it
+constexpr uint8_t RUN_FILLS = 2;    // one run fills the chunk and goes on on both sides
+
+// One group of LPR lanes per chunk.  A run (equal keys) that lies inside the chunk is finished here; the part of a run that
+// began in an earlier chunk goes to part[chunk][0], the part of one that goes on behind the chunk to part[chunk][1] (a run
+// that does both: [0]).  The chunk's keys and positions are fetched once, spread over the lanes, so that the only
+// dependent step left is position -> row, 16 rows in flight.
+template <class T, int V, int LPR>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedArgs a, const T* __restrict__ gout, T* __restrict__ grad) {
+    constexpr int E = EMB_CHUNK / LPR > 0 ? EMB_CHUNK / LPR : 1;    // entries a lane keeps
+    const int64_t chunk = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+    const int lane = threadIdx.x % LPR, group0 = (threadIdx.x & 63) - lane;
+    if (chunk >= a.chunks) return;                                  // whole groups leave
+    const int64_t s0 = chunk * EMB_CHUNK;
+    const int m = (int)(a.n - s0 < EMB_CHUNK ? a.n - s0 : EMB_CHUNK);
+    uint32_t keys[E];
+    uint32_t spos[E];
+#pragma unroll
+    for (int x = 0; x < E; ++x) {
+        const int q = x * LPR + lane;
+        const int64_t s = s0 + (q < m ? q : m - 1);
+        keys[x] = a.keys[s * a.step];
+        spos[x] = a.spos[s * a.step];
+    }
+    const uint32_t rows = (uint32_t)a.rows, none = 0xFFFFFFFFu;
+    const uint32_t before = s0 > 0 ? a.keys[(s0 - 1) * a.step] : none, behind = s0 + m < a.n ? a.keys[(s0 + m) * a.step] : none;
+    auto entry = [&](const auto (&r)[E], int q) { return __shfl(r[q / LPR < E ? q / LPR : 0], group0 + q % LPR, 64); };
+    const uint32_t k_first = entry(keys, 0), k_last = __shfl(keys[(m - 1) / LPR < E ? (m - 1) / LPR : 0], group0 + (m - 1) % LPR, 64);
+    if (lane == 0) {
+        uint8_t st = 0;
+        if (k_last < rows && k_last == behind) st = k_first == k_last && before == k_first ? RUN_FILLS : RUN_BEGINS;
+        a.state[chunk] = st;
+    }
+    if (k_first >= rows) return;                                    // sorted: nothing from here on contributes
+    for (int c0 = 0; c0 < a.d; c0 += LPR * V) {                     // every lane of the group stays for the shuffles
+        const int c = c0 + lane * V;
+        const bool on = c < a.d;
+        float acc[V];
+#pragma unroll
+        for (int x = 0; x < V; ++x) acc[x] = 0.0f;
+        uint32_t run = k_first;
+        bool carried = before == k_first;
+        auto flush = [&](uint32_t next) {                           // the run ends; `next`: the key behind it
+            if (!on) return;
+            if (carried) {
+                store_f32<float, V>(a.part + (chunk * 2) * a.d + c, acc);
+            } else if (next == run) {
+                store_f32<float, V>(a.part + (chunk * 2 + 1) * a.d + c, acc);
+            } else {
+#pragma unroll
+                for (int x = 0; x < V; ++x) acc[x] *= a.scale;
+                store_f32<T, V>(grad + (int64_t)run * a.d + c, acc);
+            }
+        };
+        const T* col = gout + (on ? c : 0);
+#pragma unroll
+        for (int q0 = 0; q0 < EMB_CHUNK; q0 += EMB_DEPTH) {
+            // unconditional loads of valid rows (entries behind the list repeat its last): under a condition each would
+            // wait for the one before
+            typename VecType<T, V>::type v[EMB_DEPTH];
+            uint32_t key[EMB_DEPTH];
+#pragma unroll
+            for (int q = 0; q < EMB_DEPTH; ++q)
+                v[q] = *reinterpret_cast<const typename VecType<T, V>::type*>(col + (int64_t)entry(spos, q0 + q) * a.d);
+#pragma unroll
+            for (int q = 0; q < EMB_DEPTH; ++q) key[q] = entry(keys, q0 + q);
+#pragma unroll
+            for (int q = 0; q < EMB_DEPTH; ++q) {
+                if (q0 + q >= m || key[q] >= rows) continue;
+                if (key[q] != run) {
+                    flush(key[q]);
+                    run = key[q];
+                    carried = false;
+#pragma unroll
+                    for (int x = 0; x < V; ++x) acc[x] = 0.0f;
+                }
+                if constexpr (V == 1) {
+                    acc[0] += (float)v[q];
+                } else {
+#pragma unroll
+                    for (int x = 0; x < V; ++x) acc[x] += (float)v[q][x];
+                }
+            }
+        }
+        flush(k_last < rows ? behind : none);
+    }
+}
+
+// Joins the runs that cross chunk borders.  A workgroup looks at four chunks; for each in which such a run begins, it
+// follows the chunks' states to the run's end (64 at a time) and adds the parts up: its 256 / LPR lane groups take every
+// (256 / LPR)-th chunk, the groups' sums are added in order.
+template <class T, int V, int LPR>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a, T* __restrict__ grad) {
     constexpr int GROUPS = 256 / LPR;
     __shared__ float red[GROUPS][LPR * V];
-    __shared__ int64_t run_s;
-    __shared__ int64_t last_s;
-    for (int64_t chunk = blockIdx.x; chunk + 1 < a.chunks; chunk += gridDim.x) {
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const int64_t s0 = chunk * EMB_CHUNK, e = s0 + EMB_CHUNK;          // e < n: not the last chunk
-            const int64_t run = embed_key<Id>(a, e - 1);
-            bool begins = run < a.rows && embed_key<Id>(a, e) == run;
-            if (begins && embed_key<Id>(a, s0) == run && s0 > 0 && embed_key<Id>(a, s0 - 1) == run) begins = false;
-            run_s = begins ? run : -1;
-            if (begins) {                                                       // last chunk the run reaches
-                int64_t lo = chunk + 1, hi = a.chunks - 1;
-                while (lo < hi) {
-                    const int64_t mid = (lo + hi + 1) >> 1;
-                    if (embed_key<Id>(a, mid * EMB_CHUNK) == run) lo = mid; else hi = mid - 1;
-                }
-                last_s = lo;
+    const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, wl = threadIdx.x & 63;
+    for (int j = 0; j < 4; ++j) {
+        const int64_t chunk = (int64_t)blockIdx.x * 4 + j;
+        if (chunk >= a.chunks || a.state[chunk] != RUN_BEGINS) continue;      // workgroup-uniform
+        int64_t last = chunk + 1;                                             // last chunk the run reaches
+        for (;;) {
+            const int64_t at = last + wl;
+            const uint64_t ends = __ballot(at >= a.chunks - 1 || a.state[at < a.chunks ? at : a.chunks - 1] != RUN_FILLS);
+            if (ends) {
+                last += __ffsll((unsigned long long)ends) - 1;
+                break;
             }
+            last += 64;
         }
-        __syncthreads();
-        const int64_t run = run_s;
-        if (run < 0) continue;                                                  // block-uniform
-        const int64_t last = last_s;
-        const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+        const int64_t run = (int64_t)a.keys[((chunk + 1) * EMB_CHUNK - 1) * a.step];
         for (int c0 = 0; c0 < a.d; c0 += LPR * V) {
             const int c = c0 + lane * V;
             float acc[V];
 #pragma unroll
             for (int x = 0; x < V; ++x) acc[x] = 0.0f;
             if (c < a.d)
-#pragma unroll 4
+#pragma unroll 8
                 for (int64_t q = chunk + group; q <= last; q += GROUPS) {
                     float v[V];
                     load_f32<float, V>(v, a.part + (q * 2 + (q == chunk ? 1 : 0)) * a.d + c);
@@ -201,8 +406,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a, T* __restr
             for (int x = 0; x < V; ++x) red[group][lane * V + x] = acc[x];
             __syncthreads();
             if (group == 0 && c < a.d) {
-#pragma unroll
-                for (int g = 1; g < GROUPS; ++g)
+                const int parts = (int)(last - chunk + 1 < GROUPS ? last - chunk + 1 : GROUPS);
+                for (int g = 1; g < parts; ++g)
 #pragma unroll
                     for (int x = 0; x < V; ++x) acc[x] += red[g][lane * V + x];
 #pragma unroll
@@ -215,8 +420,16 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a, T* __restr
 }
 
 struct EmbedLayout {
-    int64_t keys_a, keys_b, vals_a, vals_b, hdr, lsd, plan, part, total;
+    int64_t pairs_a, pairs_b, hist, state, part, total;
 };
+// digit width and number of passes that cover keys up to `rows` (the sentinel) with n keys
+static void embed_digits(int64_t rows, unsigned* bits, unsigned* passes) {
+    unsigned end_bit = 1;
+    while (end_bit < 31 && ((uint64_t)rows >> end_bit) != 0) ++end_bit;
+    *passes = end_bit <= 11 ? 1 : (end_bit <= 22 ? 2 : 3);
+    *bits = (end_bit + *passes - 1) / *passes;
+    if (*bits < 8) *bits = 8;
+}
 static EmbedLayout embed_layout(int64_t n, int d) {
     EmbedLayout L;
     int64_t off = 0;
@@ -225,17 +438,12 @@ static EmbedLayout embed_layout(int64_t n, int d) {
         off += align_up(bytes, 256);
         return o;
     };
-    L.keys_a = L.keys_b = L.vals_a = L.vals_b = L.hdr = L.lsd = L.plan = 0;
-    if (n <= EMB_SMALL_N) {
-        L.plan = take(dr_segment_plan_bytes(n, 1));
-    } else {
-        L.keys_a = take(n * 4);
-        L.keys_b = take(n * 4);
-        L.vals_a = take(n * 4);
-        L.vals_b = take(n * 4);
-        L.lsd = take(lsd_scratch_bytes(n));
-    }
-    L.part = take((n + EMB_CHUNK - 1) / EMB_CHUNK * 2 * (int64_t)d * 4);
+    const int64_t chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+    L.pairs_a = take(n * 8);
+    L.pairs_b = take(n * 8);
+    L.hist = take(n <= SRT_MAX_N ? (n + SRT_TILE - 1) / SRT_TILE * (1 << 11) * 2 : lsd_scratch_bytes(n));
+    L.state = take(chunks);
+    L.part = take(chunks * 2 * (int64_t)d * 4);
     L.total = off;
     return L;
 }
@@ -275,72 +483,128 @@ static int embed_forward_t(int dt, const void* table, int64_t rows, int d, const
     }
 }
 
-template <class T, class Id, int V, int LPR>
+template <class T, int V, int LPR>
 static int embed_sum_launch(const EmbedArgs& a, const void* gout, void* grad, hipStream_t st) {
     const int64_t blocks = (a.chunks * LPR + 255) / 256;
     DR_REQUIRE(blocks < (1ll << 31), "dr_embed_backward: too many blocks");
-    DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, Id, V, LPR>), dim3((unsigned)blocks), dim3(256), 0, st, a,
+    DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, V, LPR>), dim3((unsigned)blocks), dim3(256), 0, st, a,
                     (const T*)gout, (T*)grad);
     DR_CHECK_LAUNCH("embed_sum_kernel");
     if (a.chunks > 1) {
-        const int grid = (int)(a.chunks - 1 < 4096 ? a.chunks - 1 : 4096);
-        DR_LAUNCH_NAMED("embed_join_kernel", (embed_join_kernel<T, Id, V, LPR>), dim3(grid), dim3(256), 0, st, a, (T*)grad);
+        DR_LAUNCH_NAMED("embed_join_kernel", (embed_join_kernel<T, V, LPR>), dim3((unsigned)((a.chunks + 3) / 4)), dim3(256), 0,
+                        st, a, (T*)grad);
         DR_CHECK_LAUNCH("embed_join_kernel");
     }
     return DR_OK;
 }
-template <class T, class Id, int V>
+template <class T, int V>
 static int embed_sum_v(const EmbedArgs& a, const void* gout, void* grad, hipStream_t st) {
     const int cpr = a.d / V;
-    if (cpr <= 4) return embed_sum_launch<T, Id, V, 4>(a, gout, grad, st);
-    if (cpr <= 8) return embed_sum_launch<T, Id, V, 8>(a, gout, grad, st);
-    if (cpr <= 16) return embed_sum_launch<T, Id, V, 16>(a, gout, grad, st);
-    if (cpr <= 32) return embed_sum_launch<T, Id, V, 32>(a, gout, grad, st);
-    return embed_sum_launch<T, Id, V, 64>(a, gout, grad, st);
+    if (cpr <= 4) return embed_sum_launch<T, V, 4>(a, gout, grad, st);
+    if (cpr <= 8) return embed_sum_launch<T, V, 8>(a, gout, grad, st);
+    if (cpr <= 16) return embed_sum_launch<T, V, 16>(a, gout, grad, st);
+    if (cpr <= 32) return embed_sum_launch<T, V, 32>(a, gout, grad, st);
+    return embed_sum_launch<T, V, 64>(a, gout, grad, st);
+}
+
+// the part of the table that launch `step` of `steps` clears, after the launch's own `tiles` workgroups
+static EmbedFill embed_fill_part(void* grad, int64_t pieces, int step, int steps, int tiles) {
+    const int64_t lo = pieces * step / steps, hi = pieces * (step + 1) / steps;
+    EmbedFill f;
+    f.base = (uint4*)grad + lo;
+    f.count = hi - lo;
+    f.first = tiles;
+    const int64_t blocks = (f.count + 2047) / 2048;             // 32 KB each
+    f.blocks = (int)(blocks < 8192 ? blocks : 8192);
+    return f;
+}
+template <int BITS, class Src>
+static int embed_pass(Src src, int n, unsigned shift, void* hist, uint2* out, void* grad, int64_t pieces,
+                      int* step, int steps, hipStream_t st) {
+    const int tiles = (n + SRT_TILE - 1) / SRT_TILE;
+    uint16_t* h = nullptr;
+    if (tiles > SRT_DIRECT_TILES) {
+        h = (uint16_t*)hist;
+        const EmbedFill f = embed_fill_part(grad, pieces, (*step)++, steps, tiles);
+        DR_LAUNCH_NAMED("embed_hist_kernel", (embed_hist_kernel<BITS, Src>), dim3(tiles + f.blocks), dim3(SRT_T), 0, st, src, n,
+                        shift, h, f);
+        DR_CHECK_LAUNCH("embed_hist_kernel");
+    }
+    const EmbedFill f = embed_fill_part(grad, pieces, (*step)++, steps, tiles);
+    DR_LAUNCH_NAMED("embed_scatter_kernel", (embed_scatter_kernel<BITS, Src>), dim3(tiles + f.blocks), dim3(SRT_T), 0, st, src, n,
+                    shift, (const uint16_t*)h, tiles, out, f);
+    DR_CHECK_LAUNCH("embed_scatter_kernel");
+    return DR_OK;
+}
+template <class Src>
+static int embed_pass_bits(unsigned bits, Src src, int n, unsigned shift, void* hist, uint2* out, void* grad,
+                           int64_t pieces, int* step, int steps, hipStream_t st) {
+    switch (bits) {
+        case 8: return embed_pass<8>(src, n, shift, hist, out, grad, pieces, step, steps, st);
+        case 9: return embed_pass<9>(src, n, shift, hist, out, grad, pieces, step, steps, st);
+        case 10: return embed_pass<10>(src, n, shift, hist, out, grad, pieces, step, steps, st);
+        default: return embed_pass<11>(src, n, shift, hist, out, grad, pieces, step, steps, st);
+    }
 }
 
 template <class T, class Id>
 static int embed_backward_t(int dt, const void* gout, const void* ids, int64_t n, int64_t rows, int d, float scale,
                             int64_t padding, void* grad, char* ws, hipStream_t st) {
     const EmbedLayout L = embed_layout(n, d);
-    {
-        constexpr int V = 16 / (int)sizeof(T);
-        DR_LAUNCH_NAMED("embed_zero_kernel", (embed_zero_kernel<T>), dim3(grid_for(rows * d / V + 1, 256)), dim3(256), 0, st,
-                        (T*)grad, rows * d);
+    constexpr int VZ = 16 / (int)sizeof(T);
+    const int64_t pieces = rows * d / VZ;                          // and fewer than VZ elements behind them
+    const int n_tail = (int)(rows * d - pieces * VZ);
+    const bool own_sort = n > 0 && n <= SRT_MAX_N;
+    if (!own_sort || n_tail > 0) {
+        EmbedFill f = embed_fill_part(grad, own_sort ? 0 : pieces, 0, 1, 0);
+        if (f.blocks < 1) f.blocks = 1;
+        DR_LAUNCH_NAMED("embed_zero_kernel", (embed_zero_kernel<T>), dim3(f.blocks), dim3(256), 0, st, f, (T*)grad + pieces * VZ,
+                        n_tail);
         DR_CHECK_LAUNCH("embed_zero_kernel");
     }
     if (n == 0) return DR_OK;
     EmbedArgs a;
-    a.ids = ids;
     a.n = n;
     a.rows = rows;
-    a.padding = padding;
     a.chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
     a.d = d;
     a.scale = scale;
     a.part = (float*)(ws + L.part);
-    if (n <= EMB_SMALL_N) {
-        int rc = dr_segment_plan(ids, n, (int)sizeof(Id) * 8, rows, ws + L.plan, dr_segment_plan_bytes(n, 1), st);
-        if (rc != DR_OK) return rc;
-        rc = dr_segment_plan_view(ws + L.plan, n, &a.spos, nullptr, nullptr, nullptr);
-        if (rc != DR_OK) return rc;
-        a.keys = nullptr;
+    a.state = (uint8_t*)(ws + L.state);
+    uint2 *pa = (uint2*)(ws + L.pairs_a), *pb = (uint2*)(ws + L.pairs_b);
+    const EmbedKeys<Id> src{(const Id*)ids, rows, padding};
+    if (own_sort) {
+        unsigned bits, passes;
+        embed_digits(rows, &bits, &passes);
+        const int steps = (int)passes * ((n + SRT_TILE - 1) / SRT_TILE > SRT_DIRECT_TILES ? 2 : 1);
+        int step = 0;
+        for (unsigned q = 0; q < passes; ++q) {
+            const int rc = q == 0 ? embed_pass_bits(bits, src, (int)n, 0, ws + L.hist, pb, grad, pieces, &step, steps, st)
+                                  : embed_pass_bits(bits, EmbedPairs{pa}, (int)n, q * bits, ws + L.hist, pb, grad, pieces,
+                                                    &step, steps, st);
+            if (rc != DR_OK) return rc;
+            std::swap(pa, pb);
+        }
+        a.keys = (const uint32_t*)pa;
+        a.spos = a.keys + 1;
+        a.step = 2;
     } else {
         unsigned end_bit = 1;
         while (end_bit < 32 && ((uint64_t)rows >> end_bit) != 0) ++end_bit;     // the sentinel `rows` included
-        const int rc = lsd_sort(EmbedKeys<Id>{(const Id*)ids, rows, padding}, n, end_bit, (uint32_t*)(ws + L.keys_a),
-                                (int32_t*)(ws + L.vals_a), (uint32_t*)(ws + L.keys_b), (int32_t*)(ws + L.vals_b), ws + L.lsd,
+        uint32_t *ka = (uint32_t*)pa, *kb = (uint32_t*)pb;                      // keys, then positions
+        const int rc = lsd_sort(src, n, end_bit, ka, (int32_t*)(ka + n), kb, (int32_t*)(kb + n), ws + L.hist,
                                 (int32_t*)nullptr, st);
         if (rc != DR_OK) return rc;
-        a.keys = (const uint32_t*)(ws + L.keys_b);
-        a.spos = (const int32_t*)(ws + L.vals_b);
+        a.keys = kb;
+        a.spos = kb + n;
+        a.step = 1;
     }
     switch (embed_width(dt, d, gout, grad)) {
         case 8:
-            if constexpr (sizeof(T) == 2) return embed_sum_v<T, Id, 8>(a, gout, grad, st);
-        case 4: return embed_sum_v<T, Id, 4>(a, gout, grad, st);
-        case 2: return embed_sum_v<T, Id, 2>(a, gout, grad, st);
-        default: return embed_sum_v<T, Id, 1>(a, gout, grad, st);
+            if constexpr (sizeof(T) == 2) return embed_sum_v<T, 8>(a, gout, grad, st);
+        case 4: return embed_sum_v<T, 4>(a, gout, grad, st);
+        case 2: return embed_sum_v<T, 2>(a, gout, grad, st);
+        default: return embed_sum_v<T, 1>(a, gout, grad, st);
     }
 }
 }  // namespace dr

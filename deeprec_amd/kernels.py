@@ -3,6 +3,7 @@
 Every function takes CUDA(HIP) tensors, validates shapes / dtypes / contiguity on the host
 (the kernels assume them), and enqueues on torch's current stream.
 """
+import array
 import collections
 import ctypes as C
 
@@ -1139,7 +1140,11 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # DR_F32, D
 
 
 def _req_half(t, name, ndim=None, dtype=None):
-    """A tensor of one of DTYPES (or of exactly `dtype`): contiguous, on the current device."""
+    """A tensor of one of DTYPES (or of exactly `dtype`): contiguous, on the current device.  The usual case is settled by
+    one expression of cheap calls (these wrappers run in front of kernels of a few microseconds); _req names the fault."""
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == torch._C._cuda_getDevice() and t.is_contiguous()
+            and (t.dtype in DTYPES if dtype is None else t.dtype == dtype) and (ndim is None or t.dim() == ndim)):
+        return t
     if dtype is None:
         if isinstance(t, torch.Tensor) and t.dtype not in DTYPES:
             raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
@@ -1147,53 +1152,74 @@ def _req_half(t, name, ndim=None, dtype=None):
     return _req(t, dtype, name, ndim)
 
 
+def _raw_stream():
+    """_stream() as a plain integer."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _at(t):
+    """Address of a tensor, or None."""
+    return t.data_ptr() if t is not None else None
+
+
 # ------------------------------------------------------------------ global gradient norm and clipping
 def _norm_list(tensors, name):
-    tensors = list(tensors)
-    for i, t in enumerate(tensors):
-        _req_half(t, "%s[%d]" % (name, i))
-    n = len(tensors)
-    return tensors, (C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_int64 * n)(*[t.numel() for t in tensors]), \
-        (C.c_int32 * n)(*[DTYPES[t.dtype] for t in tensors])
+    """(addresses, element counts, types) of a tensor list, as arrays the C side reads.  Checked as a whole -- at a
+    hundred tensors a check of each by name costs more than the kernels."""
+    try:
+        where = set(map(torch.Tensor.get_device, tensors))                # -1: the CPU
+        good = -1 not in where and where <= {torch._C._cuda_getDevice()} and all(map(torch.Tensor.is_contiguous, tensors))
+        dts = [DTYPES[t.dtype] for t in tensors] if good else None
+    except (TypeError, AttributeError, KeyError):
+        dts = None
+    if dts is None:
+        for i, t in enumerate(tensors):
+            _req_half(t, "%s[%d]" % (name, i))
+        raise TypeError("%s must be a list of tensors" % name)
+    return (array.array("Q", map(torch.Tensor.data_ptr, tensors)), array.array("q", map(torch.Tensor.numel, tensors)),
+            array.array("i", dts))
 
 
-def _norm_ws(n, device):
-    return torch.empty(check(_abi.lib().dr_global_norm_bytes(n), "dr_global_norm_bytes"), dtype=torch.uint8, device=device)
+def _addr(a):
+    return a.buffer_info()[0]
+
+
+def _norm_call(ins, counts, dts, outs, clip_norm):
+    n, dev = len(ins), torch._C._cuda_getDevice()
+    lib = _abi.lib()
+    need = check(lib.dr_global_norm_bytes(n), "dr_global_norm_bytes")
+    norm = torch.empty(1, dtype=torch.float32, device="cuda")
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    check(lib.dr_clip_global_norm(_addr(ins), _addr(outs) if outs is not None else None, _addr(counts), _addr(dts), n,
+                                  clip_norm, norm.data_ptr(), ws.data_ptr(), need,
+                                  torch._C._cuda_getCurrentRawStream(dev)), "dr_clip_global_norm")
+    return norm
 
 
 def global_norm(tensors):
     """tf.global_norm: sqrt of the sum of all squared elements of a list of float32 / float16 / bfloat16 tensors, as a
     float32 device tensor [1] (no host synchronisation)."""
-    tensors, ins, counts, dts = _norm_list(tensors, "tensors")
-    dev = tensors[0].device if tensors else torch.device("cuda", torch._C._cuda_getDevice())
-    norm = torch.empty(1, dtype=torch.float32, device=dev)
-    ws = _norm_ws(len(tensors), dev)
-    check(_abi.lib().dr_clip_global_norm(ins, None, counts, dts, len(tensors), 1.0, _ptr(norm), _ptr(ws), ws.numel(),
-                                         _stream()), "dr_clip_global_norm")
-    return norm
+    ins, counts, dts = _norm_list(list(tensors), "tensors")
+    return _norm_call(ins, counts, dts, None, 1.0)
 
 
 def clip_by_global_norm(tensors, clip_norm, out=None):
     """tf.clip_by_global_norm: (list of t * clip_norm / max(norm, clip_norm), norm [1] float32 on the device).  float32,
     float16 and bfloat16 tensors may be mixed; each is read twice and written once.  out: the tensors to write (same
-    shapes and types; the list itself clips in place); None: new ones.  No host synchronisation."""
-    tensors, ins, counts, dts = _norm_list(tensors, "tensors")
+    sizes and types; the list itself clips in place); None: new ones.  No host synchronisation."""
+    tensors = list(tensors)
+    ins, counts, dts = _norm_list(tensors, "tensors")
     if out is None:
         out = [torch.empty_like(t) for t in tensors]
+        outs = array.array("Q", map(torch.Tensor.data_ptr, out))
     else:
         out = list(out)
         if len(out) != len(tensors):
             raise ValueError("clip_by_global_norm: %d tensors but %d outputs" % (len(tensors), len(out)))
-        for i, (o, t) in enumerate(zip(out, tensors)):
-            if _req_half(o, "out[%d]" % i, dtype=t.dtype).shape != t.shape:
-                raise ValueError("clip_by_global_norm: out[%d] must be shaped like tensor %d" % (i, i))
-    dev = tensors[0].device if tensors else torch.device("cuda", torch._C._cuda_getDevice())
-    norm = torch.empty(1, dtype=torch.float32, device=dev)
-    ws = _norm_ws(len(tensors), dev)
-    outs = (C.c_void_p * len(out))(*[o.data_ptr() for o in out])
-    check(_abi.lib().dr_clip_global_norm(ins, outs, counts, dts, len(tensors), float(clip_norm), _ptr(norm), _ptr(ws),
-                                         ws.numel(), _stream()), "dr_clip_global_norm")
-    return out, norm
+        outs, ocounts, odts = _norm_list(out, "out")
+        if odts != dts or ocounts != counts:
+            raise ValueError("clip_by_global_norm: out must have the tensors' sizes and types")
+    return out, _norm_call(ins, counts, dts, outs, float(clip_norm))
 
 
 # ------------------------------------------------------------------ embedding lookup with scaling
@@ -1202,11 +1228,12 @@ def embed_forward(table, ids, scale=1.0):
     table's type, rounded once.  Ids outside the table give zero rows, as gather() does."""
     table = _req_half(table, "table", 2)
     ids, bits = _ids(ids, "ids")
-    if table.shape[0] < 1 or table.shape[1] < 1:
+    rows, d = table.shape
+    if rows < 1 or d < 1:
         raise ValueError("embed_forward: the table is empty")
-    out = torch.empty(tuple(ids.shape) + (table.shape[1],), dtype=table.dtype, device=table.device)
-    check(_abi.lib().dr_embed_forward(_ptr(table), table.shape[0], table.shape[1], DTYPES[table.dtype], _ptr(ids),
-                                      ids.numel(), bits, float(scale), _ptr(out), _stream()), "dr_embed_forward")
+    out = table.new_empty(ids.shape + (d,))
+    check(_abi.lib().dr_embed_forward(table.data_ptr(), rows, d, DTYPES[table.dtype], ids.data_ptr(), ids.numel(), bits,
+                                      scale, out.data_ptr(), _raw_stream()), "dr_embed_forward")
     return out
 
 
@@ -1216,18 +1243,19 @@ def embed_backward(gout, ids, rows, scale=1.0, padding_idx=None):
     padding_idx or outside [0, rows) contribute nothing."""
     gout = _req_half(gout, "gout")
     ids, bits = _ids(ids, "ids")
-    if gout.dim() < 1 or tuple(gout.shape[:-1]) != tuple(ids.shape):
+    if gout.dim() < 1 or gout.shape[:-1] != ids.shape:
         raise ValueError("embed_backward: gout must be shaped like ids plus one dim, got %s for ids %s"
                          % (tuple(gout.shape), tuple(ids.shape)))
     n, d, rows = ids.numel(), gout.shape[-1], int(rows)
     pad = -1 if padding_idx is None else int(padding_idx)
     if padding_idx is not None and not 0 <= pad < rows:
         raise ValueError("embed_backward: padding_idx %d is outside the table of %d rows" % (pad, rows))
-    need = check(_abi.lib().dr_embed_backward_bytes(n, d), "dr_embed_backward_bytes")
-    grad = torch.empty((rows, d), dtype=gout.dtype, device=gout.device)
+    lib = _abi.lib()
+    need = check(lib.dr_embed_backward_bytes(n, d), "dr_embed_backward_bytes")
+    grad = gout.new_empty((rows, d))
     ws = torch.empty(need, dtype=torch.uint8, device=gout.device)
-    check(_abi.lib().dr_embed_backward(_ptr(gout), n, d, DTYPES[gout.dtype], _ptr(ids), bits, rows, float(scale), pad,
-                                       _ptr(grad), _ptr(ws), ws.numel(), _stream()), "dr_embed_backward")
+    check(lib.dr_embed_backward(gout.data_ptr(), n, d, DTYPES[gout.dtype], ids.data_ptr(), bits, rows, scale, pad,
+                                grad.data_ptr(), ws.data_ptr(), need, _raw_stream()), "dr_embed_backward")
     return grad
 
 

@@ -38,7 +38,8 @@ def _ids(n, rows, idt, g, bad=False):
 
 # ---- embedding -------------------------------------------------------------------------------------------------------
 EMBED = [(1, 1, 1), (7, 3, 5), (1683, 150, 5000), (50, 128, 4096), (50, 128, 4097), (300, 256, 9000), (9, 100, 20000),
-         (100001, 64, 70001), (5, 1030, 300), (70000, 7, 33)]
+         (100001, 64, 70001), (5, 1030, 300), (70000, 7, 33), (200, 6, 20000), (1500000, 2, 30000), (5000000, 4, 40001),
+         (3000, 3, 300000)]
 
 
 @gpu
