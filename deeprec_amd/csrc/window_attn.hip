@@ -21,7 +21,7 @@ namespace dr {
 
 constexpr int WA_MAX_D = 256, WA_MAX_SINKS = 64;
 constexpr int WA_BK = 32;              // keys (queries in the dK / dV kernels) per tile
-constexpr float WA_LOG2E = 1.44269504088896340736f;
+constexpr float WA_LOG2E = 1.44269504088896340736f, WA_LN2 = 0.69314718055994530942f;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <class T>
@@ -45,11 +45,15 @@ constexpr int lds_ld() {
     return DP + (sizeof(T) == 2 ? 8 : 4);
 }
 
-// 8 elements at p of which the first n exist (the rest: 0); al = bytes that every row start is aligned to
+// How rows are read: in pieces of 16 bytes (D a multiple of 8, every row start on the 16-byte grid), in words of 4, or one
+// 16-bit element at a time.  Loads are never under a condition -- each would wait for the one before -- but go to a clamped
+// place, and what does not exist is cleared when the value is used.
+enum { WA_PIECES = 0, WA_WORDS = 1, WA_ELEMS = 2 };
 template <class T>
-__device__ __forceinline__ Oct<T> load_oct(const T* p, int n, int al) {
+__device__ __forceinline__ Oct<T> load_oct(const T* row, int c, int D, int mode) {
     Oct<T> r;
-    if (n >= 8 && al >= 16) {
+    if (mode == WA_PIECES) {
+        const T* p = row + (c < D ? c : 0);
         if constexpr (sizeof(T) == 2) {
             r = *reinterpret_cast<const Oct<T>*>(p);
         } else {
@@ -60,25 +64,38 @@ __device__ __forceinline__ Oct<T> load_oct(const T* p, int n, int al) {
                 r[4 + e] = y[e];
             }
         }
-    } else if (n >= 8 && al >= 4) {
-        typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        typename std::conditional<sizeof(T) == 2, u32x4, u32x8>::type w;
+    } else if (sizeof(T) == 4 || mode == WA_WORDS) {            // D is even for 16-bit types
+        constexpr int N = (int)sizeof(T) * 2, P = 4 / (int)sizeof(T);   // words, elements per word
+        typedef uint32_t words __attribute__((ext_vector_type(N)));
+        words w;
 #pragma unroll
-        for (int e = 0; e < (int)sizeof(T) * 2; ++e) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+        for (int e = 0; e < N; ++e) w[e] = *reinterpret_cast<const uint32_t*>(row + (c + e * P < D ? c + e * P : 0));
         r = __builtin_bit_cast(Oct<T>, w);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = e < n ? p[e] : (T)0.0f;
+        for (int e = 0; e < 8; ++e) r[e] = row[c + e < D ? c + e : 0];
     }
     return r;
 }
+// the first n elements, zeros behind them (pieces: all or nothing)
 template <class T>
-__device__ __forceinline__ Oct<T> zero_oct() {
-    Oct<T> r;
+__device__ __forceinline__ Oct<T> keep_oct(const Oct<T>& r, int n, int mode) {
+    constexpr int N = (int)sizeof(T) * 2;
+    typedef uint32_t words __attribute__((ext_vector_type(N)));
+    if (mode == WA_PIECES) {
+        words w = __builtin_bit_cast(words, r);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = (T)0.0f;
-    return r;
+        for (int e = 0; e < N; ++e) w[e] = n > 0 ? w[e] : 0u;
+        return __builtin_bit_cast(Oct<T>, w);
+    }
+    Oct<T> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = e < n ? r[e] : (T)0.0f;
+    return o;
+}
+__device__ __forceinline__ int clamp_row(int row, int lo, int hi) {   // a row that exists, inside [lo, hi) if that is not empty
+    if (hi <= lo) return 0;
+    return row < lo ? lo : (row >= hi ? hi - 1 : row);
 }
 template <class T>
 __device__ __forceinline__ void lds_store_oct(T* p, const Oct<T>& r) {
@@ -142,6 +159,18 @@ __device__ __forceinline__ Oct<T> to_oct(const f32x4& a, const f32x4& b) {
     return r;
 }
 
+// over the four lane groups that share a query: every lane gets the maximum / the sum
+__device__ __forceinline__ float groups_max(float x) {
+    const int lane = threadIdx.x & 63;
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_ds_bpermute((lane ^ 16) << 2, __float_as_int(x))));
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_ds_bpermute((lane ^ 32) << 2, __float_as_int(x))));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+    const int lane = threadIdx.x & 63;
+    x += __int_as_float(__builtin_amdgcn_ds_bpermute((lane ^ 16) << 2, __float_as_int(x)));
+    return x + __int_as_float(__builtin_amdgcn_ds_bpermute((lane ^ 32) << 2, __float_as_int(x)));
+}
+
 struct WinStride {
     int64_t b, l, h;
 };
@@ -149,10 +178,11 @@ struct WinArgs {
     const void *q, *k, *v, *out, *gout;
     WinStride qs, ks, vs;      // elements; out and gout are contiguous [B, L, Hq, D]
     int B, L, Hq, Hkv, D, W, S;
-    int tiles;                 // workgroups along the sequence
+    int tiles, ktiles;         // workgroups along the sequence: 64 queries, 32 keys each
     float scale;
     const int32_t *begin, *end;
-    int al, alg;               // alignment in bytes of the rows of q, k, v / of out, gout
+    int mode, modeg;           // how rows of q, k, v / of out, gout are read
+    int wide;                  // rows of out, dq take stores of four elements
     float *lse, *delta;        // [B, Hq, L]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
     int chunks;
@@ -167,42 +197,136 @@ __device__ __forceinline__ void history(const int32_t* begin, const int32_t* end
 __device__ __forceinline__ void win_range(const WinArgs& a, int b, int& lo, int& hi) {
     history(a.begin, a.end, b, a.L, lo, hi);
 }
-__device__ __forceinline__ bool win_visible(const WinArgs& a, int q, int k, int lo) {
-    return k >= lo && k <= q && (q - k < a.W || k - lo < a.S);
+// the keys a query sees through the window are [first, first + count); count 0: none
+__device__ __forceinline__ void win_span(const WinArgs& a, int q, bool ok, int lo, int& first, int& count) {
+    first = q - a.W + 1 > lo ? q - a.W + 1 : lo;
+    count = ok ? q - first + 1 : 0;
 }
 
-// ---- staging of a 32-row tile by 256 threads: rows row0 .. row0 + 31 of the sequence, those outside [lo, hi) as zeros ----
-template <class T, int DP>
+// ---- staging of an R-row tile by 256 threads: rows t0 .. t0 + R - 1 of the sequence, those outside [lo, hi) as zeros ----
+// A thread's places in the tile stay the same, so their offsets are worked out once and a tile inside [lo, hi) costs one
+// 64-bit add per piece; only tiles at the ends clamp rows and clear what does not exist.
+template <class T, int DP, int R, bool FAST>
 struct Stage {
-    static constexpr int OCTS = WA_BK * DP / 8, N = (OCTS + 255) / 256, LD = lds_ld<T, DP>();
+    static constexpr int OCTS = R * DP / 8, N = (OCTS + 255) / 256, LD = lds_ld<T, DP>();
+    const T* base;
+    int64_t ld, off[N];
+    int lo, hi, D, mode, t0;
     Oct<T> r[N];
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int lo, int hi, int D, int al) {
+    __device__ __forceinline__ static int place(int n) {
+        const int o = (int)threadIdx.x + n * 256;
+        return OCTS % 256 == 0 || o < OCTS ? o : OCTS - 1;
+    }
+    __device__ __forceinline__ static int row(int n) { return place(n) / (DP / 8); }
+    __device__ __forceinline__ static int col(int n) { return place(n) % (DP / 8) * 8; }
+    __device__ __forceinline__ void init(const T* base_, int64_t ld_, int lo_, int hi_, int D_, int mode_) {
+        base = base_;
+        ld = ld_;
+        lo = lo_;
+        hi = hi_;
+        D = D_;
+        mode = mode_;
+        t0 = 0;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int o = (int)threadIdx.x + n * 256, row = row0 + o / (DP / 8), c = o % (DP / 8) * 8;
-            if ((OCTS % 256 == 0 || o < OCTS) && row >= lo && row < hi && c < D)
-                r[n] = load_oct<T>(base + row * ld + c, D - c, al);
-            else
-                r[n] = zero_oct<T>();
+        for (int n = 0; n < N; ++n) off[n] = row(n) * ld + (col(n) < D ? col(n) : 0);
+    }
+    __device__ __forceinline__ bool inside() const { return t0 >= lo && t0 + R <= hi; }
+    template <int MODE>
+    __device__ __forceinline__ void load_edge() {
+#pragma unroll
+        for (int n = 0; n < N; ++n) r[n] = load_oct<T>(base + (int64_t)clamp_row(t0 + row(n), lo, hi) * ld, col(n), D, MODE);
+    }
+    __device__ __forceinline__ void load(int t) {
+        t0 = t;
+        if (FAST && inside()) {
+            const T* p = base + (int64_t)t0 * ld;
+#pragma unroll
+            for (int n = 0; n < N; ++n) r[n] = load_oct<T>(p + off[n], 0, 8, WA_PIECES);
+        } else if (FAST || mode == WA_PIECES) {                // one branch around all loads, not one around each
+            load_edge<WA_PIECES>();
+        } else if (mode == WA_WORDS) {
+            load_edge<WA_WORDS>();
+        } else {
+            load_edge<WA_ELEMS>();
         }
     }
     __device__ __forceinline__ void store(T* tile) const {
+        if (FAST && inside()) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (OCTS % 256 == 0 || (int)threadIdx.x + n * 256 < OCTS) lds_store_oct<T>(tile + row(n) * LD + col(n), r[n]);
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int o = (int)threadIdx.x + n * 256;
-            if (OCTS % 256 == 0 || o < OCTS) lds_store_oct<T>(tile + o / (DP / 8) * LD + o % (DP / 8) * 8, r[n]);
+            const int at = t0 + row(n);
+            const Oct<T> x = keep_oct<T>(r[n], at >= lo && at < hi ? D - col(n) : 0, FAST ? WA_PIECES : mode);
+            if (OCTS % 256 == 0 || (int)threadIdx.x + n * 256 < OCTS) lds_store_oct<T>(tile + row(n) * LD + col(n), x);
         }
     }
 };
-// the row fragments of 16 rows (lane & 15) straight from memory
-template <class T, int DP>
-__device__ __forceinline__ void load_frags(Oct<T> (&f)[DP / 32], const T* row, bool ok, int D, int al) {
+// the row fragments of 16 rows (lane & 15) straight from memory; row: one that exists
+template <class T, int DP, bool FAST>
+__device__ __forceinline__ void load_frags(Oct<T> (&f)[DP / 32], const T* row, bool ok, int D, int mode) {
     const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-        const int c = 32 * s + 8 * g;
-        f[s] = ok && c < D ? load_oct<T>(row + c, D - c, al) : zero_oct<T>();
+    if (FAST) {
+        D = DP;
+        mode = WA_PIECES;
     }
+    if (mode == WA_PIECES) {
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) f[s] = load_oct<T>(row, 32 * s + 8 * g, D, WA_PIECES);
+    } else if (mode == WA_WORDS) {
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) f[s] = load_oct<T>(row, 32 * s + 8 * g, D, WA_WORDS);
+    } else {
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) f[s] = load_oct<T>(row, 32 * s + 8 * g, D, WA_ELEMS);
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) f[s] = keep_oct<T>(f[s], ok ? D - 32 * s - 8 * g : 0, mode);
+}
+// a 32-row tile staged by one wavefront, eight pieces of it in flight
+template <class T, int DP, bool FAST, class Row>
+__device__ __forceinline__ void wave_stage_rows(T* tile, const T* base, int D, int mode, Row row) {
+    if (FAST) {
+        D = DP;
+        mode = WA_PIECES;
+    }
+    constexpr int LD = lds_ld<T, DP>(), N = WA_BK * DP / 8 / 64, STEP = N < 8 ? N : 8;
+    const int lane = threadIdx.x & 63;
+    auto part = [&](int n0, auto how) {
+        Oct<T> r[STEP];
+#pragma unroll
+        for (int n = 0; n < STEP; ++n) {
+            const int o = lane + (n0 + n) * 64;
+            bool ok;
+            r[n] = load_oct<T>(base + row(o / (DP / 8), ok), o % (DP / 8) * 8, D, decltype(how)::value);
+        }
+#pragma unroll
+        for (int n = 0; n < STEP; ++n) {
+            const int o = lane + (n0 + n) * 64, c = o % (DP / 8) * 8;
+            bool ok;
+            row(o / (DP / 8), ok);
+            lds_store_oct<T>(tile + o / (DP / 8) * LD + c, keep_oct<T>(r[n], ok ? D - c : 0, decltype(how)::value));
+        }
+    };
+#pragma unroll
+    for (int n0 = 0; n0 < N; n0 += STEP) {
+        if (mode == WA_PIECES)
+            part(n0, std::integral_constant<int, WA_PIECES>());
+        else if (mode == WA_WORDS)
+            part(n0, std::integral_constant<int, WA_WORDS>());
+        else
+            part(n0, std::integral_constant<int, WA_ELEMS>());
+    }
+}
+template <class T, int DP, bool FAST>
+__device__ __forceinline__ void wave_stage(T* tile, const T* base, int64_t ld, int row0, int lo, int hi, int D, int mode) {
+    wave_stage_rows<T, DP, FAST>(tile, base, D, mode, [&](int r, bool& ok) {
+        ok = row0 + r >= lo && row0 + r < hi;
+        return (int64_t)clamp_row(row0 + r, lo, hi) * ld;
+    });
 }
 // which key tiles a block of queries [qlo, qhi] needs: the tiles of the first items, then those of the window
 struct KeyTiles {
@@ -231,8 +355,10 @@ template <class T, int DP>
 constexpr int fwd_buffers() {
     return DP * (int)sizeof(T) <= 512 ? 2 : 1;
 }
-template <class T, int DP>
-__global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__ out, float* __restrict__ lse) {
+// Naming the workgroups per CU keeps the accumulators in ordinary registers: left alone the compiler moves all of them to
+// the accumulation registers and back around every tile's rescaling (64 of 350 instructions).
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)sizeof(T) <= 512 ? 2 : 1)) void win_fwd_kernel(WinArgs a, T* __restrict__ out, float* __restrict__ lse) {
     constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
     extern __shared__ char smem[];
     T* kt = reinterpret_cast<T*>(smem);
@@ -247,19 +373,25 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__
     const int qw = q0 + wave * 16, qi = qw + c16;
     const bool q_ok = qi >= lo && qi < hi;
     const int qlo = qw > lo ? qw : lo, qhi = qw + 15 < hi - 1 ? qw + 15 : hi - 1;      // this wavefront's queries
-    Oct<T> qf[DP / 32];
-    load_frags<T, DP>(qf, (const T*)a.q + b * a.qs.b + qi * a.qs.l + h * a.qs.h, q_ok, a.D, a.al);
+    int k_first, k_count;
+    win_span(a, qi, q_ok, lo, k_first, k_count);
     KeyTiles kts;
     kts.set(a, q0 > lo ? q0 : lo, q0 + 63 < hi - 1 ? q0 + 63 : hi - 1, lo);
+    Stage<T, DP, WA_BK, FAST> ks, vs;
+    ks.init(kp, a.ks.l, lo, hi, a.D, a.mode);
+    vs.init(vp, a.vs.l, lo, hi, a.D, a.mode);
+    if (kts.n > 0) {                                           // the first tile and the queries arrive together
+        ks.load(kts.row0(0));
+        vs.load(kts.row0(0));
+    }
+    Oct<T> qf[DP / 32];
+    load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qs.b + (int64_t)clamp_row(qi, lo, hi) * a.qs.l + h * a.qs.h, q_ok, a.D, a.mode);
     f32x4 o[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
     float m = -__builtin_inff(), l = 0.0f;
     const float c = a.scale * WA_LOG2E;
-    Stage<T, DP> ks, vs;
     if (kts.n > 0) {
-        ks.load(kp, a.ks.l, kts.row0(0), lo, hi, a.D, a.al);
-        vs.load(vp, a.vs.l, kts.row0(0), lo, hi, a.D, a.al);
         ks.store(kt);
         vs.store(vt);
     }
@@ -269,8 +401,8 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__
         const T* kc = kt + (NB == 2 ? (n & 1) * TILE : 0);
         const T* vc = vt + (NB == 2 ? (n & 1) * TILE : 0);
         if (n + 1 < kts.n) {
-            ks.load(kp, a.ks.l, kts.row0(n + 1), lo, hi, a.D, a.al);
-            vs.load(vp, a.vs.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+            ks.load(kts.row0(n + 1));
+            vs.load(kts.row0(n + 1));
         }
         if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
             f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -282,28 +414,39 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__
             // a tile that all 16 queries see whole needs no mask
             const bool whole = t0 >= lo && t0 + WA_BK - 1 <= qw && qw >= lo && qw + 15 < hi && qw + 15 - t0 < a.W;
             if (!whole) {
+                const int k0 = t0 + 4 * g;
+                if (t0 < lo + a.S) {                           // the tile holds first items
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(q_ok && win_visible(a, qi, t0 + 16 * x + 4 * g + i, lo))) s[x][i] = -__builtin_inff();
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = k0 + 16 * x + i;
+                            const bool first = ((unsigned)(k - lo) < (unsigned)a.S) & (k <= qi) & q_ok;
+                            s[x][i] = ((unsigned)(k - k_first) < (unsigned)k_count) | first ? s[x][i] : -__builtin_inff();
+                        }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[x][i] = (unsigned)(k0 + 16 * x + i - k_first) < (unsigned)k_count ? s[x][i] : -__builtin_inff();
+                }
             }
             float mt = s[0][0];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[x][i]);
-            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float mn = fmaxf(m, mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
+            mt = groups_max(mt);
+            const float mn = fmaxf(m, mt * c), ms = mn == -__builtin_inff() ? 0.0f : mn;    // m: in units of log 2
+            const float alpha = __builtin_amdgcn_exp2f(m - ms);
             m = mn;
             float sum = 0.0f;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[x][i] = __builtin_amdgcn_exp2f((s[x][i] - ms) * c);
+                    s[x][i] = __builtin_amdgcn_exp2f(fmaf(s[x][i], c, -ms));
                     sum += s[x][i];
                 }
             l = fmaf(l, alpha, sum);
@@ -322,15 +465,14 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__
         }
         __syncthreads();
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = groups_sum(l);
     if (qi >= a.L) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     T* op = out + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
         const int d = 16 * t + 4 * g;
-        if (d + 4 <= a.D && a.alg >= 4 * (int)sizeof(T)) {
+        if (FAST || (d + 4 <= a.D && a.wide)) {
             float r[4] = {o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv};
             store_f32<T, 4>(op + d, r);
         } else {
@@ -339,14 +481,30 @@ __global__ __launch_bounds__(256) void win_fwd_kernel(WinArgs a, T* __restrict__
                 if (d + i < a.D) op[d + i] = (T)(o[t][i] * inv);
         }
     }
-    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l > 0.0f ? fmaf(m, a.scale, logf(l)) : -__builtin_inff();
+    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l > 0.0f ? (m + log2f(l)) * WA_LN2 : -__builtin_inff();
 }
 
 // ---- backward: dQ ------------------------------------------------------------------------------------------------------------
-// delta_i = <dO_i, O_i>;  dS = P (dP - delta) scale;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the others.
-template <class T, int DP>
-__global__ __launch_bounds__(256) void win_dq_kernel(WinArgs a, T* __restrict__ dq) {
+// delta_i = sum_j p_ij dP_ij;  dS = P (dP - delta) scale;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the others.
+// dP - delta cancels where one key carries a row, so delta has to be as exact as dP: for fp32 it is <dO_i, O_i>, but a
+// 16-bit O is off by half a step and its P was rounded too (measured: dQ, dK 1.8 times as far from 64 bits as the rounding
+// of the result alone), so 16-bit types run the tiles twice, first for delta from fp32 scores.  dS is split into two 16-bit
+// halves (hi + what hi misses) for the second product: one more matrix instruction instead of another half step lost.
+template <class T>
+__device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>& hi, Oct<T>& lo) {
+    hi = to_oct<T>(a, b);
+    f32x4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = a[e] - (float)hi[e];
+        y[e] = b[e] - (float)hi[4 + e];
+    }
+    lo = to_oct<T>(x, y);
+}
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_dq_kernel(WinArgs a, T* __restrict__ dq) {
     constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
+    constexpr bool TWICE = sizeof(T) == 2;
     extern __shared__ char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + NB * TILE;
@@ -357,51 +515,57 @@ __global__ __launch_bounds__(256) void win_dq_kernel(WinArgs a, T* __restrict__ 
     win_range(a, b, lo, hi);
     const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
     const T* vp = (const T*)a.v + b * a.vs.b + hk * a.vs.h;
-    const int qw = q0 + wave * 16, qi = qw + c16;
+    const int qw = q0 + wave * 16, qi = qw + c16, qc = clamp_row(qi, lo, hi);
     const bool q_ok = qi >= lo && qi < hi;
     const int qlo = qw > lo ? qw : lo, qhi = qw + 15 < hi - 1 ? qw + 15 : hi - 1;
+    int k_first, k_count;
+    win_span(a, qi, q_ok, lo, k_first, k_count);
+    KeyTiles kts;
+    kts.set(a, q0 > lo ? q0 : lo, q0 + 63 < hi - 1 ? q0 + 63 : hi - 1, lo);
+    Stage<T, DP, WA_BK, FAST> ks, vs;
+    ks.init(kp, a.ks.l, lo, hi, a.D, a.mode);
+    vs.init(vp, a.vs.l, lo, hi, a.D, a.mode);
+    if (kts.n > 0) {
+        ks.load(kts.row0(0));
+        vs.load(kts.row0(0));
+    }
     Oct<T> qf[DP / 32], gf[DP / 32];
-    load_frags<T, DP>(qf, (const T*)a.q + b * a.qs.b + qi * a.qs.l + h * a.qs.h, q_ok, a.D, a.al);
-    const int64_t orow = (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
-    load_frags<T, DP>(gf, (const T*)a.gout + orow, q_ok, a.D, a.alg);
+    const int64_t irow = (((int64_t)b * a.L + qc) * a.Hq + h) * a.D, srow = ((int64_t)b * a.Hq + h) * a.L;
+    load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qs.b + (int64_t)qc * a.qs.l + h * a.qs.h, q_ok, a.D, a.mode);
+    load_frags<T, DP, FAST>(gf, (const T*)a.gout + irow, q_ok, a.D, a.modeg);
+    const float lse2 = q_ok ? a.lse[srow + qc] * WA_LOG2E : 0.0f;            // in units of log 2
     float delta = 0.0f;
-    {
+    if constexpr (!TWICE) {
         Oct<T> of[DP / 32];
-        load_frags<T, DP>(of, (const T*)a.out + orow, q_ok, a.D, a.alg);
+        load_frags<T, DP, FAST>(of, (const T*)a.out + irow, q_ok, a.D, a.modeg);
 #pragma unroll
         for (int s = 0; s < DP / 32; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[s][e], delta);
+        delta = groups_sum(delta);
     }
-    delta += __shfl_xor(delta, 16, 64);
-    delta += __shfl_xor(delta, 32, 64);
-    const int64_t srow = ((int64_t)b * a.Hq + h) * a.L + qi;
-    float lse2 = 0.0f;                                       // in units of log 2
-    if (qi < a.L) {
-        if (q_ok) lse2 = a.lse[srow] * WA_LOG2E;
-        if (g == 0) a.delta[srow] = delta;
-    }
-    KeyTiles kts;
-    kts.set(a, q0 > lo ? q0 : lo, q0 + 63 < hi - 1 ? q0 + 63 : hi - 1, lo);
     f32x4 acc[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
     const float c = a.scale * WA_LOG2E;
-    Stage<T, DP> ks, vs;
     if (kts.n > 0) {
-        ks.load(kp, a.ks.l, kts.row0(0), lo, hi, a.D, a.al);
-        vs.load(vp, a.vs.l, kts.row0(0), lo, hi, a.D, a.al);
         ks.store(kt);
         vs.store(vt);
     }
     __syncthreads();
-    for (int n = 0; n < kts.n; ++n) {
-        const int t0 = kts.row0(n);
+    const int total = TWICE ? 2 * kts.n : kts.n;
+    for (int n = 0; n < total; ++n) {
+        const bool first = TWICE && n < kts.n;                               // this run is for delta
+        const int t0 = kts.row0(TWICE && n >= kts.n ? n - kts.n : n);
         const T* kc = kt + (NB == 2 ? (n & 1) * TILE : 0);
         const T* vc = vt + (NB == 2 ? (n & 1) * TILE : 0);
-        if (n + 1 < kts.n) {
-            ks.load(kp, a.ks.l, kts.row0(n + 1), lo, hi, a.D, a.al);
-            vs.load(vp, a.vs.l, kts.row0(n + 1), lo, hi, a.D, a.al);
+        if (n + 1 < total) {
+            const int next = kts.row0(TWICE && n + 1 >= kts.n ? n + 1 - kts.n : n + 1);
+            ks.load(next);
+            vs.load(next);
+        }
+        if (TWICE && n == kts.n) {
+            delta = groups_sum(delta);
         }
         if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
             f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -416,28 +580,59 @@ __global__ __launch_bounds__(256) void win_dq_kernel(WinArgs a, T* __restrict__ 
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -lse2));
-                    if (!whole && !(q_ok && win_visible(a, qi, t0 + 16 * y + 4 * g + i, lo))) p = 0.0f;
-                    s[y][i] = p == 0.0f ? 0.0f : p * (dp[y][i] - delta) * a.scale;
-                }
-            const Oct<T> ds = to_oct<T>(s[0], s[1]);
+                for (int i = 0; i < 4; ++i) s[y][i] = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -lse2));
+            if (!whole) {
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) acc[t] = mma(col_frag<T, LD>(kc, 16 * t), ds, acc[t]);
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = t0 + 16 * y + 4 * g + i;
+                        const bool seen = ((unsigned)(k - k_first) < (unsigned)k_count) |
+                                          (((unsigned)(k - lo) < (unsigned)a.S) & (k <= qi) & q_ok);
+                        s[y][i] = seen ? s[y][i] : 0.0f;
+                        dp[y][i] = seen ? dp[y][i] : 0.0f;     // whatever it was: 0 times a finite number
+                    }
+            }
+            if (first) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) delta = fmaf(s[y][i], dp[y][i], delta);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[y][i] = s[y][i] * ((dp[y][i] - delta) * a.scale);
+                if constexpr (TWICE) {
+                    Oct<T> dh, dl;
+                    split_oct<T>(s[0], s[1], dh, dl);
+#pragma unroll
+                    for (int t = 0; t < DP / 16; ++t) {
+                        const Oct<T> kf = col_frag<T, LD>(kc, 16 * t);
+                        acc[t] = mma(kf, dh, acc[t]);
+                        acc[t] = mma(kf, dl, acc[t]);
+                    }
+                } else {
+                    const Oct<T> ds = to_oct<T>(s[0], s[1]);
+#pragma unroll
+                    for (int t = 0; t < DP / 16; ++t) acc[t] = mma(col_frag<T, LD>(kc, 16 * t), ds, acc[t]);
+                }
+            }
         }
         if (NB == 1) __syncthreads();
-        if (n + 1 < kts.n) {
+        if (n + 1 < total) {
             ks.store(kt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
             vs.store(vt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
         }
         __syncthreads();
     }
     if (qi >= a.L) return;
-    T* op = dq + orow;
+    if (g == 0) a.delta[srow + qi] = delta;
+    T* op = dq + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
         const int d = 16 * t + 4 * g;
-        if (d + 4 <= a.D && a.alg >= 4 * (int)sizeof(T)) {
+        if (FAST || (d + 4 <= a.D && a.wide)) {
             float r[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
             store_f32<T, 4>(op + d, r);
         } else {
@@ -450,11 +645,12 @@ __global__ __launch_bounds__(256) void win_dq_kernel(WinArgs a, T* __restrict__ 
 
 // ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
 // S = Q K^T here, so a lane holds one KEY and four queries of each 16: the A operand of dV = P^T dO and dK = dS^T Q.
-// one (32 queries x 16 keys) step: adds to dk, dv.  far: only what the sinks see beyond the window; else only the window.
+// one (32 queries x 16 keys) step: adds to dk, dv what the queries [q_first, q_first + q_count) give the lane's key (whole:
+// all of them do)
 template <class T, int DP>
 __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* lse2, const float* delta,
-                                          const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int ki, int lo,
-                                          int hi, bool far, bool whole, f32x4 (&dk)[DP / 16], f32x4 (&dv)[DP / 16]) {
+                                          const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int q_first,
+                                          int q_count, bool whole, f32x4 (&dk)[DP / 16], f32x4 (&dv)[DP / 16]) {
     constexpr int LD = lds_ld<T, DP>();
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const float c = a.scale * WA_LOG2E;
@@ -472,85 +668,125 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
         const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 16 * y + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int qi = t0 + 16 * y + 4 * g + i, gap = qi - ki;
-            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i]));
-            if (!whole) {
-                const bool seen = far ? (gap >= a.W && ki - lo < a.S) : (gap >= 0 && gap < a.W);
-                if (!(seen && ki >= lo && qi < hi)) p = 0.0f;
-            }
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i])), d = (dp[y][i] - de[i]) * a.scale;
+            if (!whole && (unsigned)(t0 + 16 * y + 4 * g + i - q_first) >= (unsigned)q_count) p = d = 0.0f;
             s[y][i] = p;
-            dp[y][i] = p == 0.0f ? 0.0f : p * (dp[y][i] - de[i]) * a.scale;
+            dp[y][i] = p * d;
         }
     }
-    const Oct<T> pf = to_oct<T>(s[0], s[1]), df = to_oct<T>(dp[0], dp[1]);
+    const Oct<T> pf = to_oct<T>(s[0], s[1]);
+    if constexpr (sizeof(T) == 2) {
+        Oct<T> dh, dl;
+        split_oct<T>(dp[0], dp[1], dh, dl);
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-        dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
-        dk[t] = mma(df, col_frag<T, LD>(qc, 16 * t), dk[t]);
+        for (int t = 0; t < DP / 16; ++t) {
+            dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
+            const Oct<T> qf = col_frag<T, LD>(qc, 16 * t);
+            dk[t] = mma(dh, qf, dk[t]);
+            dk[t] = mma(dl, qf, dk[t]);
+        }
+    } else {
+        const Oct<T> df = to_oct<T>(dp[0], dp[1]);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
+            dk[t] = mma(df, col_frag<T, LD>(qc, 16 * t), dk[t]);
+        }
     }
 }
 
-// A workgroup takes 64 keys of one key head and walks the queries that see them through the window, head by head of the
-// group (so the group's sum needs no atomics); what the first items get from queries beyond the window comes from
+// A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
+// head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
+// of the queries are added up at the end.  What the first items get from queries beyond the window comes from
 // win_sink_kernel's partial sums, added last and in order.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void win_dkdv_kernel(WinArgs a, T* __restrict__ dk_out, T* __restrict__ dv_out) {
-    constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
+constexpr int dkdv_buffers() {
+    return DP * (int)sizeof(T) <= 256 ? 2 : 1;
+}
+// a second workgroup on the CU is worth more than registers to spare (at D <= 128 in 16 bits, 64 in fp32)
+template <class T, int DP, bool FAST>
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_dkdv_kernel(WinArgs a, T* __restrict__ dk_out, T* __restrict__ dv_out) {
+    constexpr int LD = lds_ld<T, DP>(), NB = dkdv_buffers<T, DP>(), R = 64, TILE = R * LD;
+    constexpr bool AHEAD = DP * (int)sizeof(T) <= 512;       // else the next tile does not fit the registers
     extern __shared__ char smem[];
     T* qt = reinterpret_cast<T*>(smem);
     T* gt = qt + NB * TILE;
-    float* st = reinterpret_cast<float*>(gt + NB * TILE);    // [NB][2][32]: lse2, delta
+    float* st = reinterpret_cast<float*>(gt + NB * TILE);    // [NB][2][64]: lse2, delta
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-    const int k0 = (int)(blockIdx.x % a.tiles) * 64, hk = (int)(blockIdx.x / a.tiles % a.Hkv);
-    const int b = (int)(blockIdx.x / a.tiles / a.Hkv), G = a.Hq / a.Hkv;
+    const int k0 = (int)(blockIdx.x % a.ktiles) * 32, hk = (int)(blockIdx.x / a.ktiles % a.Hkv);
+    const int b = (int)(blockIdx.x / a.ktiles / a.Hkv), G = a.Hq / a.Hkv, half = (wave >> 1) * 32;
     int lo, hi;
     win_range(a, b, lo, hi);
-    const int kw = k0 + wave * 16, ki = kw + c16;
+    const int kw = k0 + (wave & 1) * 16, ki = kw + c16;
     const bool k_ok = ki >= lo && ki < hi;
-    Oct<T> kf[DP / 32], vf[DP / 32];
-    load_frags<T, DP>(kf, (const T*)a.k + b * a.ks.b + ki * a.ks.l + hk * a.ks.h, k_ok, a.D, a.al);
-    load_frags<T, DP>(vf, (const T*)a.v + b * a.vs.b + ki * a.vs.l + hk * a.vs.h, k_ok, a.D, a.al);
-    f32x4 dk[DP / 16], dv[DP / 16];
-#pragma unroll
-    for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
-    const int klo = k0 > lo ? k0 : lo, khi = k0 + 63 < hi - 1 ? k0 + 63 : hi - 1;
+    // the queries that see the key through the window: [ki, ki + q_count)
+    const int q_count = k_ok ? (hi - ki < a.W ? hi - ki : a.W) : 0;
+    const int klo = k0 > lo ? k0 : lo, khi = k0 + 31 < hi - 1 ? k0 + 31 : hi - 1;
     const int qend = klo <= khi ? (khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1) : -1;   // last query
-    const int tq0 = klo / WA_BK, nt = klo <= khi ? qend / WA_BK - tq0 + 1 : 0, total = nt * G;
-    Stage<T, DP> qs, gs;
+    const int tq0 = klo / 32 * 32, nt = klo <= khi ? (qend - tq0) / R + 1 : 0, total = nt * G;
+    Stage<T, DP, R, FAST> qs, gs;
+    qs.init((const T*)a.q + b * a.qs.b + hk * G * a.qs.h, a.qs.l, lo, hi, a.D, a.mode);
+    gs.init((const T*)a.gout + ((int64_t)b * a.L * a.Hq + hk * G) * a.D, (int64_t)a.Hq * a.D, lo, hi, a.D, a.modeg);
     float stat = 0.0f;
-    auto load = [&](int n) {
-        const int h = hk * G + n / nt, t0 = (tq0 + n % nt) * WA_BK;
-        qs.load((const T*)a.q + b * a.qs.b + h * a.qs.h, a.qs.l, t0, lo, hi, a.D, a.al);
-        gs.load((const T*)a.gout + ((int64_t)b * a.L * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, t0, lo, hi, a.D, a.alg);
-        if (threadIdx.x < 64) {
-            const int qi = t0 + (int)(threadIdx.x & 31);
-            const int64_t row = ((int64_t)b * a.Hq + h) * a.L + qi;
-            stat = 0.0f;
-            if (qi >= lo && qi < hi) stat = threadIdx.x < 32 ? a.lse[row] * WA_LOG2E : a.delta[row];
+    int h_next = 0, i_next = 0;                              // next tile: head of the group, place along the sequence
+    auto load = [&]() {
+        const int t0 = tq0 + i_next * R;
+        qs.load(t0);
+        gs.load(t0);
+        if (threadIdx.x < 2 * R) {
+            const int qi = t0 + (int)(threadIdx.x & (R - 1));
+            const int64_t row = ((int64_t)b * a.Hq + hk * G + h_next) * a.L + clamp_row(qi, lo, hi);
+            stat = threadIdx.x < R ? a.lse[row] * WA_LOG2E : a.delta[row];
+            if (qi < lo || qi >= hi) stat = 0.0f;
+        }
+        if (++i_next == nt) {
+            i_next = 0;
+            ++h_next;
+            qs.base += a.qs.h;
+            gs.base += a.D;
         }
     };
     auto store = [&](int buf) {
         qs.store(qt + buf * TILE);
         gs.store(gt + buf * TILE);
-        if (threadIdx.x < 64) st[buf * 64 + threadIdx.x] = stat;
+        if (threadIdx.x < 2 * R) st[buf * 2 * R + threadIdx.x] = stat;
     };
-    if (total > 0) {
-        load(0);
-        store(0);
-    }
+    if (total > 0) load();
+    Oct<T> kf[DP / 32], vf[DP / 32];
+    load_frags<T, DP, FAST>(kf, (const T*)a.k + b * a.ks.b + (int64_t)clamp_row(ki, lo, hi) * a.ks.l + hk * a.ks.h, k_ok, a.D, a.mode);
+    load_frags<T, DP, FAST>(vf, (const T*)a.v + b * a.vs.b + (int64_t)clamp_row(ki, lo, hi) * a.vs.l + hk * a.vs.h, k_ok, a.D, a.mode);
+    f32x4 dk[DP / 16], dv[DP / 16];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
+    if (total > 0) store(0);
     __syncthreads();
-    for (int n = 0; n < total; ++n) {
-        const int t0 = (tq0 + n % nt) * WA_BK, buf = NB == 2 ? n & 1 : 0;
-        if (n + 1 < total) load(n + 1);
-        if (kw <= t0 + WA_BK - 1 && t0 - (kw + 15) < a.W && kw < hi && kw + 15 >= lo) {
-            const bool whole = kw >= lo && kw + 15 <= t0 && t0 + WA_BK - 1 < hi && t0 + WA_BK - 1 - kw < a.W;
-            dkdv_step<T, DP>(a, qt + buf * TILE, gt + buf * TILE, st + buf * 64, st + buf * 64 + 32, kf, vf, t0, ki, lo, hi,
-                             false, whole, dk, dv);
+    for (int n = 0, i = 0; n < total; ++n) {
+        const int t0 = tq0 + i * R + half, buf = NB == 2 ? n & 1 : 0;
+        if (++i == nt) i = 0;
+        if (AHEAD && n + 1 < total) load();
+        if (kw <= t0 + 31 && t0 - (kw + 15) < a.W && t0 < hi && kw < hi && kw + 15 >= lo) {
+            const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
+            dkdv_step<T, DP>(a, qt + buf * TILE + half * LD, gt + buf * TILE + half * LD, st + buf * 2 * R + half,
+                             st + buf * 2 * R + R + half, kf, vf, t0, ki, q_count, whole, dk, dv);
         }
         if (NB == 1) __syncthreads();
+        if (!AHEAD && n + 1 < total) load();
         if (n + 1 < total) store(NB == 2 ? (n + 1) & 1 : 0);
         __syncthreads();
     }
+    // the second query half's sums join the first's over LDS: [key half][2][16][DP] fp32, which the tiles have room for
+    float* red = reinterpret_cast<float*>(smem) + (wave & 1) * 32 * DP;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+        if (wave >= 2) {
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] : dk[t][i];
+        }
+    __syncthreads();
+    if (wave >= 2) return;
     // lane: column d = 16 t + c16 of keys kw + 4 g + i
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -562,11 +798,12 @@ __global__ __launch_bounds__(256) void win_dkdv_kernel(WinArgs a, T* __restrict_
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             const int d = 16 * t + c16;
-            if (d >= a.D) continue;
-            float x = dk[t][i], y = dv[t][i];
+            if (!FAST && d >= a.D) continue;
+            float x = dk[t][i] + red[(4 * g + i) * DP + d], y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
             if (sink) {
                 const int64_t step = 2 * (int64_t)a.S * a.D;
                 const float* p = a.part + ((int64_t)b * a.Hkv + hk) * a.chunks * step + (int64_t)(kk - lo) * a.D + d;
+#pragma unroll 8
                 for (int q = 0; q < a.chunks; ++q) {
                     x += p[q * step];
                     y += p[q * step + (int64_t)a.S * a.D];
@@ -579,14 +816,14 @@ __global__ __launch_bounds__(256) void win_dkdv_kernel(WinArgs a, T* __restrict_
 }
 
 // ---- backward: what the first items get from queries beyond the window ----------------------------------------------------------
-// Every query of a long history sees them, so their sums are split over chunks of 256 queries: NW wavefronts, each with its
+// Every query of a long history sees them, so their sums are split over chunks of 64 queries: NW wavefronts, each with its
 // own tiles of 32 queries in LDS, all on the same 16 first items, added up over LDS in order.
-constexpr int WA_CHUNK = 256;
+constexpr int WA_CHUNK = 64;
 template <class T, int DP>
 constexpr int sink_waves() {
     return DP * (int)sizeof(T) <= 256 ? 4 : (DP * (int)sizeof(T) <= 512 ? 2 : 1);
 }
-template <class T, int DP>
+template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
     constexpr int LD = lds_ld<T, DP>(), TILE = WA_BK * LD, NW = sink_waves<T, DP>();
     extern __shared__ char smem[];
@@ -605,9 +842,10 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
     win_range(a, b, lo, hi);
     const int kw = lo + grp * 16, ki = kw + c16;
     const bool k_ok = ki < hi && ki - lo < a.S;
+    const int q_count = k_ok && hi - ki > a.W ? hi - ki - a.W : 0;        // queries beyond the window: from ki + window on
     Oct<T> kf[DP / 32], vf[DP / 32];
-    load_frags<T, DP>(kf, (const T*)a.k + b * a.ks.b + ki * a.ks.l + hk * a.ks.h, k_ok, a.D, a.al);
-    load_frags<T, DP>(vf, (const T*)a.v + b * a.vs.b + ki * a.vs.l + hk * a.vs.h, k_ok, a.D, a.al);
+    load_frags<T, DP, FAST>(kf, (const T*)a.k + b * a.ks.b + (int64_t)clamp_row(ki, lo, hi) * a.ks.l + hk * a.ks.h, k_ok, a.D, a.mode);
+    load_frags<T, DP, FAST>(vf, (const T*)a.v + b * a.vs.b + (int64_t)clamp_row(ki, lo, hi) * a.vs.l + hk * a.vs.h, k_ok, a.D, a.mode);
     f32x4 dk[DP / 16], dv[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
@@ -618,12 +856,8 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         if (t0 >= hi || t0 + WA_BK - 1 - kw < a.W) continue;
         const T* qp = (const T*)a.q + b * a.qs.b + h * a.qs.h;
         const T* gp = (const T*)a.gout + ((int64_t)b * a.L * a.Hq + h) * a.D;
-        for (int o = lane; o < WA_BK * DP / 8; o += 64) {
-            const int r = o / (DP / 8), cc = o % (DP / 8) * 8, row = t0 + r;
-            const bool ok = row >= lo && row < hi && cc < a.D;
-            lds_store_oct<T>(qt + r * LD + cc, ok ? load_oct<T>(qp + row * a.qs.l + cc, a.D - cc, a.al) : zero_oct<T>());
-            lds_store_oct<T>(gt + r * LD + cc, ok ? load_oct<T>(gp + (int64_t)row * a.Hq * a.D + cc, a.D - cc, a.alg) : zero_oct<T>());
-        }
+        wave_stage<T, DP, FAST>(qt, qp, a.qs.l, t0, lo, hi, a.D, a.mode);
+        wave_stage<T, DP, FAST>(gt, gp, (int64_t)a.Hq * a.D, t0, lo, hi, a.D, a.modeg);
         {
             const int qi = t0 + (lane & 31);
             const int64_t row = ((int64_t)b * a.Hq + h) * a.L + qi;
@@ -633,7 +867,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki, lo, hi, true, false, dk, dv);
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki + a.W, q_count, false, dk, dv);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -676,7 +910,7 @@ struct TokenArgs {
     int B, L, Hq, Hkv, D, W, S, splits, per, hgroups;   // per: 32-key tiles of a workgroup
     float scale;
     const int32_t *begin, *end;
-    int al, alq;
+    int mode, modeq;
     void* out;                                          // [B, Hq, D]
     float* part;                                        // [B, Hq, splits, D + 2]: sum, m, l
 };
@@ -684,7 +918,7 @@ template <class T, int DP>
 constexpr int token_waves() {
     return DP * (int)sizeof(T) <= 256 ? 4 : (DP * (int)sizeof(T) <= 512 ? 2 : 1);
 }
-template <class T, int DP>
+template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
     constexpr int LD = lds_ld<T, DP>(), TILE = WA_BK * LD, NW = token_waves<T, DP>();
     __shared__ __attribute__((aligned(16))) T tiles[NW * TILE];
@@ -705,7 +939,7 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
     const int total = hi > lo ? ns + hi - first : 0;
     const int hq = hg * 16 + c16;                                          // query head inside the group
     Oct<T> qf[DP / 32];
-    load_frags<T, DP>(qf, (const T*)a.q + b * a.qb + (hk * G + hq) * a.qh, hq < G && total > 0, a.D, a.alq);
+    load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qb + (hk * G + (hq < G ? hq : 0)) * a.qh, hq < G && total > 0, a.D, a.modeq);
     const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
     const T* vp = (const T*)a.v + b * a.vs.b + hk * a.vs.h;
     f32x4 o[DP / 16];
@@ -721,14 +955,12 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             const int n = n0 + 16 * y + c16;
-            load_frags<T, DP>(kf[y], kp + pos(n < total ? n : total - 1) * a.ks.l, n < total, a.D, a.al);
+            load_frags<T, DP, FAST>(kf[y], kp + pos(n < total ? n : total - 1) * a.ks.l, n < total, a.D, a.mode);
         }
-#pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {
-            const int oo = lane + 64 * x, r = oo / (DP / 8), cc = oo % (DP / 8) * 8, n = n0 + r;
-            const bool ok = n < total && cc < a.D;
-            lds_store_oct<T>(vt + r * LD + cc, ok ? load_oct<T>(vp + pos(n) * a.vs.l + cc, a.D - cc, a.al) : zero_oct<T>());
-        }
+        wave_stage_rows<T, DP, FAST>(vt, vp, a.D, a.mode, [&](int r, bool& ok) {
+            ok = n0 + r < total;
+            return pos(ok ? n0 + r : total - 1) * a.vs.l;
+        });
         f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
         for (int x = 0; x < DP / 32; ++x)
@@ -742,8 +974,7 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
                 if (n0 + 16 * y + 4 * g + i >= total) s[y][i] = -__builtin_inff();
                 mt = fmaxf(mt, s[y][i]);
             }
-        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        mt = groups_max(mt);
         const float mn = fmaxf(m, mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
         const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
         m = mn;
@@ -766,8 +997,7 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = groups_sum(l);
     // join the wavefronts: common maximum, then sums in order
     if (g == 0) {
         sm[wave][c16] = m;
@@ -845,6 +1075,11 @@ static int row_alignment(int es, std::initializer_list<const void*> bases, std::
     for (int64_t s : strides) bits |= (uint64_t)(s * es);
     return (int)(bits & (~bits + 1)) > 16 ? 16 : (int)(bits & (~bits + 1));
 }
+// al: from row_alignment
+static int row_mode(int es, int D, int al) {
+    if (al >= 16 && D % 8 == 0) return WA_PIECES;
+    return es == 4 || (al >= 4 && D % 2 == 0) ? WA_WORDS : WA_ELEMS;
+}
 static int win_check(const char* who, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype, int64_t window,
                      int32_t sinks, float scale) {
     DR_REQUIRE(dtype_ok(dtype), "%s: dtype %d", who, dtype);
@@ -866,44 +1101,44 @@ static int64_t win_chunks(int64_t L, int64_t window, int32_t sinks) {
     return sinks > 0 && L > window ? (L + WA_CHUNK - 1) / WA_CHUNK : 0;
 }
 
-template <class T, int DP>
+template <class T, int DP, bool FAST>
 static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
     const size_t lds = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
-    int rc = win_lds(win_fwd_kernel<T, DP>, lds);
+    int rc = win_lds(win_fwd_kernel<T, DP, FAST>, lds);
     if (rc != DR_OK) return rc;
-    DR_LAUNCH_NAMED("win_fwd_kernel", (win_fwd_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), lds, st, a,
+    DR_LAUNCH_NAMED("win_fwd_kernel", (win_fwd_kernel<T, DP, FAST>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), lds, st, a,
                     (T*)out, a.lse);
     DR_CHECK_LAUNCH("win_fwd_kernel");
     return DR_OK;
 }
-template <class T, int DP>
+template <class T, int DP, bool FAST>
 static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStream_t st) {
     const size_t tiles = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
-    const size_t lds = tiles + fwd_buffers<T, DP>() * 64 * sizeof(float);
-    int rc = win_lds(win_dq_kernel<T, DP>, tiles);
+    const size_t lds = (size_t)dkdv_buffers<T, DP>() * (2 * 64 * lds_ld<T, DP>() * sizeof(T) + 128 * sizeof(float));
+    int rc = win_lds(win_dq_kernel<T, DP, FAST>, tiles);
     if (rc != DR_OK) return rc;
-    DR_LAUNCH_NAMED("win_dq_kernel", (win_dq_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), tiles, st, a,
+    DR_LAUNCH_NAMED("win_dq_kernel", (win_dq_kernel<T, DP, FAST>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), tiles, st, a,
                     (T*)dq);
     DR_CHECK_LAUNCH("win_dq_kernel");
     if (a.chunks > 0) {
         constexpr int NW = sink_waves<T, DP>();
         const size_t sl = (size_t)NW * (2 * WA_BK * lds_ld<T, DP>() * sizeof(T) + 64 * sizeof(float));
-        rc = win_lds(win_sink_kernel<T, DP>, sl);
+        rc = win_lds(win_sink_kernel<T, DP, FAST>, sl);
         if (rc != DR_OK) return rc;
-        DR_LAUNCH_NAMED("win_sink_kernel", (win_sink_kernel<T, DP>), dim3((unsigned)((a.S + 15) / 16) * a.chunks * a.Hkv * a.B),
+        DR_LAUNCH_NAMED("win_sink_kernel", (win_sink_kernel<T, DP, FAST>), dim3((unsigned)((a.S + 15) / 16) * a.chunks * a.Hkv * a.B),
                         dim3(NW * 64), sl, st, a);
         DR_CHECK_LAUNCH("win_sink_kernel");
     }
-    rc = win_lds(win_dkdv_kernel<T, DP>, lds);
+    rc = win_lds(win_dkdv_kernel<T, DP, FAST>, lds);
     if (rc != DR_OK) return rc;
-    DR_LAUNCH_NAMED("win_dkdv_kernel", (win_dkdv_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hkv * a.B), dim3(256), lds, st, a,
+    DR_LAUNCH_NAMED("win_dkdv_kernel", (win_dkdv_kernel<T, DP, FAST>), dim3((unsigned)a.ktiles * a.Hkv * a.B), dim3(256), lds, st, a,
                     (T*)dk, (T*)dv);
     DR_CHECK_LAUNCH("win_dkdv_kernel");
     return DR_OK;
 }
-template <class T, int DP>
+template <class T, int DP, bool FAST>
 static int win_token_launch(const TokenArgs& a, hipStream_t st) {
-    DR_LAUNCH_NAMED("win_token_kernel", (win_token_kernel<T, DP>), dim3((unsigned)a.splits * a.hgroups * a.Hkv * a.B),
+    DR_LAUNCH_NAMED("win_token_kernel", (win_token_kernel<T, DP, FAST>), dim3((unsigned)a.splits * a.hgroups * a.Hkv * a.B),
                     dim3(64 * token_waves<T, DP>()), 0, st, a);
     DR_CHECK_LAUNCH("win_token_kernel");
     if (a.splits > 1) {
@@ -913,11 +1148,11 @@ static int win_token_launch(const TokenArgs& a, hipStream_t st) {
     }
     return DR_OK;
 }
-// workgroups per sequence and key head, 32-key tiles each: 2 workgroups per CU, none below 128 keys
+// workgroups per sequence and key head, 32-key tiles each: 2 workgroups per CU, none below 256 keys
 static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int* splits, int* per) {
     const int64_t tiles = (keys + WA_BK - 1) / WA_BK, rows = B * Hkv * hgroups;
     int64_t s = (512 + rows - 1) / rows;
-    if (s > tiles / 4) s = tiles / 4;
+    if (s > tiles / 8) s = tiles / 8;
     if (s > 128) s = 128;
     if (s < 1) s = 1;
     *per = (int)((tiles + s - 1) / s);
@@ -925,11 +1160,12 @@ static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int* spli
 }
 static int64_t token_keys(int64_t L, int64_t window, int32_t sinks) { return window >= L ? L : (window + sinks < L ? window + sinks : L); }
 
-#define WIN_BY_D(T, launch, ...)                                    \
-    return a.D <= 32    ? launch<T, 32>(__VA_ARGS__)                \
-           : a.D <= 64  ? launch<T, 64>(__VA_ARGS__)                \
-           : a.D <= 128 ? launch<T, 128>(__VA_ARGS__)               \
-                        : launch<T, 256>(__VA_ARGS__)
+// FAST: the head dim fills its tile and rows are read in 16-byte pieces (no column checks anywhere)
+#define WIN_BY_D(T, fast, launch, ...)                                                                        \
+    return a.D <= 32    ? ((fast) && a.D == 32 ? launch<T, 32, true>(__VA_ARGS__) : launch<T, 32, false>(__VA_ARGS__))   \
+           : a.D <= 64  ? ((fast) && a.D == 64 ? launch<T, 64, true>(__VA_ARGS__) : launch<T, 64, false>(__VA_ARGS__))   \
+           : a.D <= 128 ? ((fast) && a.D == 128 ? launch<T, 128, true>(__VA_ARGS__) : launch<T, 128, false>(__VA_ARGS__)) \
+                        : launch<T, 256, false>(__VA_ARGS__)
 }  // namespace dr
 
 extern "C" int32_t dr_window_attn_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -962,12 +1198,15 @@ extern "C" int32_t dr_window_attn_forward(const void* q, const int64_t* q_stride
     a.end = end;
     a.lse = lse;
     a.tiles = (int)((L + 63) / 64);
+    a.ktiles = (int)((L + 31) / 32);
     DR_REQUIRE((int64_t)a.tiles * Hq * B < (1ll << 31), "dr_window_attn_forward: too many workgroups");
-    a.al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
-    a.alg = row_alignment(es, {out}, {(int64_t)D});
-    DR_REQUIRE(a.al >= es && a.alg >= es, "dr_window_attn_forward: a pointer is not aligned to its element size");
+    const int al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    const int alg = row_alignment(es, {out}, {(int64_t)D});
+    DR_REQUIRE(al >= es && alg >= es, "dr_window_attn_forward: a pointer is not aligned to its element size");
+    a.mode = row_mode(es, D, al);
+    a.wide = alg >= 4 * es;
     hipStream_t st = (hipStream_t)stream;
-#define WIN_FWD(T) WIN_BY_D(T, win_fwd_launch, a, out, st)
+#define WIN_FWD(T) WIN_BY_D(T, a.mode == WA_PIECES && a.wide, win_fwd_launch, a, out, st)
     DR_BY_DTYPE(dtype, WIN_FWD);
 #undef WIN_FWD
 }
@@ -1022,14 +1261,18 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.part = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
     a.chunks = (int)win_chunks(L, window, sinks);
     a.tiles = (int)((L + 63) / 64);
-    DR_REQUIRE((int64_t)a.tiles * Hq * B < (1ll << 31) && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < (1ll << 31),
+    a.ktiles = (int)((L + 31) / 32);
+    DR_REQUIRE((int64_t)a.ktiles * Hq * B < (1ll << 31) && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < (1ll << 31),
                "dr_window_attn_backward: too many workgroups");
-    a.al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
-    a.alg = row_alignment(es, {out, gout, dq}, {(int64_t)D});
-    DR_REQUIRE(a.al >= es && a.alg >= es && aligned_to(dk, es) && aligned_to(dv, es),
+    const int al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    const int alg = row_alignment(es, {out, gout, dq}, {(int64_t)D});
+    DR_REQUIRE(al >= es && alg >= es && aligned_to(dk, es) && aligned_to(dv, es),
                "dr_window_attn_backward: a pointer is not aligned to its element size");
+    a.mode = row_mode(es, D, al);
+    a.modeg = row_mode(es, D, alg);
+    a.wide = alg >= 4 * es;
     hipStream_t st = (hipStream_t)stream;
-#define WIN_BWD(T) WIN_BY_D(T, win_bwd_launch, a, dq, dk, dv, st)
+#define WIN_BWD(T) WIN_BY_D(T, a.mode == WA_PIECES && a.modeg == WA_PIECES && a.wide, win_bwd_launch, a, dq, dk, dv, st)
     DR_BY_DTYPE(dtype, WIN_BWD);
 #undef WIN_BWD
 }
@@ -1083,13 +1326,15 @@ extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides,
     a.scale = scale;
     a.begin = begin;
     a.end = end;
-    a.al = row_alignment(es, {k, v}, {a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
-    a.alq = row_alignment(es, {q}, {a.qb, a.qh});
-    DR_REQUIRE(a.al >= es && a.alq >= es && aligned_to(out, es), "dr_window_attn_token: a pointer is not aligned to its element size");
+    const int al = row_alignment(es, {k, v}, {a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
+    const int alq = row_alignment(es, {q}, {a.qb, a.qh});
+    DR_REQUIRE(al >= es && alq >= es && aligned_to(out, es), "dr_window_attn_token: a pointer is not aligned to its element size");
+    a.mode = row_mode(es, D, al);
+    a.modeq = row_mode(es, D, alq);
     a.out = out;
     a.part = (float*)ws;
     hipStream_t st = (hipStream_t)stream;
-#define WIN_TOK(T) WIN_BY_D(T, win_token_launch, a, st)
+#define WIN_TOK(T) WIN_BY_D(T, a.mode == WA_PIECES && a.modeq == WA_PIECES, win_token_launch, a, st)
     DR_BY_DTYPE(dtype, WIN_TOK);
 #undef WIN_TOK
 }
