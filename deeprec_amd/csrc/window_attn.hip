@@ -786,29 +786,38 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
                     red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] : dk[t][i];
         }
     __syncthreads();
+    const int far = a.chunks > 0 && klo <= khi && k0 < lo + a.S ? (lo + a.S < khi + 1 ? lo + a.S : khi + 1) - klo : 0;
+    if (far > 0) {                                           // workgroup-uniform: first items klo .. klo + far - 1
+        const int64_t step = 2 * (int64_t)a.S * a.D;
+        const float* p = a.part + ((int64_t)b * a.Hkv + hk) * a.chunks * step + (int64_t)(klo - lo) * a.D;
+        for (int e = threadIdx.x; e < 2 * far * a.D; e += 256) {
+            const int which = e / (far * a.D), r = e - which * far * a.D, key = klo - k0 + r / a.D, d = r % a.D;
+            const float* pe = p + (int64_t)which * a.S * a.D + r;
+            float x = 0.0f;
+            for (int q0 = 0; q0 < a.chunks; q0 += 16) {      // 16 chunks requested together
+                float v[16];
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] = pe[(q0 + q < a.chunks ? q0 + q : 0) * step];
+#pragma unroll
+                for (int q = 0; q < 16; ++q) x += q0 + q < a.chunks ? v[q] : 0.0f;
+            }
+            reinterpret_cast<float*>(smem)[(key >> 4) * 32 * DP + which * 16 * DP + (key & 15) * DP + d] += x;
+        }
+        __syncthreads();
+    }
     if (wave >= 2) return;
     // lane: column d = 16 t + c16 of keys kw + 4 g + i
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int kk = kw + 4 * g + i;
         if (kk >= a.L) continue;
-        const bool sink = a.chunks > 0 && kk >= lo && kk < hi && kk - lo < a.S;
         T* ko = dk_out + (((int64_t)b * a.L + kk) * a.Hkv + hk) * a.D;
         T* vo = dv_out + (((int64_t)b * a.L + kk) * a.Hkv + hk) * a.D;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             const int d = 16 * t + c16;
             if (!FAST && d >= a.D) continue;
-            float x = dk[t][i] + red[(4 * g + i) * DP + d], y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
-            if (sink) {
-                const int64_t step = 2 * (int64_t)a.S * a.D;
-                const float* p = a.part + ((int64_t)b * a.Hkv + hk) * a.chunks * step + (int64_t)(kk - lo) * a.D + d;
-#pragma unroll 8
-                for (int q = 0; q < a.chunks; ++q) {
-                    x += p[q * step];
-                    y += p[q * step + (int64_t)a.S * a.D];
-                }
-            }
+            const float x = dk[t][i] + red[(4 * g + i) * DP + d], y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
             ko[d] = (T)x;
             vo[d] = (T)y;
         }
