@@ -472,10 +472,10 @@ constexpr int LP_WAVE_V = 2048;
 extern "C" int64_t dr_item_logprobs_bytes(int64_t N, int64_t V, int32_t K) {
     using namespace dr;
     if (N < 0 || V < 1 || V > 0x7FFFFFFF || K < 0 || K > LP_MAX_K) return DR_ERR_ARG;
-    if (N == 0 || V <= LP_WAVE_V) return 256;
+    if (N == 0 || V <= LP_WAVE_V) return 0;
     int splits, seg;
     logp_split(N, (int)V, LP_FILL, &splits, &seg);
-    if (splits == 1) return 256;
+    if (splits == 1) return 0;
     return align_up(N * splits * 16, 256) + align_up(N * splits * 4 * (int64_t)K * 8, 256);
 }
 
@@ -494,10 +494,11 @@ extern "C" int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64
     DR_REQUIRE(logits && entropy && lse && (T == 0 || (targets && logp)) && (K == 0 || (top_idx && top_logp)),
                "dr_item_logprobs_forward: NULL pointer");
     DR_REQUIRE(aligned_to(logits, dtype_size(dtype)), "dr_item_logprobs_forward: logits not aligned to the element size");
-    DR_REQUIRE(ws && aligned_to(ws, 256), "dr_item_logprobs_forward: workspace is NULL or not 256-byte aligned");
-    if (ws_bytes < dr_item_logprobs_bytes(N, V, K))
-        DR_FAIL(DR_ERR_WORKSPACE, "dr_item_logprobs_forward: workspace %lld < required %lld", (long long)ws_bytes,
-                (long long)dr_item_logprobs_bytes(N, V, K));
+    const int64_t need = dr_item_logprobs_bytes(N, V, K);
+    DR_REQUIRE(need == 0 || ws != nullptr, "dr_item_logprobs_forward: workspace is NULL");
+    DR_REQUIRE(aligned_to(ws, 256), "dr_item_logprobs_forward: workspace is not 256-byte aligned");
+    if (ws_bytes < need)
+        DR_FAIL(DR_ERR_WORKSPACE, "dr_item_logprobs_forward: workspace %lld < required %lld", (long long)ws_bytes, (long long)need);
     hipStream_t st = (hipStream_t)stream;
     LogpArgs a;
     a.x = logits;

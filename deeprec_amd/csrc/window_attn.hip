@@ -1089,6 +1089,10 @@ static int row_mode(int es, int D, int al) {
     if (al >= 16 && D % 8 == 0) return WA_PIECES;
     return es == 4 || (al >= 4 && D % 2 == 0) ? WA_WORDS : WA_ELEMS;
 }
+// the stride of a dim of one entry is never used and may be anything
+static WinStride win_stride(const int64_t* s, int64_t B, int64_t L, int64_t H) {
+    return WinStride{B > 1 ? s[0] : 0, L > 1 ? s[1] : 0, H > 1 ? s[2] : 0};
+}
 static int win_check(const char* who, int64_t B, int64_t L, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype, int64_t window,
                      int32_t sinks, float scale) {
     DR_REQUIRE(dtype_ok(dtype), "%s: dtype %d", who, dtype);
@@ -1192,9 +1196,9 @@ extern "C" int32_t dr_window_attn_forward(const void* q, const int64_t* q_stride
     a.q = q;
     a.k = k;
     a.v = v;
-    a.qs = WinStride{q_strides[0], q_strides[1], q_strides[2]};
-    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
-    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.qs = win_stride(q_strides, B, L, Hq);
+    a.ks = win_stride(k_strides, B, L, Hkv);
+    a.vs = win_stride(v_strides, B, L, Hkv);
     a.B = (int)B;
     a.L = (int)L;
     a.Hq = Hq;
@@ -1252,9 +1256,9 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.v = v;
     a.out = out;
     a.gout = gout;
-    a.qs = WinStride{q_strides[0], q_strides[1], q_strides[2]};
-    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
-    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.qs = win_stride(q_strides, B, L, Hq);
+    a.ks = win_stride(k_strides, B, L, Hkv);
+    a.vs = win_stride(v_strides, B, L, Hkv);
     a.B = (int)B;
     a.L = (int)L;
     a.Hq = Hq;
@@ -1291,10 +1295,10 @@ extern "C" int64_t dr_window_attn_token_bytes(int64_t B, int64_t L, int32_t Hq, 
     using namespace dr;
     int rc = win_check("dr_window_attn_token_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
     if (rc != DR_OK) return rc;
-    if (B == 0) return 256;
+    if (B == 0) return 0;
     int splits, per;
     token_split(B, Hkv, (Hq / Hkv + 15) / 16, token_keys(L, window, sinks), &splits, &per);
-    return splits > 1 ? align_up(B * Hq * splits * ((int64_t)D + 2) * 4, 256) : 256;
+    return splits > 1 ? align_up(B * Hq * splits * ((int64_t)D + 2) * 4, 256) : 0;
 }
 
 extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1307,8 +1311,9 @@ extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides,
     if (rc != DR_OK) return rc;
     if (B == 0) return DR_OK;
     DR_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides, "dr_window_attn_token: NULL pointer");
-    DR_REQUIRE(ws && aligned_to(ws, 256), "dr_window_attn_token: workspace is NULL or not 256-byte aligned");
     const int64_t need = dr_window_attn_token_bytes(B, L, Hq, Hkv, D, window, sinks);
+    DR_REQUIRE(need == 0 || ws != nullptr, "dr_window_attn_token: workspace is NULL");
+    DR_REQUIRE(aligned_to(ws, 256), "dr_window_attn_token: workspace is not 256-byte aligned");
     if (ws_bytes < need)
         DR_FAIL(DR_ERR_WORKSPACE, "dr_window_attn_token: workspace %lld < required %lld", (long long)ws_bytes, (long long)need);
     const int es = dtype_size(dtype);
@@ -1317,10 +1322,10 @@ extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides,
     a.q = q;
     a.k = k;
     a.v = v;
-    a.qb = q_strides[0];
-    a.qh = q_strides[1];
-    a.ks = WinStride{k_strides[0], k_strides[1], k_strides[2]};
-    a.vs = WinStride{v_strides[0], v_strides[1], v_strides[2]};
+    a.qb = B > 1 ? q_strides[0] : 0;
+    a.qh = Hq > 1 ? q_strides[1] : 0;
+    a.ks = win_stride(k_strides, B, L, Hkv);
+    a.vs = win_stride(v_strides, B, L, Hkv);
     a.B = (int)B;
     a.L = (int)L;
     a.Hq = Hq;

@@ -1268,21 +1268,25 @@ def _logits(t, targets):
     """logits [N, V] with unit column stride (any row stride >= V); targets None, [N] or [N, T]."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("logits must be a CUDA/HIP tensor (deeprec_amd has no CPU path)")
-    _on_current_device(t, "logits")
+    if t.get_device() != torch._C._cuda_getDevice():
+        _on_current_device(t, "logits")
     if t.dtype not in DTYPES:
         raise TypeError("logits must be float32, float16 or bfloat16, got %s" % t.dtype)
     if t.dim() != 2 or t.shape[1] < 1:
         raise ValueError("logits must be [N, V] with V >= 1, got %s" % (tuple(t.shape),))
     N, V = t.shape
-    ld = t.stride(0) if N > 1 else V
-    if (V > 1 and t.stride(1) != 1) or ld < V:
+    ld, col = t.stride()
+    if N <= 1:
+        ld = V
+    if (V > 1 and col != 1) or ld < V:
         raise ValueError("logits must have unit column stride and rows that do not overlap")
     if targets is None:
         return N, V, ld, None, 32, 0
     targets, bits = _ids(targets, "targets")
-    if targets.dim() not in (1, 2) or targets.shape[0] != N:
-        raise ValueError("targets must be [N] or [N, T], got %s" % (tuple(targets.shape),))
-    T = targets.shape[1] if targets.dim() == 2 else 1
+    shape = targets.shape
+    if len(shape) not in (1, 2) or shape[0] != N:
+        raise ValueError("targets must be [N] or [N, T], got %s" % (tuple(shape),))
+    T = shape[1] if len(shape) == 2 else 1
     if T > LOGP_MAX_T:
         raise ValueError("at most %d targets a row" % LOGP_MAX_T)
     return N, V, ld, targets, bits, T
@@ -1299,15 +1303,17 @@ def item_logprobs_forward(logits, targets=None, K=0):
     if not 0 <= K <= LOGP_MAX_K:
         raise ValueError("K must be 0..%d" % LOGP_MAX_K)
     dev = logits.device
-    logp = torch.empty(targets.shape, dtype=torch.float32, device=dev) if targets is not None else None
     ent = torch.empty(N, dtype=torch.float32, device=dev)
-    lse = torch.empty((N, 2), dtype=torch.float32, device=dev)
+    lse = ent.new_empty((N, 2))
+    logp = ent.new_empty(targets.shape) if targets is not None else None
+    top = ent.new_empty((N, K)) if K else None
     idx = torch.empty((N, K), dtype=torch.int32, device=dev) if K else None
-    top = torch.empty((N, K), dtype=torch.float32, device=dev) if K else None
-    ws = torch.empty(check(_abi.lib().dr_item_logprobs_bytes(N, V, K), "dr_item_logprobs_bytes"), dtype=torch.uint8, device=dev)
-    check(_abi.lib().dr_item_logprobs_forward(_ptr(logits), N, V, ld, DTYPES[logits.dtype], _ptr(targets), bits, T, K,
-                                              _ptr(logp), _ptr(ent), _ptr(lse), _ptr(idx), _ptr(top), _ptr(ws), ws.numel(),
-                                              _stream()), "dr_item_logprobs_forward")
+    lib = _abi.lib()
+    need = check(lib.dr_item_logprobs_bytes(N, V, K), "dr_item_logprobs_bytes")
+    ws = _scratch(need, dev)
+    check(lib.dr_item_logprobs_forward(logits.data_ptr(), N, V, ld, DTYPES[logits.dtype], _at(targets), bits, T, K, _at(logp),
+                                       ent.data_ptr(), lse.data_ptr(), _at(idx), _at(top), _at(ws), need, _raw_stream()),
+          "dr_item_logprobs_forward")
     return LogProbs(logp, ent, lse, idx, top)
 
 
@@ -1315,18 +1321,18 @@ def item_logprobs_backward(logits, targets, lse, entropy, g_logp, g_entropy=None
     """d loss / d logits [N, V] (contiguous, the logits' type) of item_logprobs_forward's logp and entropy: g_logp shaped
     like targets (None without targets), g_entropy [N] or None; lse and entropy as the forward returned them."""
     N, V, ld, targets, bits, T = _logits(logits, targets)
-    if tuple(_req(lse, torch.float32, "lse", 2).shape) != (N, 2):
+    if tuple(_req_half(lse, "lse", 2, torch.float32).shape) != (N, 2):
         raise ValueError("lse must be [N, 2] as item_logprobs_forward returns it")
-    if targets is not None and _req(g_logp, torch.float32, "g_logp").shape != targets.shape:
+    if targets is not None and _req_half(g_logp, "g_logp", None, torch.float32).shape != targets.shape:
         raise ValueError("g_logp must be shaped like targets")
-    if g_entropy is not None and (tuple(_req(g_entropy, torch.float32, "g_entropy", 1).shape) != (N,)
-                                  or tuple(_req(entropy, torch.float32, "entropy", 1).shape) != (N,)):
+    if g_entropy is not None and (tuple(_req_half(g_entropy, "g_entropy", 1, torch.float32).shape) != (N,)
+                                  or tuple(_req_half(entropy, "entropy", 1, torch.float32).shape) != (N,)):
         raise ValueError("g_entropy and entropy must be [N]")
-    out = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
-    check(_abi.lib().dr_item_logprobs_backward(_ptr(logits), N, V, ld, DTYPES[logits.dtype], _ptr(targets), bits, T,
-                                               _ptr(lse), _ptr(entropy) if g_entropy is not None else None,
-                                               _ptr(g_logp) if targets is not None else None, _ptr(g_entropy), _ptr(out),
-                                               _stream()), "dr_item_logprobs_backward")
+    out = _like(logits)
+    check(_abi.lib().dr_item_logprobs_backward(logits.data_ptr(), N, V, ld, DTYPES[logits.dtype], _at(targets), bits, T,
+                                               lse.data_ptr(), entropy.data_ptr() if g_entropy is not None else None,
+                                               g_logp.data_ptr() if targets is not None else None, _at(g_entropy),
+                                               out.data_ptr(), _raw_stream()), "dr_item_logprobs_backward")
     return out
 
 
@@ -1338,37 +1344,56 @@ def _win_tensor(t, name, ndim, dtype=None):
     """An attention operand: any strides, last dim contiguous."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA/HIP tensor (deeprec_amd has no CPU path)" % name)
-    _on_current_device(t, name)
+    if t.get_device() != torch._C._cuda_getDevice():
+        _on_current_device(t, name)
     if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
         raise TypeError("%s must be %s, got %s" % (name, dtype or "float32, float16 or bfloat16", t.dtype))
     if t.dim() != ndim:
         raise ValueError("%s must have %d dims, got shape %s" % (name, ndim, tuple(t.shape)))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    stride = t.stride()
+    if stride[-1] != 1 and t.shape[-1] > 1:
         raise ValueError("%s: the last dim must be contiguous" % name)
-    # the stride of a dim of one entry is never used and may be anything
-    return (C.c_int64 * (ndim - 1))(*[st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])])
+    return stride
 
 
-def _win_mask(B, window, sinks, scale, D, begin, end):
+_WIN_STRIDES = C.c_int64 * 3
+
+
+def _win_operands(q, k, v, q_dims, window, sinks, scale, begin, end):
+    """Checks what the three calls share: strides as C arrays, sizes, mask arguments."""
+    sq = _win_tensor(q, "q", q_dims)
+    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
+    qs, ks = q.shape, k.shape
+    B, L, Hkv, D = ks
+    Hq = qs[-2]
+    if ks != v.shape or qs[0] != B or qs[-1] != D:
+        raise ValueError("q %s, k %s and v %s do not fit" % (tuple(qs), tuple(ks), tuple(v.shape)))
+    if not 1 <= D <= WIN_MAX_D:
+        raise ValueError("head dim must be 1..%d" % WIN_MAX_D)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("%d query heads are no multiple of %d key heads" % (Hq, Hkv))
+    if L < 1:
+        raise ValueError("the sequence dim is empty")
+    if q_dims == 4 and qs[1] != L:
+        raise ValueError("q and k must have the same length, got %d and %d" % (qs[1], L))
     window, sinks = int(window), int(sinks)
     if window < 1 or not 0 <= sinks <= WIN_MAX_SINKS:
         raise ValueError("window must be >= 1 and sinks 0..%d, got %d and %d" % (WIN_MAX_SINKS, window, sinks))
     for name, t in (("begin", begin), ("end", end)):
-        if t is not None and _req(t, torch.int32, name, 1).numel() != B:
+        if t is not None and _req_half(t, name, 1, torch.int32).shape[0] != B:
             raise ValueError("%s must hold one position per sequence" % name)
-    return min(window, 1 << 40), sinks, float(D ** -0.5 if scale is None else scale)
+    return (_WIN_STRIDES(*sq[:-1]), _WIN_STRIDES(*sk[:3]), _WIN_STRIDES(*sv[:3]), B, L, Hq, Hkv, D, DTYPES[q.dtype],
+            window if window < L else L, sinks, float(D ** -0.5 if scale is None else scale))
 
 
-def _win_shapes(q, k, v):
-    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[-1] != k.shape[-1]:
-        raise ValueError("q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if not 1 <= q.shape[-1] <= WIN_MAX_D:
-        raise ValueError("head dim must be 1..%d" % WIN_MAX_D)
-    Hq, Hkv = q.shape[-2], k.shape[-2]
-    if Hkv < 1 or Hq < 1 or Hq % Hkv:
-        raise ValueError("%d query heads are no multiple of %d key heads" % (Hq, Hkv))
-    if k.shape[1] < 1:
-        raise ValueError("the sequence dim is empty")
+def _like(t, shape=None):
+    """A new contiguous tensor of t's type (and shape)."""
+    return torch.empty_like(t) if shape is None and t.is_contiguous() else t.new_empty(t.shape if shape is None else shape)
+
+
+def _scratch(need, device):
+    """A workspace, or None where the call needs none."""
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
 
 
 def window_attn_forward(q, k, v, window, sinks=0, scale=None, begin=None, end=None):
@@ -1377,17 +1402,11 @@ def window_attn_forward(q, k, v, window, sinks=0, scale=None, begin=None, end=No
     Key j is visible to query i iff begin <= j <= i < end and (i - j < window or j - begin < sinks); begin / end: int32 [B]
     (None: the whole row), so padding may stand on either side; padded positions are never read and give zero rows.
     scale None: D ** -0.5.  Returns (out [B, L, Hq, D], lse float32 [B, Hq, L])."""
-    sq = _win_tensor(q, "q", 4)
-    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
-    _win_shapes(q, k, v)
-    B, L, Hq, D = q.shape
-    if k.shape[1] != L:
-        raise ValueError("q and k must have the same length, got %d and %d" % (L, k.shape[1]))
-    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
-    out = torch.empty((B, L, Hq, D), dtype=q.dtype, device=q.device)
+    sq, sk, sv, B, L, Hq, Hkv, D, dt, window, sinks, scale = _win_operands(q, k, v, 4, window, sinks, scale, begin, end)
+    out = _like(q)
     lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device)
-    check(_abi.lib().dr_window_attn_forward(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, B, L, Hq, k.shape[2], D, DTYPES[q.dtype],
-                                            window, sinks, scale, _ptr(begin), _ptr(end), _ptr(out), _ptr(lse), _stream()),
+    check(_abi.lib().dr_window_attn_forward(q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, B, L, Hq, Hkv, D, dt, window,
+                                            sinks, scale, _at(begin), _at(end), out.data_ptr(), lse.data_ptr(), _raw_stream()),
           "dr_window_attn_forward")
     return out, lse
 
@@ -1395,27 +1414,20 @@ def window_attn_forward(q, k, v, window, sinks=0, scale=None, begin=None, end=No
 def window_attn_backward(q, k, v, out, lse, gout, window, sinks=0, scale=None, begin=None, end=None):
     """(dq [B, L, Hq, D], dk, dv [B, L, Hkv, D]) of window_attn_forward for d loss / d out = gout; out and lse as it
     returned them.  Bit-repeatable."""
-    sq = _win_tensor(q, "q", 4)
-    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
-    _win_shapes(q, k, v)
-    B, L, Hq, D = q.shape
-    if k.shape[1] != L:
-        raise ValueError("q and k must have the same length, got %d and %d" % (L, k.shape[1]))
+    sq, sk, sv, B, L, Hq, Hkv, D, dt, window, sinks, scale = _win_operands(q, k, v, 4, window, sinks, scale, begin, end)
     for name, t in (("out", out), ("gout", gout)):
-        if _req(t, q.dtype, name, 4).shape != q.shape:
+        if _req_half(t, name, 4, q.dtype).shape != q.shape:
             raise ValueError("%s must be shaped like q" % name)
-    if tuple(_req(lse, torch.float32, "lse", 3).shape) != (B, Hq, L):
+    if tuple(_req_half(lse, "lse", 3, torch.float32).shape) != (B, Hq, L):
         raise ValueError("lse must be [B, Hq, L]")
-    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
-    Hkv = k.shape[2]
-    dq = torch.empty((B, L, Hq, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((B, L, Hkv, D), dtype=q.dtype, device=q.device)
-    dv = torch.empty((B, L, Hkv, D), dtype=q.dtype, device=q.device)
-    ws = torch.empty(check(_abi.lib().dr_window_attn_backward_bytes(B, L, Hq, Hkv, D, window, sinks),
-                           "dr_window_attn_backward_bytes"), dtype=torch.uint8, device=q.device)
-    check(_abi.lib().dr_window_attn_backward(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, _ptr(out), _ptr(lse), _ptr(gout), B, L, Hq,
-                                             Hkv, D, DTYPES[q.dtype], window, sinks, scale, _ptr(begin), _ptr(end), _ptr(dq),
-                                             _ptr(dk), _ptr(dv), _ptr(ws), ws.numel(), _stream()), "dr_window_attn_backward")
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    lib = _abi.lib()
+    ws = _scratch(check(lib.dr_window_attn_backward_bytes(B, L, Hq, Hkv, D, window, sinks), "dr_window_attn_backward_bytes"),
+                  q.device)
+    check(lib.dr_window_attn_backward(q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, out.data_ptr(), lse.data_ptr(),
+                                      gout.data_ptr(), B, L, Hq, Hkv, D, dt, window, sinks, scale, _at(begin), _at(end),
+                                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream()),
+          "dr_window_attn_backward")
     return dq, dk, dv
 
 
@@ -1423,16 +1435,12 @@ def window_attn_token(q, k, v, window, sinks=0, scale=None, begin=None, end=None
     """The serving form: one new token per sequence.  q [B, Hq, D] stands at position end - 1 of the caches k, v
     [B, L, Hkv, D], which already hold its own key and value; it sees what window_attn_forward's last query sees.
     Returns out [B, Hq, D] (zeros for an empty history)."""
-    sq = _win_tensor(q, "q", 3)
-    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
-    _win_shapes(q, k, v)
-    B, Hq, D = q.shape
-    L, Hkv = k.shape[1], k.shape[2]
-    window, sinks, scale = _win_mask(B, window, sinks, scale, D, begin, end)
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
-    ws = torch.empty(check(_abi.lib().dr_window_attn_token_bytes(B, L, Hq, Hkv, D, window, sinks),
-                           "dr_window_attn_token_bytes"), dtype=torch.uint8, device=q.device)
-    check(_abi.lib().dr_window_attn_token(_ptr(q), sq, _ptr(k), sk, _ptr(v), sv, B, L, Hq, Hkv, D, DTYPES[q.dtype], window,
-                                          sinks, scale, _ptr(begin), _ptr(end), _ptr(out), _ptr(ws), ws.numel(), _stream()),
+    sq, sk, sv, B, L, Hq, Hkv, D, dt, window, sinks, scale = _win_operands(q, k, v, 3, window, sinks, scale, begin, end)
+    out = _like(q)
+    lib = _abi.lib()
+    need = check(lib.dr_window_attn_token_bytes(B, L, Hq, Hkv, D, window, sinks), "dr_window_attn_token_bytes")
+    ws = _scratch(need, q.device)
+    check(lib.dr_window_attn_token(q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, B, L, Hq, Hkv, D, dt, window, sinks,
+                                   scale, _at(begin), _at(end), out.data_ptr(), _at(ws), need, _raw_stream()),
           "dr_window_attn_token")
     return out

@@ -581,7 +581,8 @@ int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype,
  * contiguous -> dq [B, L, Hq, D], dk, dv [B, L, Hkv, D] contiguous, overwritten; sums over a group's heads included; no
  * atomics, bit-repeatable.  ws: dr_window_attn_backward_bytes(...), 256-byte aligned.
  * token: ONE query per sequence, q [B, Hq, D] (strides {batch, head}), at position end[b] - 1 of a cache k, v [B, L, Hkv, D]
- * that already holds its own key and value -> out [B, Hq, D] contiguous.  ws: dr_window_attn_token_bytes(...). */
+ * that already holds its own key and value -> out [B, Hq, D] contiguous.  ws: dr_window_attn_token_bytes(...), 256-byte
+ * aligned (0 bytes: NULL). */
 int32_t dr_window_attn_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                const void* v, const int64_t* v_strides, int64_t B, int64_t L, int32_t Hq, int32_t Hkv,
                                int32_t D, int32_t dtype, int64_t window, int32_t sinks, float scale, const int32_t* begin,
@@ -610,7 +611,7 @@ int32_t dr_window_attn_token(const void* q, const int64_t* q_strides, const void
  *                   by lower index; -1 / -inf behind the last item offered
  * A row without any offered item: logp -inf, entropy 0, lse (-inf, 0), no best items, gradient 0.  A NaN or +inf logit makes
  * the row's logp, entropy and gradients NaN (NaN is never among the best).  ws: dr_item_logprobs_bytes(N, V, K), 256-byte
- * aligned.  backward: g_logp [N, T] and g_entropy [N] (NULL: none) fp32 -> glogits [N, V] contiguous, in the logits' type:
+ * aligned (0 bytes: NULL).  backward: g_logp [N, T] and g_entropy [N] (NULL: none) fp32 -> glogits [N, V] contiguous, in the logits' type:
  *   sum_t g_t [v = target_t] - p_v (sum_t g_t + g_entropy (log p_v + entropy)), rounded once. */
 int64_t dr_item_logprobs_bytes(int64_t N, int64_t V, int32_t K);
 int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64_t V, int64_t ld, int32_t dtype, const void* targets,

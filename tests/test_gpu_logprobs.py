@@ -272,7 +272,10 @@ def test_logprobs_refusals_cpu():
     for i, v in ((0, None), (1, -1), (2, 0), (3, 9), (4, 3), (5, None), (6, 16), (7, 65), (8, 65), (9, None), (10, None),
                  (11, None), (12, None), (14, C.c_void_p(4100)), (0, C.c_void_p(4098))):
         assert call(i, v) == -1, (i, v)
-    assert call(15, 16) == -2
+    wide = [100001 if j in (2, 3) else y for j, y in enumerate(ok)]           # a row split over workgroups needs scratch
+    wide[15] = 16
+    assert lib.dr_item_logprobs_bytes(4, 100001, 3) > 16 and lib.dr_item_logprobs_forward(*wide) == -2
+    assert lib.dr_item_logprobs_bytes(4, 10, 3) == 0
     assert lib.dr_item_logprobs_bytes(-1, 5, 1) < 0 and lib.dr_item_logprobs_bytes(4, 5, 65) < 0
     assert lib.dr_item_logprobs_backward(p, 4, 10, 9, 0, p, 32, 1, p, p, p, p, p, None) == -1
     assert lib.dr_item_logprobs_backward(p, 4, 10, 10, 0, p, 32, 1, p, None, p, p, p, None) == -1
