@@ -10,8 +10,9 @@
 // loop has no workgroup barrier.  Candidates cost nothing on the way: a group of pieces is looked at only if its maximum
 // (needed anyway) reaches the wavefront's threshold, which starts at the K-th best of the lanes' first maxima -- a
 // lower bound of the K-th best -- and rises whenever the list of 256 is cut back to K.
-//   V <= 2048                one wavefront per row (no joining)
-//   many rows                one workgroup of 4 wavefronts per row
+//   V <= 2048, or many rows of up to 16384   one wavefront per row (nothing to join; at 4096 x 3707 fp16 the forward takes
+//                            LPT1 us so, LPT4 us with a workgroup per row)
+//   many longer rows         one workgroup of 4 wavefronts per row
 //   few rows                 the row is split over workgroups; logp_join_kernel adds up their parts
 #include "dr_types.h"
 
@@ -198,13 +199,15 @@ __device__ __forceinline__ Stat scan_row(const T* p, int lo, int hi, int wave, i
         const float m = fmaxf(st.m, mv), d0 = st.m - m, f = lp_exp(d0);
         float z = 0.0f, s = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            if (base + (int64_t)u * waves * 64 >= w_hi) break;          // wavefront-uniform: nothing but padding from here on
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 const float d = x[u][q] - m, e = lp_exp(d);
                 z += e;
                 s = fmaf(e, fmaxf(d, LP_FLOOR), s);
             }
+        }
         st.s = fmaf(f, fmaf(st.z, fmaxf(d0, LP_FLOOR), st.s), s);
         st.z = fmaf(st.z, f, z);
         st.m = m;
@@ -356,9 +359,21 @@ __global__ __launch_bounds__(256) void logp_join_kernel(LogpArgs a) {
     if constexpr (TOP) {
         const int n = a.splits * 4 * a.K;
         const uint64_t* keys = a.pkey + (int64_t)row * n;
-        for (int i0 = wave * 64; i0 < n; i0 += 256) {
-            const uint64_t k = i0 + lane < n ? keys[i0 + lane] : 0ull;
-            best.add(k != 0, k, a.K);
+        constexpr int J = 4;                                   // keys a lane requests together
+        for (int i0 = wave * 64 * J; i0 < n; i0 += 256 * J) {
+            uint64_t k[J], top = 0;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int i = i0 + j * 64 + lane;
+                k[j] = keys[i < n ? i : n - 1];
+                if (i >= n) k[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) top = k[j] > top ? k[j] : top;
+            // the K-th best of the lanes' best bounds the K-th best of all: hardly more than K candidates remain
+            if (i0 < 256 * J) best.bound(top ? order_value((uint32_t)(top >> 32)) : -__builtin_inff(), a.K);
+#pragma unroll
+            for (int j = 0; j < J; ++j) best.add(k[j] != 0 && order_value((uint32_t)(k[j] >> 32)) >= best.thr, k[j], a.K);
         }
     }
     __syncthreads();
@@ -379,11 +394,14 @@ struct LogpGradArgs {
     void* dx;                          // [N, V]
 };
 
-template <class T>
+// ROWS rows (or row parts) per workgroup: 4 = a wavefront each, 1 = all four on one
+template <class T, int ROWS>
 __global__ __launch_bounds__(256) void logp_grad_kernel(LogpGradArgs a) {
-    constexpr int V = 16 / (int)sizeof(T), U = 4;
-    const int64_t row = blockIdx.x / a.splits;
-    const int64_t lo = (int64_t)(blockIdx.x % a.splits) * a.seg, hi = lo + a.seg < a.V ? lo + a.seg : a.V;
+    constexpr int V = 16 / (int)sizeof(T), U = 4, NT = 256 / ROWS;
+    const int64_t part = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT, row = part / a.splits;
+    const int tid = threadIdx.x % NT;
+    if (row >= a.N) return;                                 // whole wavefronts; ROWS = 1: never
+    const int64_t lo = part % a.splits * a.seg, hi = lo + a.seg < a.V ? lo + a.seg : a.V;
     const T* p = (const T*)a.x + row * a.ld;
     T* o = (T*)a.dx + row * a.V;
     const float m = a.lse[2 * row], lz = a.lse[2 * row + 1];
@@ -404,11 +422,11 @@ __global__ __launch_bounds__(256) void logp_grad_kernel(LogpGradArgs a) {
     const int off = (int)(((uintptr_t)p & 15) / sizeof(T));
     if (off == (int)(((uintptr_t)o & 15) / sizeof(T))) {
         const int64_t w_lo = (lo + off) / V, w_hi = (hi + off + V - 1) / V;
-        for (int64_t base = w_lo + threadIdx.x; base < w_hi; base += 256 * U) {
+        for (int64_t base = w_lo + tid; base < w_hi; base += NT * U) {
             float x[U][V];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t e = (base + u * 256) * V - off;
+                const int64_t e = (base + u * NT) * V - off;
                 if (e >= lo && e + V <= hi) {
                     load_f32<T, V>(x[u], p + e);
                 } else {
@@ -418,7 +436,8 @@ __global__ __launch_bounds__(256) void logp_grad_kernel(LogpGradArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t e = (base + u * 256) * V - off;
+                const int64_t e = (base + u * NT) * V - off;
+                if (e >= hi) break;
 #pragma unroll
                 for (int q = 0; q < V; ++q) x[u][q] = grad(x[u][q]);
                 if (e >= lo && e + V <= hi) {
@@ -432,21 +451,25 @@ __global__ __launch_bounds__(256) void logp_grad_kernel(LogpGradArgs a) {
         }
     } else {                                               // rows of x and dx lie differently on the 16-byte grid
 #pragma unroll 8
-        for (int64_t e = lo + threadIdx.x; e < hi; e += 256) o[e] = (T)grad((float)p[e]);
+        for (int64_t e = lo + tid; e < hi; e += NT) o[e] = (T)grad((float)p[e]);
     }
     if (a.T == 0) return;
     // the targets' own terms: added before the one rounding, so their elements are written again, by the first of the
-    // entries that name the item (its repeats are summed in list order)
-    __syncthreads();
-    const int t = threadIdx.x;
-    if (t < a.T && !none) {
-        const int64_t v = target(t);
+    // entries that name the item (its repeats are summed in list order) -- after the first writes have arrived
+    if constexpr (ROWS == 1) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (tid < a.T && !none) {
+        const int64_t v = target(tid);
         if (v >= lo && v < hi) {
             float s = 0.0f;
             bool mine = true;
             for (int q = 0; q < a.T; ++q)
                 if (target(q) == v) {
-                    if (q < t) mine = false;
+                    if (q < tid) mine = false;
                     s += a.g[row * a.T + q];
                 }
             if (mine) o[v] = (T)(grad((float)p[v]) + s);
@@ -465,14 +488,14 @@ static void logp_split(int64_t N, int V, int64_t want, int* splits, int* seg) {
     *splits = (int)(((int64_t)V + *seg - 1) / *seg);
 }
 constexpr int64_t LP_FILL = 1024;      // 4 workgroups per CU
-constexpr int LP_WAVE_V = 2048;
+static bool logp_wave_rows(int64_t N, int64_t V) { return V <= 2048 || (V <= 16384 && N >= 2048); }
 
 }  // namespace dr
 
 extern "C" int64_t dr_item_logprobs_bytes(int64_t N, int64_t V, int32_t K) {
     using namespace dr;
     if (N < 0 || V < 1 || V > 0x7FFFFFFF || K < 0 || K > LP_MAX_K) return DR_ERR_ARG;
-    if (N == 0 || V <= LP_WAVE_V) return 0;
+    if (N == 0 || logp_wave_rows(N, V)) return 0;
     int splits, seg;
     logp_split(N, (int)V, LP_FILL, &splits, &seg);
     if (splits == 1) return 0;
@@ -518,7 +541,7 @@ extern "C" int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64
     a.seg = a.V;
     a.pst = nullptr;
     a.pkey = nullptr;
-    if (V <= LP_WAVE_V) {
+    if (logp_wave_rows(N, V)) {
         DR_REQUIRE((N + 3) / 4 < (1ll << 31), "dr_item_logprobs_forward: too many rows");
 #define LP_WAVE(T_)                                                                                                     \
     if (K)                                                                                                              \
@@ -588,13 +611,23 @@ extern "C" int32_t dr_item_logprobs_backward(const void* logits, int64_t N, int6
     a.g = g_logp;
     a.gh = g_entropy;
     a.dx = glogits;
-    logp_split(N, a.V, LP_FILL, &a.splits, &a.seg);
-    DR_REQUIRE(N * a.splits < (1ll << 31), "dr_item_logprobs_backward: too many rows");
     hipStream_t st = (hipStream_t)stream;
+    if (logp_wave_rows(N, V)) {
+        a.splits = 1;
+        a.seg = a.V;
+        DR_REQUIRE((N + 3) / 4 < (1ll << 31), "dr_item_logprobs_backward: too many rows");
 #define LP_GRAD(T_) \
-    DR_LAUNCH_NAMED("logp_grad_kernel", (logp_grad_kernel<T_>), dim3((unsigned)(N * a.splits)), dim3(256), 0, st, a)
-    DR_BY_DTYPE(dtype, LP_GRAD);
+    DR_LAUNCH_NAMED("logp_grad_kernel", (logp_grad_kernel<T_, 4>), dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, a)
+        DR_BY_DTYPE(dtype, LP_GRAD);
 #undef LP_GRAD
+    } else {
+        logp_split(N, a.V, LP_FILL, &a.splits, &a.seg);
+        DR_REQUIRE(N * a.splits < (1ll << 31), "dr_item_logprobs_backward: too many rows");
+#define LP_GRAD(T_) \
+    DR_LAUNCH_NAMED("logp_grad_kernel", (logp_grad_kernel<T_, 1>), dim3((unsigned)(N * a.splits)), dim3(256), 0, st, a)
+        DR_BY_DTYPE(dtype, LP_GRAD);
+#undef LP_GRAD
+    }
     DR_CHECK_LAUNCH("logp_grad_kernel");
     return DR_OK;
 }

@@ -1188,12 +1188,12 @@ def _norm_call(ins, counts, dts, outs, clip_norm):
     n, dev = len(ins), torch._C._cuda_getDevice()
     lib = _abi.lib()
     need = check(lib.dr_global_norm_bytes(n), "dr_global_norm_bytes")
-    norm = torch.empty(1, dtype=torch.float32, device="cuda")
-    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    buf = torch.empty(need // 4 + 1, dtype=torch.float32, device="cuda")       # the workspace, and the norm behind it
+    ws = buf.data_ptr()
     check(lib.dr_clip_global_norm(_addr(ins), _addr(outs) if outs is not None else None, _addr(counts), _addr(dts), n,
-                                  clip_norm, norm.data_ptr(), ws.data_ptr(), need,
-                                  torch._C._cuda_getCurrentRawStream(dev)), "dr_clip_global_norm")
-    return norm
+                                  clip_norm, ws + need, ws, need, torch._C._cuda_getCurrentRawStream(dev)),
+          "dr_clip_global_norm")
+    return buf[need // 4:]
 
 
 def global_norm(tensors):
