@@ -184,6 +184,7 @@ struct WinArgs {
     int mode, modeg;           // how rows of q, k, v / of out, gout are read
     int wide;                  // rows of out, dq take stores of four elements
     float *lse, *delta;        // [B, Hq, L]
+    float* gmax;               // fp16: largest |dO| of every 16 queries [B, Hq, 4 tiles]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
     int chunks;
 };
@@ -485,11 +486,14 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
 }
 
 // ---- backward: dQ ------------------------------------------------------------------------------------------------------------
-// delta_i = sum_j p_ij dP_ij;  dS = P (dP - delta) scale;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the others.
-// dP - delta cancels where one key carries a row, so delta has to be as exact as dP: for fp32 it is <dO_i, O_i>, but a
-// 16-bit O is off by half a step and its P was rounded too (measured: dQ, dK 1.8 times as far from 64 bits as the rounding
-// of the result alone), so 16-bit types run the tiles twice, first for delta from fp32 scores.  dS is split into two 16-bit
-// halves (hi + what hi misses) for the second product: one more matrix instruction instead of another half step lost.
+// dS = P (dP - delta) scale with delta_i = sum_j p_ij dP_ij;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the
+// others.  dP - delta cancels where one key carries a row, so delta has to be as exact as dP.  For fp32 it is <dO_i, O_i>;
+// a 16-bit O is off by half a step and its P was rounded too (measured: dQ, dK 1.8 times as far from 64 bits as the rounding
+// of the result alone).  16-bit types start from that delta_0 and correct it: with r = sum p (dP - delta_0) = delta - delta_0,
+//   dQ = scale (sum p (dP - delta_0) K - r sum p K),
+// r being small, the second sum needs no more than P rounded to 16 bits.  The first one's weights are split into two halves
+// (hi + what hi misses), one more matrix instruction instead of another half step lost.  (Running the tiles twice, first
+// for delta, is as exact and took 77 us where this takes 48 at 4 x 2047 x 8 x 128.)
 template <class T>
 __device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>& hi, Oct<T>& lo) {
     hi = to_oct<T>(a, b);
@@ -501,10 +505,15 @@ __device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>
     }
     lo = to_oct<T>(x, y);
 }
+// power of two that brings x into [1, 2); 1 for 0 and what is not finite
+__device__ __forceinline__ float grad_up(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 255u);
+    return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t)(254 - e) << 23);
+}
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_dq_kernel(WinArgs a, T* __restrict__ dq) {
     constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
-    constexpr bool TWICE = sizeof(T) == 2;
+    constexpr bool FIX = sizeof(T) == 2;                                     // delta is corrected
     extern __shared__ char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + NB * TILE;
@@ -534,8 +543,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qs.b + (int64_t)qc * a.qs.l + h * a.qs.h, q_ok, a.D, a.mode);
     load_frags<T, DP, FAST>(gf, (const T*)a.gout + irow, q_ok, a.D, a.modeg);
     const float lse2 = q_ok ? a.lse[srow + qc] * WA_LOG2E : 0.0f;            // in units of log 2
-    float delta = 0.0f;
-    if constexpr (!TWICE) {
+    float delta = 0.0f, fix = 0.0f;
+    {
         Oct<T> of[DP / 32];
         load_frags<T, DP, FAST>(of, (const T*)a.out + irow, q_ok, a.D, a.modeg);
 #pragma unroll
@@ -544,28 +553,39 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[s][e], delta);
         delta = groups_sum(delta);
     }
-    f32x4 acc[DP / 16];
+    // fp16 has no range for dS of every gradient scale: the rows are brought to dO of about 1 first
+    float up = 1.0f, down = 1.0f;
+    if constexpr (std::is_same<T, f16>::value) {
+        float big = 0.0f;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
+        for (int s = 0; s < DP / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf((float)gf[s][e]));
+        big = groups_max(big);
+        up = grad_up(big);
+        down = 1.0f / up;
+        for (int off = 8; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
+        if (lane == 0) a.gmax[(((int64_t)b * a.Hq + h) * a.tiles + q0 / 64) * 4 + wave] = big;   // of these 16 queries
+    }
+    f32x4 acc[DP / 16], pk[FIX ? DP / 16 : 1];                               // sums of p (dP - delta) K and of p K
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        acc[t] = f32x4{0, 0, 0, 0};
+        if (FIX) pk[t] = f32x4{0, 0, 0, 0};
+    }
     const float c = a.scale * WA_LOG2E;
     if (kts.n > 0) {
         ks.store(kt);
         vs.store(vt);
     }
     __syncthreads();
-    const int total = TWICE ? 2 * kts.n : kts.n;
-    for (int n = 0; n < total; ++n) {
-        const bool first = TWICE && n < kts.n;                               // this run is for delta
-        const int t0 = kts.row0(TWICE && n >= kts.n ? n - kts.n : n);
+    for (int n = 0; n < kts.n; ++n) {
+        const int t0 = kts.row0(n);
         const T* kc = kt + (NB == 2 ? (n & 1) * TILE : 0);
         const T* vc = vt + (NB == 2 ? (n & 1) * TILE : 0);
-        if (n + 1 < total) {
-            const int next = kts.row0(TWICE && n + 1 >= kts.n ? n + 1 - kts.n : n + 1);
-            ks.load(next);
-            vs.load(next);
-        }
-        if (TWICE && n == kts.n) {
-            delta = groups_sum(delta);
+        if (n + 1 < kts.n) {
+            ks.load(kts.row0(n + 1));
+            vs.load(kts.row0(n + 1));
         }
         if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
             f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -593,52 +613,59 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
                         dp[y][i] = seen ? dp[y][i] : 0.0f;     // whatever it was: 0 times a finite number
                     }
             }
-            if (first) {
+            const Oct<T> p = to_oct<T>(s[0], s[1]);
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) delta = fmaf(s[y][i], dp[y][i], delta);
-            } else {
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[y][i] = s[y][i] * ((dp[y][i] - delta) * a.scale);
-                if constexpr (TWICE) {
-                    Oct<T> dh, dl;
-                    split_oct<T>(s[0], s[1], dh, dl);
-#pragma unroll
-                    for (int t = 0; t < DP / 16; ++t) {
-                        const Oct<T> kf = col_frag<T, LD>(kc, 16 * t);
-                        acc[t] = mma(kf, dh, acc[t]);
-                        acc[t] = mma(kf, dl, acc[t]);
-                    }
-                } else {
-                    const Oct<T> ds = to_oct<T>(s[0], s[1]);
-#pragma unroll
-                    for (int t = 0; t < DP / 16; ++t) acc[t] = mma(col_frag<T, LD>(kc, 16 * t), ds, acc[t]);
+                for (int i = 0; i < 4; ++i) {
+                    s[y][i] *= (dp[y][i] - delta) * up;
+                    fix += s[y][i];
                 }
+            if constexpr (FIX) {
+                Oct<T> dh, dl;
+                split_oct<T>(s[0], s[1], dh, dl);
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    const Oct<T> kf = col_frag<T, LD>(kc, 16 * t);
+                    acc[t] = mma(kf, dh, acc[t]);
+                    pk[t] = mma(kf, p, pk[t]);
+                    acc[t] = mma(kf, dl, acc[t]);
+                }
+            } else {
+                const Oct<T> ds = to_oct<T>(s[0], s[1]);
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) acc[t] = mma(col_frag<T, LD>(kc, 16 * t), ds, acc[t]);
             }
         }
         if (NB == 1) __syncthreads();
-        if (n + 1 < total) {
+        if (n + 1 < kts.n) {
             ks.store(kt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
             vs.store(vt + (NB == 2 ? ((n + 1) & 1) * TILE : 0));
         }
         __syncthreads();
     }
+    if constexpr (FIX) {
+        fix = groups_sum(fix);
+        delta += fix * down;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(-fix, pk[t][i], acc[t][i]);
+    }
     if (qi >= a.L) return;
     if (g == 0) a.delta[srow + qi] = delta;
+    down *= a.scale;
     T* op = dq + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
         const int d = 16 * t + 4 * g;
         if (FAST || (d + 4 <= a.D && a.wide)) {
-            float r[4] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+            float r[4] = {acc[t][0] * down, acc[t][1] * down, acc[t][2] * down, acc[t][3] * down};
             store_f32<T, 4>(op + d, r);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (d + i < a.D) op[d + i] = (T)acc[t][i];
+                if (d + i < a.D) op[d + i] = (T)(acc[t][i] * down);
         }
     }
 }
@@ -650,7 +677,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 template <class T, int DP>
 __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* lse2, const float* delta,
                                           const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int q_first,
-                                          int q_count, bool whole, f32x4 (&dk)[DP / 16], f32x4 (&dv)[DP / 16]) {
+                                          int q_count, bool whole, float dscale, f32x4 (&dk)[DP / 16],
+                                          f32x4 (&dv)[DP / 16]) {
     constexpr int LD = lds_ld<T, DP>();
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const float c = a.scale * WA_LOG2E;
@@ -668,7 +696,7 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
         const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 16 * y + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i])), d = (dp[y][i] - de[i]) * a.scale;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i])), d = (dp[y][i] - de[i]) * dscale;
             if (!whole && (unsigned)(t0 + 16 * y + 4 * g + i - q_first) >= (unsigned)q_count) p = d = 0.0f;
             s[y][i] = p;
             dp[y][i] = p * d;
@@ -695,6 +723,18 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
     }
 }
 
+// The factor that brings the gradients of the queries [q0, q1] of a group's heads to about 1 (fp16; see win_dq_kernel)
+template <class T>
+__device__ __forceinline__ float grad_scale(const WinArgs& a, int b, int h0, int heads, int q0, int q1) {
+    if constexpr (!std::is_same<T, f16>::value) return 1.0f;
+    float big = 0.0f;
+    const int r0 = q0 / 16, n = q1 / 16 - r0 + 1;
+    for (int i = threadIdx.x & 63; i < n * heads; i += 64)
+        big = fmaxf(big, a.gmax[((int64_t)b * a.Hq + h0 + i / n) * a.tiles * 4 + r0 + i % n]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
+    return grad_up(big);
+}
 // A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
 // head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
 // of the queries are added up at the end.  What the first items get from queries beyond the window comes from
@@ -724,6 +764,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     const int klo = k0 > lo ? k0 : lo, khi = k0 + 31 < hi - 1 ? k0 + 31 : hi - 1;
     const int qend = klo <= khi ? (khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1) : -1;   // last query
     const int tq0 = klo / 32 * 32, nt = klo <= khi ? (qend - tq0) / R + 1 : 0, total = nt * G;
+    const float up = total > 0 ? grad_scale<T>(a, b, hk * G, G, tq0, qend) : 1.0f;
     Stage<T, DP, R, FAST> qs, gs;
     qs.init((const T*)a.q + b * a.qs.b + hk * G * a.qs.h, a.qs.l, lo, hi, a.D, a.mode);
     gs.init((const T*)a.gout + ((int64_t)b * a.L * a.Hq + hk * G) * a.D, (int64_t)a.Hq * a.D, lo, hi, a.D, a.modeg);
@@ -767,7 +808,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         if (kw <= t0 + 31 && t0 - (kw + 15) < a.W && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
             dkdv_step<T, DP>(a, qt + buf * TILE + half * LD, gt + buf * TILE + half * LD, st + buf * 2 * R + half,
-                             st + buf * 2 * R + R + half, kf, vf, t0, ki, q_count, whole, dk, dv);
+                             st + buf * 2 * R + R + half, kf, vf, t0, ki, q_count, whole, a.scale * up, dk, dv);
         }
         if (NB == 1) __syncthreads();
         if (!AHEAD && n + 1 < total) load();
@@ -775,6 +816,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         __syncthreads();
     }
     // the second query half's sums join the first's over LDS: [key half][2][16][DP] fp32, which the tiles have room for
+    const float down = 1.0f / up;
     float* red = reinterpret_cast<float*>(smem) + (wave & 1) * 32 * DP;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
@@ -801,7 +843,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 #pragma unroll
                 for (int q = 0; q < 16; ++q) x += q0 + q < a.chunks ? v[q] : 0.0f;
             }
-            reinterpret_cast<float*>(smem)[(key >> 4) * 32 * DP + which * 16 * DP + (key & 15) * DP + d] += x;
+            reinterpret_cast<float*>(smem)[(key >> 4) * 32 * DP + which * 16 * DP + (key & 15) * DP + d] += which ? x : x * up;
         }
         __syncthreads();
     }
@@ -817,7 +859,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         for (int t = 0; t < DP / 16; ++t) {
             const int d = 16 * t + c16;
             if (!FAST && d >= a.D) continue;
-            const float x = dk[t][i] + red[(4 * g + i) * DP + d], y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
+            const float x = (dk[t][i] + red[(4 * g + i) * DP + d]) * down, y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
             ko[d] = (T)x;
             vo[d] = (T)y;
         }
@@ -859,6 +901,8 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
     const int first = chunk * WA_CHUNK, per = WA_CHUNK / WA_BK;
+    const float up = grad_scale<T>(a, b, hk * G, G, first, first + WA_CHUNK <= a.L ? first + WA_CHUNK - 1 : a.L - 1);
+    const float down = 1.0f / up;
     for (int n = wave; n < per * G; n += NW) {
         const int h = hk * G + n / per, t0 = first + n % per * WA_BK;
         // wavefront-uniform: no query of the tile is both in the history and beyond the window of the group's first key
@@ -876,7 +920,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki + a.W, q_count, false, dk, dv);
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki + a.W, q_count, false, a.scale * up, dk, dv);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -894,7 +938,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float* r = red + (4 * g + i) * DP + 16 * t + c16;
-                        const float x = which ? dv[t][i] : dk[t][i];
+                        const float x = which ? dv[t][i] : dk[t][i] * down;
                         *r = w == 0 ? x : *r + x;
                     }
             }
@@ -1229,7 +1273,8 @@ extern "C" int64_t dr_window_attn_backward_bytes(int64_t B, int64_t L, int32_t H
     using namespace dr;
     int rc = win_check("dr_window_attn_backward_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
     if (rc != DR_OK) return rc;
-    return align_up(B * Hq * L * 4, 256) + align_up(B * Hkv * win_chunks(L, window, sinks) * 2 * sinks * D * 4, 256) + 256;
+    return align_up(B * Hq * L * 4, 256) + align_up(B * Hq * ((L + 63) / 64) * 16, 256) +
+           align_up(B * Hkv * win_chunks(L, window, sinks) * 2 * sinks * D * 4, 256) + 256;
 }
 
 extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1271,7 +1316,8 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.end = end;
     a.lse = const_cast<float*>(lse);
     a.delta = (float*)ws;
-    a.part = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
+    a.gmax = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
+    a.part = (float*)((char*)a.gmax + align_up(B * Hq * ((L + 63) / 64) * 16, 256));
     a.chunks = (int)win_chunks(L, window, sinks);
     a.tiles = (int)((L + 63) / 64);
     a.ktiles = (int)((L + 31) / 32);

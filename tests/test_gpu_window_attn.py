@@ -326,3 +326,25 @@ def test_window_attention_refusals_cpu():
     assert call(6, 0) == 0
     assert lib.dr_window_attn_backward_bytes(2, 4, 3, 2, 8, 3, 1) == -1
     assert lib.dr_window_attn_token(p, s, p, s, p, s, 1, 9000, 2, 1, 8, 0, 9000, 1, 0.5, None, None, p, p, 16, None) == -2
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** 10])
+def test_gradient_scale(dev, dt, size):
+    """Gradients far from 1 (none or a large loss scale): a power of two in, the same power of two out, to the type's range.
+    With dO = size * (exact in every type), dQ, dK, dV are size times those of dO up to rounding where neither is subnormal;
+    compared with the 64-bit restatement at the usual limits, and 2^-24 (half the smallest subnormal) for fp16."""
+    from deeprec_amd import kernels as Kn
+    B, L, Hq, Hkv, D, W, S = 2, 150, 4, 2, 64, 40, 3
+    q, k, v, go, begin, end = _inputs(B, L, Hq, Hkv, D, dt, 21)
+    go = (go.float() * size).to(dt)
+    scale = D ** -0.5
+    r = _ref(q, k, v, go, _visible(B, L, W, S, begin, end), scale)
+    _, lq, lk, lv = _limits(r, dt, D, Hq // Hkv, scale)
+    d = lambda t: t.to(dev)
+    mask = dict(window=W, sinks=S, begin=d(begin), end=d(end))
+    out, lse = Kn.window_attn_forward(d(q), d(k), d(v), **mask)
+    for name, x, ref, lim in zip(("dq", "dk", "dv"), Kn.window_attn_backward(d(q), d(k), d(v), out, lse, d(go), **mask),
+                                 (r["dq"], r["dk"], r["dv"]), (lq, lk, lv)):
+        _within(name, x, ref, lim + (2.0 ** -24 if dt == torch.float16 else 0.0))
