@@ -210,8 +210,10 @@ class TFOptimizer:
     NSLOTS = {"sgd": 0, "adam": 2, "adagrad": 1, "rmsprop": 2}
 
     def __init__(self, kind, learning_rate, eps=None, beta1=0.9, beta2=0.999, initial_accumulator_value=0.1,
-                 rho=0.9, momentum=0.0):
+                 rho=0.9, momentum=0.0, clip_norm=None):
+        """clip_norm: the global norm that clip() holds a step's gradients to (None: clip() does nothing)."""
         self.kind, self.lr = kind, float(learning_rate)
+        self.clip_norm = None if clip_norm is None else float(clip_norm)
         self.eps = float(eps if eps is not None else (1e-8 if kind == "adam" else 1e-10))
         self.beta1, self.beta2, self.acc0, self.rho, self.momentum = beta1, beta2, initial_accumulator_value, rho, momentum
         self.step_count = 0
@@ -286,6 +288,27 @@ class TFOptimizer:
                             eps=self.eps, rho=self.rho, momentum=self.momentum,
                             reg=0.0 if reg_dev is not None else float(reg), reg_mode=reg_mode,
                             alpha_dev=self._dev.alpha if self._dev is not None else None, reg_dev=reg_dev)
+
+    def clip(self, tables, params=()):
+        """Hold the global norm of one step's gradients -- the rows recorded for `tables` and the .grad of `params` -- to
+        clip_norm before they are applied (tf.clip_by_global_norm; dr_clip_global_norm).  As with TensorFlow's
+        IndexedSlices every recorded row counts, duplicates not combined; the L2 terms that the optimizer kernels add
+        are not part of the norm.  Returns the norm (a device tensor [1]) or None without clip_norm."""
+        if self.clip_norm is None:
+            return None
+        if any(t.shard is not None for t in tables):
+            raise ValueError("TFOptimizer.clip: the rows of a sharded table are spread over ranks; their global norm is not "
+                             "offered")
+        rows = [(t, i) for t in tables for i in range(len(t.pending))]
+        grads = [p for p in params if p.grad is not None]
+        # new tensors, not in place: autograd may hand the same gradient to two lookups
+        out, norm = K.clip_by_global_norm([t.pending[i][1] for t, i in rows] + [p.grad.contiguous() for p in grads],
+                                          self.clip_norm)
+        for (t, i), r in zip(rows, out):
+            t.pending[i] = (t.pending[i][0], r)
+        for p, g in zip(grads, out[len(rows):]):
+            p.grad = g
+        return norm
 
     def apply_dense(self, w, grad, reg=0.0):
         """Whole-tensor application; reg > 0 adds reg*w (tf l2_regularizer / l2_loss terms)."""
@@ -748,6 +771,79 @@ class _SeqDotLoss(torch.autograd.Function):
 
 def seq_dot_loss(x, tW, tb, tgt, neg, scale=1.0, items=None):
     return _SeqDotLoss.apply(x, tW, tb, tgt, neg, float(scale), items)
+
+
+# ----------------------------------------------------------------------------------------------
+# next-item models over long histories: scaled embeddings, windowed attention, catalog log-probabilities
+# (float32, float16 or bfloat16; gradients through the HIP kernels, no double backward)
+# ----------------------------------------------------------------------------------------------
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape[0], scale, padding_idx)
+        return K.embed_forward(weight, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        rows, scale, padding_idx = ctx.args
+        return K.embed_backward(gout.contiguous(), ctx.saved_tensors[0], rows, scale, padding_idx), None, None, None
+
+
+def embedding(weight, ids, scale=1.0, padding_idx=None):
+    """scale * weight[ids] with a dense gradient for `weight` [rows, d] (dr_embed_forward / dr_embed_backward); row
+    padding_idx gets none.  The lookup of weights that autograd owns; Table.lookup serves the optimizer's sparse tables."""
+    return _Embedding.apply(weight, ids, float(scale), padding_idx)
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, begin, end):
+        out, lse = K.window_attn_forward(q, k, v, window, sinks, scale, begin, end)
+        ctx.save_for_backward(q, k, v, out, lse, begin, end)
+        ctx.args = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        q, k, v, out, lse, begin, end = ctx.saved_tensors
+        return K.window_attn_backward(q, k, v, out, lse, gout.contiguous(), *ctx.args, begin, end) + (None,) * 5
+
+
+def window_attention(q, k, v, window, sinks=0, scale=None, begin=None, end=None):
+    """Causal attention over the last `window` positions and the first `sinks` items of every history (kernels.
+    window_attn_forward says what is visible), differentiable in q, k and v."""
+    return _WindowAttention.apply(q, k, v, window, sinks, scale, begin, end)
+
+
+class _ItemLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, k):
+        ctx.set_materialize_grads(False)
+        r = K.item_logprobs_forward(logits, targets, k)
+        ctx.save_for_backward(logits, targets, r.lse, r.entropy)
+        ctx.mark_non_differentiable(*[t for t in (r.lse, r.top_idx, r.top_logp) if t is not None])
+        return tuple(r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, *_):
+        logits, targets, lse, entropy = ctx.saved_tensors
+        if g_logp is None and g_entropy is None:
+            return None, None, None
+        if g_logp is None:
+            targets = None                                  # only the entropy is part of the loss
+        return K.item_logprobs_backward(logits, targets, lse, entropy,
+                                        g_logp.contiguous() if g_logp is not None else None,
+                                        g_entropy.contiguous() if g_entropy is not None else None), None, None
+
+
+def item_logprobs(logits, targets=None, k=0):
+    """kernels.LogProbs of softmax(logits) over the catalog: logp of the targets and entropy differentiable, the k best
+    items with their log-probabilities not."""
+    return K.LogProbs(*_ItemLogprobs.apply(logits, targets, k))
 
 
 def bi_interaction(table, feats):

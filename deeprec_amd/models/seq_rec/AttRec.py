@@ -32,7 +32,9 @@ def timing_signal(length, channels, device, min_timescale=1.0, max_timescale=1.0
 
 class AttRec(SeqBase):
     def __init__(self, sess, num_user=None, num_item=None, learning_rate=0.05, reg_rate=1e-2, epoch=5000, batch_size=1000,
-                 show_time=False, T=1, display_step=1000, verbose=False, device=None, shard=None, sampler="reference"):
+                 show_time=False, T=1, display_step=1000, verbose=False, device=None, shard=None, sampler="reference", clip_norm=None):
+        # clip_norm: global norm that a step's gradients are held to (TFOptimizer.clip); None: the reference's behaviour
+        self.clip_norm = clip_norm
         self.sess, self.num_user, self.num_item = shift_sess(sess, num_user, num_item)
         self.shard = active_shard(shard)                    # _common.Shard: data-parallel over ranks, tables row-sharded
         self.learning_rate = learning_rate
@@ -75,7 +77,7 @@ class AttRec(SeqBase):
         self.linear_project = Wp.requires_grad_(True)
         self._timing = None
         self.unfused = False        # True: distances / hinge as library elementwise ops under autograd
-        self.optimizer = TFOptimizer("adagrad", self.learning_rate, initial_accumulator_value=0.05)
+        self.optimizer = TFOptimizer("adagrad", self.learning_rate, initial_accumulator_value=0.05, clip_norm=self.clip_norm)
         # hipGraph replay pays off while the step is launch-bound (the reference's B = 1000, L = 5: ~80 short launches);
         # at C5 (B = 4096, L = 50) the kernels fill the GPU and the eager loop is faster (2.52 vs 2.69 ms).  The sharded
         # lookups synchronise with the host (split sizes), so they are never captured.
@@ -159,6 +161,7 @@ class AttRec(SeqBase):
         o = self.optimizer
         o.begin_step()
         with torch.no_grad():
+            o.clip((self.P, self.X, self.Q), [self.linear_project])
             for t in (self.P, self.V, self.X, self.Q):
                 o.apply_table(t, 0.001, K.REG_DENSE)
             o.apply_dense(self.linear_project.data, self.linear_project.grad, self.reg_rate)

@@ -89,7 +89,9 @@ def caser_convs_fused(e, conv_v_w, conv_v_b, hw_cat, hb_cat, n_h):
 
 class Caser(SeqBase):
     def __init__(self, sess, num_user=None, num_item=None, learning_rate=0.001, reg_rate=1e-6, epoch=500, batch_size=1000,
-                 show_time=False, T=1, display_step=1000, verbose=False, device=None, shard=None, sampler="reference"):
+                 show_time=False, T=1, display_step=1000, verbose=False, device=None, shard=None, sampler="reference", clip_norm=None):
+        # clip_norm: global norm that a step's gradients are held to (TFOptimizer.clip); None: the reference's behaviour
+        self.clip_norm = clip_norm
         self.sess, self.num_user, self.num_item = shift_sess(sess, num_user, num_item)
         self.shard = active_shard(shard)                    # _common.Shard: data-parallel over ranks, tables row-sharded
         self.learning_rate = learning_rate
@@ -157,7 +159,7 @@ class Caser(SeqBase):
         # tf.layers.dense default kernel init would be glorot; the reference passes random_normal_initializer (sigma 1)
         self.full_w, self.full_b = dense("full_w", (fin, d), 1.0), dense("full_b", (d,), 0)
         self.fc1_dim_v, self.fc1_dim_h = n_v * d, n_h * d
-        self.optimizer = TFOptimizer("adam", self.learning_rate, eps=1e-8)
+        self.optimizer = TFOptimizer("adam", self.learning_rate, eps=1e-8, clip_norm=self.clip_norm)
         self.unfused = False        # True: score / BCE as library elementwise ops under autograd
         self.loss_scale = 1.0       # a caller that feeds 1/n of a batch per call sets 1/n (the loss is a batch MEAN)
         return self
@@ -230,6 +232,7 @@ class Caser(SeqBase):
         o = self.optimizer
         o.begin_step()
         with torch.no_grad():
+            o.clip((self.P, self.Q, self.W, self.b), self._dense_params())
             for t in (self.P, self.Q, self.V, self.W, self.b):
                 o.apply_table(t, self.reg_rate, K.REG_DENSE)
             for p in self._dense_params():

@@ -16,7 +16,9 @@ from ._seq_common import SeqBase
 
 class PRME(SeqBase):
     def __init__(self, sess, num_user=None, num_item=None, learning_rate=0.001, reg_rate=1e-2, epoch=5000, batch_size=1000,
-                 show_time=False, T=1, display_step=1000, verbose=False, device=None, sampler="reference"):
+                 show_time=False, T=1, display_step=1000, verbose=False, device=None, sampler="reference", clip_norm=None):
+        # clip_norm: global norm that a step's gradients are held to (TFOptimizer.clip); None: the reference's behaviour
+        self.clip_norm = clip_norm
         self.sess, self.num_user, self.num_item = shift_sess(sess, num_user, num_item)
         self.learning_rate = learning_rate
         self.epochs = epoch
@@ -43,7 +45,7 @@ class PRME(SeqBase):
         tab = lambda n, rows: Table(to_dev(init[n], torch.float32, dev) if n in init else normal_((rows, num_factor), 0.001, dev))
         self.P, self.V = tab("P", self.num_user), tab("V", self.num_user)
         self.Q, self.X = tab("Q", self.num_item), tab("X", self.num_item)
-        self.optimizer = TFOptimizer("adam", self.learning_rate, eps=1e-8)
+        self.optimizer = TFOptimizer("adam", self.learning_rate, eps=1e-8, clip_norm=self.clip_norm)
         self.unfused = False        # True: the distances / loss as library elementwise ops under autograd (what the fused kernel is tested against)
         return self
 
@@ -66,6 +68,7 @@ class PRME(SeqBase):
         o = self.optimizer
         o.begin_step()
         with torch.no_grad():
+            o.clip((self.P, self.X, self.Q))
             for t in (self.P, self.X, self.Q):
                 o.apply_table(t, 0.01, K.REG_DENSE)
         return loss.detach()
