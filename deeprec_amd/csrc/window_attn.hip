@@ -186,7 +186,8 @@ struct WinArgs {
     float *lse, *delta;        // [B, Hq, L]
     float* gmax;               // fp16: largest |dO| of every 16 queries [B, Hq, 4 tiles]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
-    int chunks;
+    int chunks;                // far sinks: workgroups along the sequence; 0: none
+    int here;                  // far sinks: taken by win_dkdv_kernel itself
 };
 // [begin[b], end[b]) cut to the row, whatever the arrays hold
 __device__ __forceinline__ void history(const int32_t* begin, const int32_t* end, int b, int L, int& lo, int& hi) {
@@ -737,8 +738,9 @@ __device__ __forceinline__ float grad_scale(const WinArgs& a, int b, int h0, int
 }
 // A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
 // head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
-// of the queries are added up at the end.  What the first items get from queries beyond the window comes from
-// win_sink_kernel's partial sums, added last and in order.
+// of the queries are added up at the end.  What the first items get from queries beyond the window is found here too
+// where that is at most 8 more steps (short rows: at 64 x 200 x 2 x 64 fp32 a launch of 11 us is saved); else it comes
+// from win_sink_kernel's partial sums, added last and in order.
 template <class T, int DP>
 constexpr int dkdv_buffers() {
     return DP * (int)sizeof(T) <= 256 ? 2 : 1;
@@ -759,10 +761,11 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     win_range(a, b, lo, hi);
     const int kw = k0 + (wave & 1) * 16, ki = kw + c16;
     const bool k_ok = ki >= lo && ki < hi;
-    // the queries that see the key through the window: [ki, ki + q_count)
-    const int q_count = k_ok ? (hi - ki < a.W ? hi - ki : a.W) : 0;
+    // the queries that see the key: [ki, ki + q_count), through the window or (first items, when they are taken here) all
+    const int first_end = a.here ? lo + a.S : lo;            // keys below it are first items taken here
+    const int q_count = k_ok ? (ki >= first_end && hi - ki > a.W ? a.W : hi - ki) : 0;
     const int klo = k0 > lo ? k0 : lo, khi = k0 + 31 < hi - 1 ? k0 + 31 : hi - 1;
-    const int qend = klo <= khi ? (khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1) : -1;   // last query
+    const int qend = klo > khi ? -1 : (klo >= first_end && khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1);
     const int tq0 = klo / 32 * 32, nt = klo <= khi ? (qend - tq0) / R + 1 : 0, total = nt * G;
     const float up = total > 0 ? grad_scale<T>(a, b, hk * G, G, tq0, qend) : 1.0f;
     Stage<T, DP, R, FAST> qs, gs;
@@ -805,7 +808,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         const int t0 = tq0 + i * R + half, buf = NB == 2 ? n & 1 : 0;
         if (++i == nt) i = 0;
         if (AHEAD && n + 1 < total) load();
-        if (kw <= t0 + 31 && t0 - (kw + 15) < a.W && t0 < hi && kw < hi && kw + 15 >= lo) {
+        if (kw <= t0 + 31 && (t0 - (kw + 15) < a.W || kw < first_end) && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
             dkdv_step<T, DP>(a, qt + buf * TILE + half * LD, gt + buf * TILE + half * LD, st + buf * 2 * R + half,
                              st + buf * 2 * R + R + half, kf, vf, t0, ki, q_count, whole, a.scale * up, dk, dv);
@@ -1154,8 +1157,9 @@ static int win_lds(Kernel k, size_t bytes) {
         DR_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     return DR_OK;
 }
-static int64_t win_chunks(int64_t L, int64_t window, int32_t sinks) {
-    return sinks > 0 && L > window ? (L + WA_CHUNK - 1) / WA_CHUNK : 0;
+static int64_t win_chunks(int64_t L, int64_t window, int32_t sinks, int group) {
+    if (sinks == 0 || L <= window || (L - window + 63) / 64 * group <= 8) return 0;
+    return (L + WA_CHUNK - 1) / WA_CHUNK;
 }
 
 template <class T, int DP, bool FAST>
@@ -1274,7 +1278,7 @@ extern "C" int64_t dr_window_attn_backward_bytes(int64_t B, int64_t L, int32_t H
     int rc = win_check("dr_window_attn_backward_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
     if (rc != DR_OK) return rc;
     return align_up(B * Hq * L * 4, 256) + align_up(B * Hq * ((L + 63) / 64) * 16, 256) +
-           align_up(B * Hkv * win_chunks(L, window, sinks) * 2 * sinks * D * 4, 256) + 256;
+           align_up(B * Hkv * win_chunks(L, window, sinks, Hq / Hkv) * 2 * sinks * D * 4, 256) + 256;
 }
 
 extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1318,7 +1322,8 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.delta = (float*)ws;
     a.gmax = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
     a.part = (float*)((char*)a.gmax + align_up(B * Hq * ((L + 63) / 64) * 16, 256));
-    a.chunks = (int)win_chunks(L, window, sinks);
+    a.chunks = (int)win_chunks(L, window, sinks, Hq / Hkv);
+    a.here = sinks > 0 && a.chunks == 0;
     a.tiles = (int)((L + 63) / 64);
     a.ktiles = (int)((L + 31) / 32);
     DR_REQUIRE((int64_t)a.ktiles * Hq * B < (1ll << 31) && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < (1ll << 31),

@@ -1231,7 +1231,7 @@ def embed_forward(table, ids, scale=1.0):
     rows, d = table.shape
     if rows < 1 or d < 1:
         raise ValueError("embed_forward: the table is empty")
-    out = table.new_empty(ids.shape + (d,))
+    out = torch.empty(ids.shape + (d,), dtype=table.dtype, device=table.device)
     check(_abi.lib().dr_embed_forward(table.data_ptr(), rows, d, DTYPES[table.dtype], ids.data_ptr(), ids.numel(), bits,
                                       scale, out.data_ptr(), _raw_stream()), "dr_embed_forward")
     return out
