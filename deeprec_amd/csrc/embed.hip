@@ -486,7 +486,7 @@ static int embed_forward_t(int dt, const void* table, int64_t rows, int d, const
 template <class T, int V, int LPR>
 static int embed_sum_launch(const EmbedArgs& a, const void* gout, void* grad, hipStream_t st) {
     const int64_t blocks = (a.chunks * LPR + 255) / 256;
-    DR_REQUIRE(blocks < (1ll << 31), "dr_embed_backward: too many blocks");
+    DR_REQUIRE(blocks < (1ll << 24), "dr_embed_backward: too many blocks");      // a launch counts threads in 32 bits
     DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, V, LPR>), dim3((unsigned)blocks), dim3(256), 0, st, a,
                     (const T*)gout, (T*)grad);
     DR_CHECK_LAUNCH("embed_sum_kernel");

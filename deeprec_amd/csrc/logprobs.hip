@@ -21,6 +21,7 @@ namespace dr {
 constexpr int LP_MAX_K = 64, LP_MAX_T = 64;
 constexpr int LP_CAP = 256;        // candidates of a wavefront
 constexpr int LP_MAX_SPLITS = 256;
+constexpr int64_t LP_MAX_GRID = 1 << 24;   // workgroups of 256: a launch counts its threads in 32 bits
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 constexpr float LP_LOWEST = -3.402823466e38f;
 constexpr float LP_FLOOR = -200.0f;   // exp(-200) is 0 in fp32: keeps 0 * -inf out of the entropy sum
@@ -542,7 +543,7 @@ extern "C" int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64
     a.pst = nullptr;
     a.pkey = nullptr;
     if (logp_wave_rows(N, V)) {
-        DR_REQUIRE((N + 3) / 4 < (1ll << 31), "dr_item_logprobs_forward: too many rows");
+        DR_REQUIRE((N + 3) / 4 < LP_MAX_GRID, "dr_item_logprobs_forward: too many rows");
 #define LP_WAVE(T_)                                                                                                     \
     if (K)                                                                                                              \
         DR_LAUNCH_NAMED("logp_row_wave_kernel", (logp_row_wave_kernel<T_, true>), dim3((unsigned)((N + 3) / 4)),        \
@@ -556,7 +557,7 @@ extern "C" int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64
         return DR_OK;
     }
     logp_split(N, a.V, LP_FILL, &a.splits, &a.seg);
-    DR_REQUIRE(N * a.splits < (1ll << 31), "dr_item_logprobs_forward: too many rows");
+    DR_REQUIRE(N * a.splits < LP_MAX_GRID, "dr_item_logprobs_forward: too many rows");
     if (a.splits > 1) {
         a.pst = (float*)ws;
         a.pkey = (uint64_t*)((char*)ws + align_up(N * a.splits * 16, 256));
@@ -615,14 +616,14 @@ extern "C" int32_t dr_item_logprobs_backward(const void* logits, int64_t N, int6
     if (logp_wave_rows(N, V)) {
         a.splits = 1;
         a.seg = a.V;
-        DR_REQUIRE((N + 3) / 4 < (1ll << 31), "dr_item_logprobs_backward: too many rows");
+        DR_REQUIRE((N + 3) / 4 < LP_MAX_GRID, "dr_item_logprobs_backward: too many rows");
 #define LP_GRAD(T_) \
     DR_LAUNCH_NAMED("logp_grad_kernel", (logp_grad_kernel<T_, 4>), dim3((unsigned)((N + 3) / 4)), dim3(256), 0, st, a)
         DR_BY_DTYPE(dtype, LP_GRAD);
 #undef LP_GRAD
     } else {
         logp_split(N, a.V, LP_FILL, &a.splits, &a.seg);
-        DR_REQUIRE(N * a.splits < (1ll << 31), "dr_item_logprobs_backward: too many rows");
+        DR_REQUIRE(N * a.splits < LP_MAX_GRID, "dr_item_logprobs_backward: too many rows");
 #define LP_GRAD(T_) \
     DR_LAUNCH_NAMED("logp_grad_kernel", (logp_grad_kernel<T_, 1>), dim3((unsigned)(N * a.splits)), dim3(256), 0, st, a)
         DR_BY_DTYPE(dtype, LP_GRAD);

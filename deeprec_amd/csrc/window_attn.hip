@@ -20,6 +20,7 @@
 namespace dr {
 
 constexpr int WA_MAX_D = 256, WA_MAX_SINKS = 64;
+constexpr int64_t WA_MAX_GRID = 1 << 24;   // workgroups of 256: a launch counts its threads in 32 bits
 constexpr int WA_BK = 32;              // keys (queries in the dK / dV kernels) per tile
 constexpr float WA_LOG2E = 1.44269504088896340736f, WA_LN2 = 0.69314718055994530942f;
 
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
     }
     l = groups_sum(l);
     if (qi >= a.L) return;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;                 // a NaN stays one
     T* op = out + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
                 if (d + i < a.D) op[d + i] = (T)(o[t][i] * inv);
         }
     }
-    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l > 0.0f ? (m + log2f(l)) * WA_LN2 : -__builtin_inff();
+    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * WA_LN2;
 }
 
 // ---- backward: dQ ------------------------------------------------------------------------------------------------------------
@@ -1093,7 +1094,7 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
         const int64_t row = (int64_t)b * a.Hq + hk * G + hh;
         const float lr = sl[0][r];
         if (a.splits == 1) {
-            ((T*)a.out)[row * a.D + d] = (T)(lr > 0.0f ? red[e] / lr : 0.0f);
+            ((T*)a.out)[row * a.D + d] = (T)(lr == 0.0f ? 0.0f : red[e] / lr);
         } else {
             float* p = a.part + (row * a.splits + sp) * (a.D + 2);
             p[d] = red[e];
@@ -1119,7 +1120,7 @@ __global__ __launch_bounds__(64) void win_join_kernel(const float* __restrict__ 
             l = fmaf(p[s * (D + 2) + D + 1], f, l);
             o = fmaf(p[s * (D + 2) + d], f, o);
         }
-        out[(int64_t)blockIdx.x * D + d] = (T)(l > 0.0f ? o / l : 0.0f);
+        out[(int64_t)blockIdx.x * D + d] = (T)(l == 0.0f ? 0.0f : o / l);
     }
 }
 
@@ -1148,7 +1149,7 @@ static int win_check(const char* who, int64_t B, int64_t L, int32_t Hq, int32_t 
                "%s: bad sizes (B=%lld L=%lld Hq=%d Hkv=%d D=%d)", who, (long long)B, (long long)L, Hq, Hkv, D);
     DR_REQUIRE(window >= 1 && sinks >= 0 && sinks <= WA_MAX_SINKS, "%s: window=%lld (>= 1), sinks=%d (0..%d)", who,
                (long long)window, sinks, WA_MAX_SINKS);
-    DR_REQUIRE(scale > 0.0f && scale <= 3.402823466e38f, "%s: scale must be positive and finite", who);
+    DR_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "%s: scale must lie in [1e-30, 1e30]", who);
     return DR_OK;
 }
 template <class Kernel>
@@ -1260,7 +1261,7 @@ extern "C" int32_t dr_window_attn_forward(const void* q, const int64_t* q_stride
     a.lse = lse;
     a.tiles = (int)((L + 63) / 64);
     a.ktiles = (int)((L + 31) / 32);
-    DR_REQUIRE((int64_t)a.tiles * Hq * B < (1ll << 31), "dr_window_attn_forward: too many workgroups");
+    DR_REQUIRE((int64_t)a.tiles * Hq * B < WA_MAX_GRID, "dr_window_attn_forward: too many workgroups");
     const int al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
     const int alg = row_alignment(es, {out}, {(int64_t)D});
     DR_REQUIRE(al >= es && alg >= es, "dr_window_attn_forward: a pointer is not aligned to its element size");
@@ -1326,7 +1327,7 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.here = sinks > 0 && a.chunks == 0;
     a.tiles = (int)((L + 63) / 64);
     a.ktiles = (int)((L + 31) / 32);
-    DR_REQUIRE((int64_t)a.ktiles * Hq * B < (1ll << 31) && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < (1ll << 31),
+    DR_REQUIRE((int64_t)a.ktiles * Hq * B < WA_MAX_GRID && (int64_t)((sinks + 15) / 16) * a.chunks * Hkv * B < WA_MAX_GRID,
                "dr_window_attn_backward: too many workgroups");
     const int al = row_alignment(es, {q, k, v}, {a.qs.b, a.qs.l, a.qs.h, a.ks.b, a.ks.l, a.ks.h, a.vs.b, a.vs.l, a.vs.h});
     const int alg = row_alignment(es, {out, gout, dq}, {(int64_t)D});
@@ -1386,7 +1387,7 @@ extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides,
     a.S = sinks;
     a.hgroups = (Hq / Hkv + 15) / 16;
     token_split(B, Hkv, a.hgroups, token_keys(L, window, sinks), &a.splits, &a.per);
-    DR_REQUIRE((int64_t)a.splits * a.hgroups * Hkv * B < (1ll << 31) && B * Hq < (1ll << 31),
+    DR_REQUIRE((int64_t)a.splits * a.hgroups * Hkv * B < WA_MAX_GRID && B * Hq < WA_MAX_GRID,
                "dr_window_attn_token: too many workgroups");
     a.scale = scale;
     a.begin = begin;

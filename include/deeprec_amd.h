@@ -575,11 +575,14 @@ int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype,
  * q [B, L, Hq, D], k, v [B, L, Hkv, D], Hq a multiple of Hkv (query head h reads key head h / (Hq / Hkv)), one type
  * (DR_F32 / DR_F16 / DR_BF16), 1 <= D <= 256; the last dim is contiguous, *_strides = element strides {batch, position, head}.
  * Key j is visible to query i iff begin[b] <= j <= i < end[b] and (i - j < window or j - begin[b] < sinks); window >= 1,
- * 0 <= sinks <= 64; begin / end int32 [B] on the device (NULL: 0 / L), cut to [0, L].  scale > 0.
+ * 0 <= sinks <= 64; begin / end int32 [B] on the device (NULL: 0 / L), cut to [0, L].  1e-30 <= scale <= 1e30.
  * forward: out [B, L, Hq, D] contiguous, lse [B, Hq, L] fp32 = log sum exp(scale <q, k>).  A position outside [begin, end)
  * gives a zero row (lse -inf, gradients 0) and is never read.  backward: out, lse as written, gout [B, L, Hq, D]
  * contiguous -> dq [B, L, Hq, D], dk, dv [B, L, Hkv, D] contiguous, overwritten; sums over a group's heads included; no
  * atomics, bit-repeatable.  ws: dr_window_attn_backward_bytes(...), 256-byte aligned.
+ * A position that is not finite inside the history makes NaN what sees it, and may make NaN what shares a tile of 32
+ * positions with it without seeing it (the products run over whole tiles); outside the history it may be anything.  Outputs
+ * and workspace must not overlap the inputs.
  * token: ONE query per sequence, q [B, Hq, D] (strides {batch, head}), at position end[b] - 1 of a cache k, v [B, L, Hkv, D]
  * that already holds its own key and value -> out [B, Hq, D] contiguous.  ws: dr_window_attn_token_bytes(...), 256-byte
  * aligned (0 bytes: NULL). */
@@ -612,7 +615,8 @@ int32_t dr_window_attn_token(const void* q, const int64_t* q_strides, const void
  * A row without any offered item: logp -inf, entropy 0, lse (-inf, 0), no best items, gradient 0.  A NaN or +inf logit makes
  * the row's logp, entropy and gradients NaN (NaN is never among the best).  ws: dr_item_logprobs_bytes(N, V, K), 256-byte
  * aligned (0 bytes: NULL).  backward: g_logp [N, T] and g_entropy [N] (NULL: none) fp32 -> glogits [N, V] contiguous, in the logits' type:
- *   sum_t g_t [v = target_t] - p_v (sum_t g_t + g_entropy (log p_v + entropy)), rounded once. */
+ *   sum_t g_t [v = target_t] - p_v (sum_t g_t + g_entropy (log p_v + entropy)), rounded once.  glogits must not overlap
+ * the logits. */
 int64_t dr_item_logprobs_bytes(int64_t N, int64_t V, int32_t K);
 int32_t dr_item_logprobs_forward(const void* logits, int64_t N, int64_t V, int64_t ld, int32_t dtype, const void* targets,
                                  int32_t id_bits, int32_t T, int32_t K, float* logp, float* entropy, float* lse,

@@ -199,3 +199,37 @@ def test_clip_refuses_sharded_tables():
     with pytest.raises(ValueError, match="sharded"):
         opt.clip([Table(torch.zeros(4, 2), Shard(1, 0, force=True))])
     assert TFOptimizer("sgd", 0.1).clip([]) is None
+
+
+@gpu
+def test_captured_training_step(dev):
+    """Forward and backward of the whole path in one hipGraph: every replay equals the eager step on the same values."""
+    p, begin, seq, tgt = _setup(torch.float32)
+    begin, seq, tgt = begin.to(dev), seq.to(dev), tgt.to(dev)
+
+    def step(w):
+        loss, _ = _loss(w, begin, seq, tgt)
+        return (loss.detach(),) + torch.autograd.grad(loss, [w[n] for n in NAMES])
+
+    def leaves():
+        return {n: t.to(dev).requires_grad_(True) for n, t in p.items()}
+    w = leaves()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(w)
+    for _ in range(3):
+        with torch.no_grad():
+            for n in NAMES:
+                p[n] = torch.randn(p[n].shape) * 0.125
+                w[n].copy_(p[n])
+            seq.copy_(seq[:, torch.randperm(L, device=dev)])
+        graph.replay()
+        eager = step(leaves())
+        torch.cuda.synchronize()
+        for a, b in zip(res, eager):
+            assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * float(b.float().abs().max()))   # library products may differ in order

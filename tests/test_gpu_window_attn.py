@@ -348,3 +348,44 @@ def test_gradient_scale(dev, dt, size):
     for name, x, ref, lim in zip(("dq", "dk", "dv"), Kn.window_attn_backward(d(q), d(k), d(v), out, lse, d(go), **mask),
                                  (r["dq"], r["dk"], r["dv"]), (lq, lk, lv)):
         _within(name, x, ref, lim + (2.0 ** -24 if dt == torch.float16 else 0.0))
+
+
+@gpu
+def test_nan_is_not_an_empty_row(dev):
+    """A NaN that a query sees comes out of every form as NaN: only a query without keys gives zeros and lse -inf."""
+    from deeprec_amd import kernels as Kn
+    q, k, v, go, _, _ = (t.to(dev) for t in _inputs(2, 40, 2, 1, 32, torch.float32, 4))
+    k[0] = math.nan
+    end = torch.tensor([40, 0], dtype=torch.int32, device=dev)
+    out, lse = Kn.window_attn_forward(q, k, v, 8, 2, end=end)
+    assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all())
+    assert not bool(out[1].any()) and bool((lse[1] == -math.inf).all())
+    one = Kn.window_attn_token(q[:, 0], k, v, 8, 2, end=end)
+    assert bool(one[0].isnan().all()) and not bool(one[1].any())
+    many = Kn.window_attn_token(q[:1, 0], k[:1, :1].expand(1, 2000, 1, 32), v[:1, :1].expand(1, 2000, 1, 32), 2000)  # split keys
+    assert bool(many.isnan().all())
+
+
+@gpu
+def test_scale_range(dev):
+    from deeprec_amd import kernels as Kn
+    from deeprec_amd._abi import DeepRecError
+    q, k, v, _, _, _ = (t.to(dev) for t in _inputs(1, 40, 1, 1, 32, torch.float32, 4))
+    for bad in (1e-39, 3e38):
+        with pytest.raises(DeepRecError, match="scale"):
+            Kn.window_attn_forward(q, k, v, 8, scale=bad)
+    out, _ = Kn.window_attn_forward(q, k, v, 8, scale=1e-30)                 # every visible key weighs the same
+    vd = v[0, :, 0].double().cpu()
+    want = torch.stack([vd[max(0, i - 7):i + 1].mean(0) for i in range(40)])
+    assert float((out[0, :, 0].cpu().double() - want).abs().max()) < 1e-5    # 8 terms of about 1, sums in fp32
+
+
+def test_window_attention_refuses_a_grid_too_large_cpu():
+    import ctypes as C
+    from deeprec_amd import _abi
+    lib = _abi.lib()
+    p, s = C.c_void_p(4096), (C.c_int64 * 3)(64, 16, 8)
+    assert lib.dr_window_attn_forward(p, s, p, s, p, s, 2 ** 24, 4, 1, 1, 8, 0, 3, 1, 0.5, None, None, p, p, None) == -1
+    assert lib.dr_item_logprobs_forward(p, 2 ** 27, 8, 8, 0, None, 32, 0, 0, None, p, p, None, None, None, 0, None) == -1
+    for bad in (1e-39, 3e38):
+        assert lib.dr_window_attn_forward(p, s, p, s, p, s, 2, 4, 2, 1, 8, 0, 3, 1, bad, None, None, p, p, None) == -1
