@@ -20,6 +20,7 @@
 namespace dr {
 
 constexpr int WA_MAX_D = 256, WA_MAX_SINKS = 64;
+constexpr int WA_MAX_SPLITS = 256;
 constexpr int64_t WA_MAX_GRID = 1 << 24;   // workgroups of 256: a launch counts its threads in 32 bits
 constexpr int WA_BK = 32;              // keys (queries in the dK / dV kernels) per tile
 constexpr float WA_LOG2E = 1.44269504088896340736f, WA_LN2 = 0.69314718055994530942f;
@@ -979,7 +980,7 @@ template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
     constexpr int LD = lds_ld<T, DP>(), TILE = WA_BK * LD, NW = token_waves<T, DP>();
     __shared__ __attribute__((aligned(16))) T tiles[NW * TILE];
-    __shared__ float sm[NW][16], sl[NW][16];
+    __shared__ float sm[NW][16], sl[NW][16], tm[16], tl[16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     T* vt = tiles + wave * TILE;
     int id = (int)blockIdx.x;
@@ -1069,59 +1070,72 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
     float lt = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) lt += sl[w][c16] * __builtin_amdgcn_exp2f((sm[w][c16] - ms) * c);
-    float* red = reinterpret_cast<float*>(tiles);                          // [16 heads][DP] fp32: 64 DP bytes of the tiles
-#pragma unroll 1
-    for (int w = 0; w < NW; ++w) {
-        if (wave == w) {
+    // every wavefront's sums [16 heads][DP] fp32 into its own tile (64 DP bytes of it); one barrier, then they are added
+    constexpr int RED = TILE * (int)sizeof(T) / 4;
+    float* red = reinterpret_cast<float*>(tiles);
 #pragma unroll
-            for (int x = 0; x < DP / 16; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float* r = red + c16 * DP + 16 * x + 4 * g + i;
-                    *r = w == 0 ? o[x][i] * f : *r + o[x][i] * f;
-                }
-        }
-        __syncthreads();
-    }
+    for (int x = 0; x < DP / 16; ++x)
+        *reinterpret_cast<f32x4*>(red + wave * RED + c16 * DP + 16 * x + 4 * g) = o[x] * f;
     if (wave == 0 && g == 0) {
-        sm[0][c16] = mx;
-        sl[0][c16] = lt;
+        tm[c16] = mx;
+        tl[c16] = lt;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < 16 * DP; e += NW * 64) {
         const int r = e / DP, d = e % DP, hh = hg * 16 + r;
         if (hh >= G || d >= a.D) continue;
         const int64_t row = (int64_t)b * a.Hq + hk * G + hh;
-        const float lr = sl[0][r];
+        const float lr = tl[r];
+        float x = red[e];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) x += red[w * RED + e];
         if (a.splits == 1) {
-            ((T*)a.out)[row * a.D + d] = (T)(lr == 0.0f ? 0.0f : red[e] / lr);
+            ((T*)a.out)[row * a.D + d] = (T)(lr == 0.0f ? 0.0f : x / lr);
         } else {
             float* p = a.part + (row * a.splits + sp) * (a.D + 2);
-            p[d] = red[e];
+            p[d] = x;
             if (d == 0) {
-                p[a.D] = sm[0][r];
+                p[a.D] = tm[r];
                 p[a.D + 1] = lr;
             }
         }
     }
 }
+// joins the splits of one query: a thread per split for the common maximum and sum, then 256 / W groups of W lanes take the
+// splits in turn (W: D rounded up to 32, 64, .. 256) and are added in order
 template <class T>
-__global__ __launch_bounds__(64) void win_join_kernel(const float* __restrict__ part, int splits, int D, float scale,
-                                                      T* __restrict__ out) {
+__global__ __launch_bounds__(256) void win_join_kernel(const float* __restrict__ part, int splits, int D, float scale,
+                                                       T* __restrict__ out) {
+    __shared__ float f[WA_MAX_SPLITS], red[256], sm[4], sl[4];
     const float* p = part + (int64_t)blockIdx.x * splits * (D + 2);
     const float c = scale * WA_LOG2E;
-    float m = -__builtin_inff();
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, p[s * (D + 2) + D]);
-    const float ms = m == -__builtin_inff() ? 0.0f : m;
-    for (int d = threadIdx.x; d < D; d += 64) {
-        float l = 0.0f, o = 0.0f;
-        for (int s = 0; s < splits; ++s) {
-            const float f = __builtin_amdgcn_exp2f((p[s * (D + 2) + D] - ms) * c);
-            l = fmaf(p[s * (D + 2) + D + 1], f, l);
-            o = fmaf(p[s * (D + 2) + d], f, o);
-        }
-        out[(int64_t)blockIdx.x * D + d] = (T)(l == 0.0f ? 0.0f : o / l);
-    }
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const bool on = tid < splits;                            // splits <= 256
+    const float m = on ? p[(int64_t)tid * (D + 2) + D] : -__builtin_inff(), l = on ? p[(int64_t)tid * (D + 2) + D + 1] : 0.0f;
+    float mx = m;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    if (lane == 0) sm[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    const float e = __builtin_amdgcn_exp2f((m - (mx == -__builtin_inff() ? 0.0f : mx)) * c);
+    f[tid] = e;
+    float lt = l * e;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) lt += __shfl_xor(lt, off, 64);
+    if (lane == 0) sl[wave] = lt;
+    __syncthreads();
+    lt = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    const int W = D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256, d = tid % W, groups = 256 / W;
+    float o = 0.0f;
+    if (d < D)
+#pragma unroll 8
+        for (int s = tid / W; s < splits; s += groups) o = fmaf(p[(int64_t)s * (D + 2) + d], f[s], o);
+    red[tid] = o;
+    __syncthreads();
+    if (tid >= D) return;
+    for (int q = 1; q < groups; ++q) o += red[q * W + tid];
+    out[(int64_t)blockIdx.x * D + tid] = (T)(lt == 0.0f ? 0.0f : o / lt);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------
@@ -1204,18 +1218,22 @@ static int win_token_launch(const TokenArgs& a, hipStream_t st) {
                     dim3(64 * token_waves<T, DP>()), 0, st, a);
     DR_CHECK_LAUNCH("win_token_kernel");
     if (a.splits > 1) {
-        DR_LAUNCH_NAMED("win_join_kernel", (win_join_kernel<T>), dim3((unsigned)(a.B * a.Hq)), dim3(64), 0, st,
+        DR_LAUNCH_NAMED("win_join_kernel", (win_join_kernel<T>), dim3((unsigned)(a.B * a.Hq)), dim3(256), 0, st,
                         (const float*)a.part, a.splits, a.D, a.scale, (T*)a.out);
         DR_CHECK_LAUNCH("win_join_kernel");
     }
     return DR_OK;
 }
-// workgroups per sequence and key head, 32-key tiles each: 2 workgroups per CU, none below 256 keys
-static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int* splits, int* per) {
+// workgroups per sequence and key head, 32-key tiles each.  A workgroup's NW wavefronts take NW tiles a round; joining
+// costs 3 us, as much as two rounds or more, so up to three rounds stay in one workgroup (64 x 260 keys x 8 / 2 heads x 64
+// bf16: 6.5 us so, 8.5 us split in two).  Beyond, the keys are split until there are 2 workgroups per CU or 2 tiles each:
+// 1 x 2048 keys takes 7.3 us with 2 tiles each, 8.8 us with 8; 1 x 1000 x 4 heads x 128 fp32 takes 10.9 and 23.4 us.
+static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int D, int es, int* splits, int* per) {
+    const int row = (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es, nw = row <= 256 ? 4 : (row <= 512 ? 2 : 1);
     const int64_t tiles = (keys + WA_BK - 1) / WA_BK, rows = B * Hkv * hgroups;
-    int64_t s = (512 + rows - 1) / rows;
-    if (s > tiles / 8) s = tiles / 8;
-    if (s > 128) s = 128;
+    int64_t s = tiles <= 3 * nw ? 1 : (512 + rows - 1) / rows;
+    if (s > tiles / 2) s = tiles / 2;
+    if (s > WA_MAX_SPLITS) s = WA_MAX_SPLITS;
     if (s < 1) s = 1;
     *per = (int)((tiles + s - 1) / s);
     *splits = (int)((tiles + *per - 1) / *per);
@@ -1348,8 +1366,10 @@ extern "C" int64_t dr_window_attn_token_bytes(int64_t B, int64_t L, int32_t Hq, 
     int rc = win_check("dr_window_attn_token_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
     if (rc != DR_OK) return rc;
     if (B == 0) return 0;
-    int splits, per;
-    token_split(B, Hkv, (Hq / Hkv + 15) / 16, token_keys(L, window, sinks), &splits, &per);
+    int splits, more, per;                                     // the types split differently: enough for each
+    token_split(B, Hkv, (Hq / Hkv + 15) / 16, token_keys(L, window, sinks), D, 2, &splits, &per);
+    token_split(B, Hkv, (Hq / Hkv + 15) / 16, token_keys(L, window, sinks), D, 4, &more, &per);
+    if (more > splits) splits = more;
     return splits > 1 ? align_up(B * Hq * splits * ((int64_t)D + 2) * 4, 256) : 0;
 }
 
@@ -1386,7 +1406,7 @@ extern "C" int32_t dr_window_attn_token(const void* q, const int64_t* q_strides,
     a.W = (int)(window < L ? window : L);
     a.S = sinks;
     a.hgroups = (Hq / Hkv + 15) / 16;
-    token_split(B, Hkv, a.hgroups, token_keys(L, window, sinks), &a.splits, &a.per);
+    token_split(B, Hkv, a.hgroups, token_keys(L, window, sinks), D, es, &a.splits, &a.per);
     DR_REQUIRE((int64_t)a.splits * a.hgroups * Hkv * B < WA_MAX_GRID && B * Hq < WA_MAX_GRID,
                "dr_window_attn_token: too many workgroups");
     a.scale = scale;

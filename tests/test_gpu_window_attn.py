@@ -389,3 +389,27 @@ def test_window_attention_refuses_a_grid_too_large_cpu():
     assert lib.dr_item_logprobs_forward(p, 2 ** 27, 8, 8, 0, None, 32, 0, 0, None, p, p, None, None, None, 0, None) == -1
     for bad in (1e-39, 3e38):
         assert lib.dr_window_attn_forward(p, s, p, s, p, s, 2, 4, 2, 1, 8, 0, 3, 1, bad, None, None, p, p, None) == -1
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,L,Hq,Hkv,D", [(1, 20000, 2, 1, 24), (1, 33000, 1, 1, 64), (2, 900, 20, 1, 128), (1, 700, 4, 2, 200)])
+def test_token_over_many_splits(dev, B, L, Hq, Hkv, D, dt):
+    """Long caches, whose keys are shared out over up to 256 workgroups (the first two), against 64 bits."""
+    from deeprec_amd import kernels as Kn
+    g = torch.Generator().manual_seed(L)
+    r = lambda *s: torch.randn(s, generator=g).to(dt)
+    q, k, v = r(B, Hq, D), r(B, L, Hkv, D), r(B, L, Hkv, D)
+    end = torch.full((B,), L - 3, dtype=torch.int32)
+    out = Kn.window_attn_token(q.to(dev), k.to(dev), v.to(dev), L, end=end.to(dev))
+    K, V = (t[:, :L - 3].double().repeat_interleave(Hq // Hkv, 2) for t in (k, v))
+    scale = D ** -0.5
+    s = torch.einsum("bhd,blhd->bhl", q.double(), K) * scale
+    p = torch.softmax(s, -1)
+    ref = torch.einsum("bhl,blhd->bhd", p, V)
+    e = torch.finfo(dt).eps / 2
+    ds = ((D + 4) * U * torch.einsum("bhd,blhd->bhl", q.double().abs(), K.abs()) * scale).amax(-1, keepdim=True)
+    lse = torch.logsumexp(s, -1, keepdim=True).abs()
+    rel = 2 * ds + (L / 8 + 40) * U + (0.0 if dt == torch.float32 else e) + 4 * U * lse
+    lim = rel * torch.einsum("bhl,blhd->bhd", p, V.abs()) * (1 + e) + e * ref.abs() + 1e-30 + torch.finfo(dt).smallest_normal * e
+    _within("out", out, ref, lim)
