@@ -2,8 +2,8 @@
 //   forward   out[e, :] = scale * table[ids[e], :]            (an id outside [0, rows): a zero row, as dr_gather_f32)
 //   backward  grad[r, :] = scale * sum over e with ids[e] == r of gout[e, :]   for EVERY row r (untouched rows: 0);
 //             ids equal to padding, or outside [0, rows), contribute nothing.
-// HBM-bound both ways.  Sums are fp32 in a fixed order (sorted list cut into blocks of EMB_CHUNK entries, entries in list
-// order inside a block, a row's blocks in ascending order): the same ids and gradients give the same bits, with no atomics.
+// HBM-bound both ways.  Sums are fp32 in a fixed order (sorted list cut into chunks of 8 or 32 entries, entries in list
+// order inside a chunk, a row's chunks in ascending order): the same ids and gradients give the same bits, with no atomics.
 #include <utility>
 
 #include "dr_lsd_sort.h"
@@ -12,8 +12,9 @@
 namespace dr {
 
 constexpr int EMB_MAX_D = 32768;
-constexpr int EMB_CHUNK = 32;        // sorted entries a group of lanes sums
-constexpr int EMB_DEPTH = 16;        // gradient rows of a chunk in flight per lane group
+// Sorted entries a group of lanes sums: few where the list is short and the chip would idle (whole gradient of 20000 rows of
+// 128 bf16: 29 us with 8, 33 us with 32; of 100000: 41 and 37 us)
+static int embed_chunk(int64_t n) { return n <= 65536 ? 8 : 32; }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 // A block owns R whole rows = R * cpr vectors of V elements, dealt to its threads in order, so every lane moves 16 bytes
@@ -58,9 +59,13 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict_
 // runs most of the chip would idle: its launches carry extra workgroups that clear the gradient table (rows no id names
 // stay 0), which therefore costs next to nothing.
 constexpr int SRT_T = 512, SRT_WAVES = SRT_T / 64, SRT_IPT = 4, SRT_TILE = SRT_T * SRT_IPT;
-constexpr int SRT_MAX_TILES = 128;      // beyond, every workgroup would read too many tile histograms: lsd_sort
+// beyond, every workgroup would read too many tile histograms: lsd_sort (gradient of 400000 rows of 64 fp32: 69 us, 93 us with
+// lsd_sort)
+constexpr int SRT_MAX_TILES = 512;
 constexpr int64_t SRT_MAX_N = SRT_MAX_TILES * SRT_TILE;
-constexpr int SRT_DIRECT_TILES = 8;     // up to here a workgroup counts all keys itself instead of a histogram launch
+// up to here a workgroup counts all keys itself instead of a histogram launch (gradient of 8192 rows of 64 fp32: 22.6 us, 26.5 us
+// with the launch; of 16000: 33.4 and 28.5 us)
+constexpr int SRT_DIRECT_TILES = 4;
 
 template <class Id>
 struct EmbedKeys {  // ids -> sort keys; ids that contribute nothing sort behind every row
@@ -274,7 +279,7 @@ struct EmbedArgs {
     const uint32_t* spos;   // their list positions, likewise
     int step;
     int64_t n, rows, chunks;
-    int d;
+    int chunk, d;
     float scale;
     float* part;            // [chunks, 2, d] sums of the runs that cross a chunk border: first run, last run
     uint8_t* state;         // [chunks] RUN_*
@@ -286,14 +291,15 @@ constexpr uint8_t RUN_FILLS = 2;    // one run fills the chunk and goes on on bo
 // began in an earlier chunk goes to part[chunk][0], the part of one that goes on behind the chunk to part[chunk][1] (a run
 // that does both: [0]).  The chunk's keys and positions are fetched once, spread over the lanes, so that the only
 // dependent step left is position -> row, 16 rows in flight.
-template <class T, int V, int LPR>
+template <class T, int V, int LPR, int CH>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedArgs a, const T* __restrict__ gout, T* __restrict__ grad) {
-    constexpr int E = EMB_CHUNK / LPR > 0 ? EMB_CHUNK / LPR : 1;    // entries a lane keeps
+    constexpr int E = CH / LPR > 0 ? CH / LPR : 1;                  // entries a lane keeps
+    constexpr int DEPTH = CH < 16 ? CH : 16;                        // gradient rows in flight
     const int64_t chunk = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
     const int lane = threadIdx.x % LPR, group0 = (threadIdx.x & 63) - lane;
     if (chunk >= a.chunks) return;                                  // whole groups leave
-    const int64_t s0 = chunk * EMB_CHUNK;
-    const int m = (int)(a.n - s0 < EMB_CHUNK ? a.n - s0 : EMB_CHUNK);
+    const int64_t s0 = chunk * CH;
+    const int m = (int)(a.n - s0 < CH ? a.n - s0 : CH);
     uint32_t keys[E];
     uint32_t spos[E];
 #pragma unroll
@@ -307,64 +313,62 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedArgs a, const T* __
     const uint32_t before = s0 > 0 ? a.keys[(s0 - 1) * a.step] : none, behind = s0 + m < a.n ? a.keys[(s0 + m) * a.step] : none;
     auto entry = [&](const auto (&r)[E], int q) { return __shfl(r[q / LPR < E ? q / LPR : 0], group0 + q % LPR, 64); };
     const uint32_t k_first = entry(keys, 0), k_last = __shfl(keys[(m - 1) / LPR < E ? (m - 1) / LPR : 0], group0 + (m - 1) % LPR, 64);
-    if (lane == 0) {
+    if (lane == 0 && blockIdx.y == 0) {
         uint8_t st = 0;
         if (k_last < rows && k_last == behind) st = k_first == k_last && before == k_first ? RUN_FILLS : RUN_BEGINS;
         a.state[chunk] = st;
     }
     if (k_first >= rows) return;                                    // sorted: nothing from here on contributes
-    for (int c0 = 0; c0 < a.d; c0 += LPR * V) {                     // every lane of the group stays for the shuffles
-        const int c = c0 + lane * V;
-        const bool on = c < a.d;
-        float acc[V];
+    const int c = (int)blockIdx.y * LPR * V + lane * V;             // this workgroup's columns
+    const bool on = c < a.d;                                        // every lane of the group stays for the shuffles
+    float acc[V];
 #pragma unroll
-        for (int x = 0; x < V; ++x) acc[x] = 0.0f;
-        uint32_t run = k_first;
-        bool carried = before == k_first;
-        auto flush = [&](uint32_t next) {                           // the run ends; `next`: the key behind it
-            if (!on) return;
-            if (carried) {
-                store_f32<float, V>(a.part + (chunk * 2) * a.d + c, acc);
-            } else if (next == run) {
-                store_f32<float, V>(a.part + (chunk * 2 + 1) * a.d + c, acc);
+    for (int x = 0; x < V; ++x) acc[x] = 0.0f;
+    uint32_t run = k_first;
+    bool carried = before == k_first;
+    auto flush = [&](uint32_t next) {                           // the run ends; `next`: the key behind it
+        if (!on) return;
+        if (carried) {
+            store_f32<float, V>(a.part + (chunk * 2) * a.d + c, acc);
+        } else if (next == run) {
+            store_f32<float, V>(a.part + (chunk * 2 + 1) * a.d + c, acc);
+        } else {
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[x] *= a.scale;
+            store_f32<T, V>(grad + (int64_t)run * a.d + c, acc);
+        }
+    };
+    const T* col = gout + (on ? c : 0);
+#pragma unroll
+    for (int q0 = 0; q0 < CH; q0 += DEPTH) {
+        // unconditional loads of valid rows (entries behind the list repeat its last): under a condition each would
+        // wait for the one before
+        typename VecType<T, V>::type v[DEPTH];
+        uint32_t key[DEPTH];
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q)
+            v[q] = *reinterpret_cast<const typename VecType<T, V>::type*>(col + (int64_t)entry(spos, q0 + q) * a.d);
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q) key[q] = entry(keys, q0 + q);
+#pragma unroll
+        for (int q = 0; q < DEPTH; ++q) {
+            if (q0 + q >= m || key[q] >= rows) continue;
+            if (key[q] != run) {
+                flush(key[q]);
+                run = key[q];
+                carried = false;
+#pragma unroll
+                for (int x = 0; x < V; ++x) acc[x] = 0.0f;
+            }
+            if constexpr (V == 1) {
+                acc[0] += (float)v[q];
             } else {
 #pragma unroll
-                for (int x = 0; x < V; ++x) acc[x] *= a.scale;
-                store_f32<T, V>(grad + (int64_t)run * a.d + c, acc);
-            }
-        };
-        const T* col = gout + (on ? c : 0);
-#pragma unroll
-        for (int q0 = 0; q0 < EMB_CHUNK; q0 += EMB_DEPTH) {
-            // unconditional loads of valid rows (entries behind the list repeat its last): under a condition each would
-            // wait for the one before
-            typename VecType<T, V>::type v[EMB_DEPTH];
-            uint32_t key[EMB_DEPTH];
-#pragma unroll
-            for (int q = 0; q < EMB_DEPTH; ++q)
-                v[q] = *reinterpret_cast<const typename VecType<T, V>::type*>(col + (int64_t)entry(spos, q0 + q) * a.d);
-#pragma unroll
-            for (int q = 0; q < EMB_DEPTH; ++q) key[q] = entry(keys, q0 + q);
-#pragma unroll
-            for (int q = 0; q < EMB_DEPTH; ++q) {
-                if (q0 + q >= m || key[q] >= rows) continue;
-                if (key[q] != run) {
-                    flush(key[q]);
-                    run = key[q];
-                    carried = false;
-#pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] = 0.0f;
-                }
-                if constexpr (V == 1) {
-                    acc[0] += (float)v[q];
-                } else {
-#pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] += (float)v[q][x];
-                }
+                for (int x = 0; x < V; ++x) acc[x] += (float)v[q][x];
             }
         }
-        flush(k_last < rows ? behind : none);
     }
+    flush(k_last < rows ? behind : none);
 }
 
 // Joins the runs that cross chunk borders.  A workgroup looks at four chunks; for each in which such a run begins, it
@@ -388,34 +392,32 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a, T* __restr
             }
             last += 64;
         }
-        const int64_t run = (int64_t)a.keys[((chunk + 1) * EMB_CHUNK - 1) * a.step];
-        for (int c0 = 0; c0 < a.d; c0 += LPR * V) {
-            const int c = c0 + lane * V;
-            float acc[V];
+        const int64_t run = (int64_t)a.keys[((chunk + 1) * a.chunk - 1) * a.step];
+        const int c = (int)blockIdx.y * LPR * V + lane * V;
+        float acc[V];
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] = 0.0f;
-            if (c < a.d)
+        for (int x = 0; x < V; ++x) acc[x] = 0.0f;
+        if (c < a.d)
 #pragma unroll 8
-                for (int64_t q = chunk + group; q <= last; q += GROUPS) {
-                    float v[V];
-                    load_f32<float, V>(v, a.part + (q * 2 + (q == chunk ? 1 : 0)) * a.d + c);
+            for (int64_t q = chunk + group; q <= last; q += GROUPS) {
+                float v[V];
+                load_f32<float, V>(v, a.part + (q * 2 + (q == chunk ? 1 : 0)) * a.d + c);
 #pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] += v[x];
-                }
-#pragma unroll
-            for (int x = 0; x < V; ++x) red[group][lane * V + x] = acc[x];
-            __syncthreads();
-            if (group == 0 && c < a.d) {
-                const int parts = (int)(last - chunk + 1 < GROUPS ? last - chunk + 1 : GROUPS);
-                for (int g = 1; g < parts; ++g)
-#pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] += red[g][lane * V + x];
-#pragma unroll
-                for (int x = 0; x < V; ++x) acc[x] *= a.scale;
-                store_f32<T, V>(grad + run * a.d + c, acc);
+                for (int x = 0; x < V; ++x) acc[x] += v[x];
             }
-            __syncthreads();
+#pragma unroll
+        for (int x = 0; x < V; ++x) red[group][lane * V + x] = acc[x];
+        __syncthreads();
+        if (group == 0 && c < a.d) {
+            const int parts = (int)(last - chunk + 1 < GROUPS ? last - chunk + 1 : GROUPS);
+            for (int g = 1; g < parts; ++g)
+#pragma unroll
+                for (int x = 0; x < V; ++x) acc[x] += red[g][lane * V + x];
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[x] *= a.scale;
+            store_f32<T, V>(grad + run * a.d + c, acc);
         }
+        __syncthreads();
     }
 }
 
@@ -438,7 +440,7 @@ static EmbedLayout embed_layout(int64_t n, int d) {
         off += align_up(bytes, 256);
         return o;
     };
-    const int64_t chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+    const int64_t chunks = (n + embed_chunk(n) - 1) / embed_chunk(n);
     L.pairs_a = take(n * 8);
     L.pairs_b = take(n * 8);
     L.hist = take(n <= SRT_MAX_N ? (n + SRT_TILE - 1) / SRT_TILE * (1 << 11) * 2 : lsd_scratch_bytes(n));
@@ -487,12 +489,17 @@ template <class T, int V, int LPR>
 static int embed_sum_launch(const EmbedArgs& a, const void* gout, void* grad, hipStream_t st) {
     const int64_t blocks = (a.chunks * LPR + 255) / 256;
     DR_REQUIRE(blocks < (1ll << 24), "dr_embed_backward: too many blocks");      // a launch counts threads in 32 bits
-    DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, V, LPR>), dim3((unsigned)blocks), dim3(256), 0, st, a,
-                    (const T*)gout, (T*)grad);
+    const unsigned cols = (unsigned)((a.d + LPR * V - 1) / (LPR * V));      // wide rows: workgroups side by side
+    if (a.chunk == 8)
+        DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, V, LPR, 8>), dim3((unsigned)blocks, cols), dim3(256), 0, st, a,
+                        (const T*)gout, (T*)grad);
+    else
+        DR_LAUNCH_NAMED("embed_sum_kernel", (embed_sum_kernel<T, V, LPR, 32>), dim3((unsigned)blocks, cols), dim3(256), 0, st, a,
+                        (const T*)gout, (T*)grad);
     DR_CHECK_LAUNCH("embed_sum_kernel");
     if (a.chunks > 1) {
-        DR_LAUNCH_NAMED("embed_join_kernel", (embed_join_kernel<T, V, LPR>), dim3((unsigned)((a.chunks + 3) / 4)), dim3(256), 0,
-                        st, a, (T*)grad);
+        DR_LAUNCH_NAMED("embed_join_kernel", (embed_join_kernel<T, V, LPR>), dim3((unsigned)((a.chunks + 3) / 4), cols), dim3(256),
+                        0, st, a, (T*)grad);
         DR_CHECK_LAUNCH("embed_join_kernel");
     }
     return DR_OK;
@@ -566,7 +573,8 @@ static int embed_backward_t(int dt, const void* gout, const void* ids, int64_t n
     EmbedArgs a;
     a.n = n;
     a.rows = rows;
-    a.chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+    a.chunk = embed_chunk(n);
+    a.chunks = (n + a.chunk - 1) / a.chunk;
     a.d = d;
     a.scale = scale;
     a.part = (float*)(ws + L.part);

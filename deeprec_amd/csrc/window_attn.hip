@@ -332,6 +332,16 @@ __device__ __forceinline__ void wave_stage(T* tile, const T* base, int64_t ld, i
         return (int64_t)clamp_row(row0 + r, lo, hi) * ld;
     });
 }
+// Workgroups go to the 8 XCDs in turn and each XCD has its own L2: dealt out one by one, neighbours along the sequence, which
+// read the same rows, would fetch them into 8 caches.  So runs of WA_RUN neighbours go to one XCD, the runs in turn (whole
+// eighths of the grid would leave an XCD with nothing but the short histories of a batch).
+constexpr int WA_RUN = 32;
+__device__ __forceinline__ unsigned win_block() {
+    constexpr unsigned ROUND = 8 * WA_RUN;
+    const unsigned id = blockIdx.x, base = id / ROUND * ROUND;
+    if (base + ROUND > gridDim.x) return id;                   // what is left of the grid: as it comes
+    return base + (id % 8) * WA_RUN + id % ROUND / 8;
+}
 // which key tiles a block of queries [qlo, qhi] needs: the tiles of the first items, then those of the window
 struct KeyTiles {
     int s0, ns, w0, n;
@@ -368,8 +378,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + NB * TILE;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-    const int q0 = (int)(blockIdx.x % a.tiles) * 64, h = (int)(blockIdx.x / a.tiles % a.Hq);
-    const int b = (int)(blockIdx.x / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
+    const unsigned id = win_block();
+    const int q0 = (int)(id % a.tiles) * 64, h = (int)(id / a.tiles % a.Hq);
+    const int b = (int)(id / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
     int lo, hi;
     win_range(a, b, lo, hi);
     const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
@@ -521,8 +532,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + NB * TILE;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-    const int q0 = (int)(blockIdx.x % a.tiles) * 64, h = (int)(blockIdx.x / a.tiles % a.Hq);
-    const int b = (int)(blockIdx.x / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
+    const unsigned id = win_block();
+    const int q0 = (int)(id % a.tiles) * 64, h = (int)(id / a.tiles % a.Hq);
+    const int b = (int)(id / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
     int lo, hi;
     win_range(a, b, lo, hi);
     const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
@@ -757,8 +769,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     T* gt = qt + NB * TILE;
     float* st = reinterpret_cast<float*>(gt + NB * TILE);    // [NB][2][64]: lse2, delta
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-    const int k0 = (int)(blockIdx.x % a.ktiles) * 32, hk = (int)(blockIdx.x / a.ktiles % a.Hkv);
-    const int b = (int)(blockIdx.x / a.ktiles / a.Hkv), G = a.Hq / a.Hkv, half = (wave >> 1) * 32;
+    const unsigned id = win_block();
+    const int k0 = (int)(id % a.ktiles) * 32, hk = (int)(id / a.ktiles % a.Hkv);
+    const int b = (int)(id / a.ktiles / a.Hkv), G = a.Hq / a.Hkv, half = (wave >> 1) * 32;
     int lo, hi;
     win_range(a, b, lo, hi);
     const int kw = k0 + (wave & 1) * 16, ki = kw + c16;

@@ -260,3 +260,32 @@ def test_clip_refusals_cpu():
     assert lib.dr_clip_global_norm(one, one, (C.c_int64 * 1)(-1), dt, 1, 1.0, None, w, n, None) == -1
     odd = (C.c_void_p * 1)(4098)
     assert lib.dr_clip_global_norm(odd, one, cnt, dt, 1, 1.0, None, w, n, None) == -1 and b"aligned" in lib.dr_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("n", [300001, (1 << 20) + 5])
+def test_embed_backward_long_lists(dev, n):
+    """Lists of half a thousand sort tiles, and beyond: rows sums of small integers, exact in fp32."""
+    from deeprec_amd import kernels as K
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(-1, 7001, (n,), generator=g)
+    gout = torch.randint(-8, 9, (n, 3), generator=g).float()
+    got = K.embed_backward(gout.to(dev), ids.to(dev), 7000, padding_idx=5)
+    ok = (ids >= 0) & (ids < 7000) & (ids != 5)
+    ref = torch.zeros((7000, 3), dtype=torch.float64).index_add_(0, ids[ok], gout[ok].double())
+    assert torch.equal(got.cpu().double(), ref)                              # |sums| < 2^24: no rounding anywhere
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [700, 1030, 131])
+def test_embed_backward_wide_rows(dev, d, dt):
+    """Rows wider than a workgroup's columns; runs inside a chunk, over one border and over many."""
+    from deeprec_amd import kernels as K
+    g = torch.Generator().manual_seed(d)
+    for n in (7, 70, 3000, 70001 if d < 200 else 300):
+        ids = torch.where(torch.rand(n, generator=g) < 0.4, 3, torch.randint(0, 60, (n,), generator=g))
+        gout = torch.randint(-3, 4, (n, d), generator=g).to(dt)
+        got = K.embed_backward(gout.to(dev), ids.to(dev), 60, scale=0.5)
+        ref = (torch.zeros((60, d), dtype=torch.float64).index_add_(0, ids, gout.double()) * 0.5).to(dt)   # exact, one rounding
+        assert torch.equal(got.cpu(), ref)
