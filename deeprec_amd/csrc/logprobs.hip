@@ -217,14 +217,21 @@ __device__ __forceinline__ Stat scan_row(const T* p, int lo, int hi, int wave, i
             if (first) best.bound(mv, K);
             first = false;
             if (__ballot(mv >= best.thr) != 0) {
+                // one bit per element, then each lane's candidates in turn, read again: the list's code stands here once
+                // (once per element it would not fit the instruction cache)
+                uint32_t want = 0;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int q = 0; q < V; ++q)
-                        if (__ballot(x[u][q] >= best.thr) != 0) {
-                            const int64_t e = (base + (int64_t)u * waves * 64 + lane) * V - a + q;
-                            best.add(x[u][q] >= best.thr, make_key(x[u][q], (int)e), K);
-                        }
+                    for (int q = 0; q < V; ++q) want |= x[u][q] >= best.thr ? 1u << (u * V + q) : 0u;
+#pragma unroll 1
+                while (__ballot(want != 0) != 0) {
+                    const int at = want != 0 ? __ffs((int)want) - 1 : 0;
+                    const int64_t e = (base + (int64_t)(at / V) * waves * 64 + lane) * V - a + at % V;
+                    const float v = want != 0 ? (float)p[e] : -__builtin_inff();
+                    best.add(v >= best.thr, make_key(v, (int)e), K);
+                    want &= want - 1;
+                }
             }
         }
     }
@@ -268,23 +275,19 @@ __device__ __forceinline__ void write_best(const LogpArgs& a, int64_t row, const
 // the four wavefronts' lists -> the row's K best (called by all 256 threads)
 __device__ __forceinline__ void block_best(const LogpArgs& a, int64_t row, const Stat& st, Best& best, uint64_t* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int rank;
-    const uint64_t key = best.ranked(a.K, rank);
-    if (rank < a.K) best.buf[rank] = key;                  // sorted, at most K
-    if (lane >= best.count || lane >= a.K) best.buf[lane] = 0ull;
+    if (best.count > 64) best.cut(a.K);
+    if (lane >= best.count) best.buf[lane] = 0ull;
     __syncthreads();
     if (wave != 0) return;
-    Best sum;
-    sum.init(all);
-    uint64_t k[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k[j] = all[j * LP_CAP + lane];
-    wave_sync_lds();
-    // the four lists fit the first wavefront's 256 entries
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum.add(k[j] != 0, k[j], a.K);
-    const uint64_t mine = sum.ranked(a.K, rank);
-    write_best(a, row, st, mine, rank, sum.count);
+    // at most 64 keys of each list: they fit the first wavefront's 256 entries, which its own list begins
+#pragma unroll 1
+    for (int j = 1; j < 4; ++j) {
+        const uint64_t k = all[j * LP_CAP + lane];
+        best.add(k != 0, k, a.K);
+    }
+    int rank;
+    const uint64_t mine = best.ranked(a.K, rank);
+    write_best(a, row, st, mine, rank, best.count);
 }
 
 template <class T, bool TOP>
@@ -361,7 +364,7 @@ __global__ __launch_bounds__(256) void logp_join_kernel(LogpArgs a) {
     if constexpr (TOP) {
         const int n = a.splits * 4 * a.K;
         const uint64_t* keys = a.pkey + (int64_t)row * n;
-        constexpr int J = 4;                                   // keys a lane requests together
+        constexpr int J = 4;                                   // keys a lane requests together (the selection below names them)
         for (int i0 = wave * 64 * J; i0 < n; i0 += 256 * J) {
             uint64_t k[J], top = 0;
 #pragma unroll
@@ -374,8 +377,15 @@ __global__ __launch_bounds__(256) void logp_join_kernel(LogpArgs a) {
             for (int j = 0; j < J; ++j) top = k[j] > top ? k[j] : top;
             // the K-th best of the lanes' best bounds the K-th best of all: hardly more than K candidates remain
             if (i0 < 256 * J) best.bound(top ? order_value((uint32_t)(top >> 32)) : -__builtin_inff(), a.K);
+            uint32_t want = 0;
 #pragma unroll
-            for (int j = 0; j < J; ++j) best.add(k[j] != 0 && order_value((uint32_t)(k[j] >> 32)) >= best.thr, k[j], a.K);
+            for (int j = 0; j < J; ++j) want |= k[j] != 0 && order_value((uint32_t)(k[j] >> 32)) >= best.thr ? 1u << j : 0u;
+#pragma unroll 1
+            while (__ballot(want != 0) != 0) {
+                const uint64_t key = want & 1u ? k[0] : want & 2u ? k[1] : want & 4u ? k[2] : k[3];
+                best.add(want != 0, key, a.K);
+                want &= want - 1;
+            }
         }
     }
     __syncthreads();
