@@ -365,22 +365,23 @@ struct KeyTiles {
 // ---- forward ---------------------------------------------------------------------------------------------------------------
 // A workgroup of 4 wavefronts takes 64 queries of one head; the key and value tiles it needs go through LDS, the next
 // tile's loads in flight while one is used (two buffers; one where two would not leave room for a second workgroup).
+// NH = 2: two heads of a group at once, which share the tiles, the key and value operands read from LDS and the masks.
 template <class T, int DP>
 constexpr int fwd_buffers() {
     return DP * (int)sizeof(T) <= 512 ? 2 : 1;
 }
 // Naming the workgroups per CU keeps the accumulators in ordinary registers: left alone the compiler moves all of them to
 // the accumulation registers and back around every tile's rescaling (64 of 350 instructions).
-template <class T, int DP, bool FAST>
-__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)sizeof(T) <= 512 ? 2 : 1)) void win_fwd_kernel(WinArgs a, T* __restrict__ out, float* __restrict__ lse) {
+template <class T, int DP, bool FAST, int NH>
+__global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)sizeof(T) <= 512 ? 2 : 1)) void win_fwd_kernel(WinArgs a, T* __restrict__ out, float* __restrict__ lse) {
     constexpr int LD = lds_ld<T, DP>(), NB = fwd_buffers<T, DP>(), TILE = WA_BK * LD;
     extern __shared__ char smem[];
     T* kt = reinterpret_cast<T*>(smem);
     T* vt = kt + NB * TILE;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const unsigned id = win_block();
-    const int q0 = (int)(id % a.tiles) * 64, h = (int)(id / a.tiles % a.Hq);
-    const int b = (int)(id / a.tiles / a.Hq), hk = h / (a.Hq / a.Hkv);
+    const int q0 = (int)(id % a.tiles) * 64, h = (int)(id / a.tiles % (a.Hq / NH)) * NH;   // this head, .. h + NH - 1
+    const int b = (int)(id / a.tiles / (a.Hq / NH)), hk = h / (a.Hq / a.Hkv);
     int lo, hi;
     win_range(a, b, lo, hi);
     const T* kp = (const T*)a.k + b * a.ks.b + hk * a.ks.h;
@@ -399,12 +400,17 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
         ks.load(kts.row0(0));
         vs.load(kts.row0(0));
     }
-    Oct<T> qf[DP / 32];
-    load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qs.b + (int64_t)clamp_row(qi, lo, hi) * a.qs.l + h * a.qs.h, q_ok, a.D, a.mode);
-    f32x4 o[DP / 16];
+    Oct<T> qf[NH][DP / 32];
+    f32x4 o[NH][DP / 16];
+    float m[NH], l[NH];
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f;
+    for (int y = 0; y < NH; ++y) {
+        load_frags<T, DP, FAST>(qf[y], (const T*)a.q + b * a.qs.b + (int64_t)clamp_row(qi, lo, hi) * a.qs.l + (h + y) * a.qs.h, q_ok, a.D, a.mode);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) o[y][t] = f32x4{0, 0, 0, 0};
+        m[y] = -__builtin_inff();
+        l[y] = 0.0f;
+    }
     const float c = a.scale * WA_LOG2E;
     if (kts.n > 0) {
         ks.store(kt);
@@ -420,11 +426,17 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
             vs.load(kts.row0(n + 1));
         }
         if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
-            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+            f32x4 s[NH][2];
+#pragma unroll
+            for (int y = 0; y < NH; ++y) s[y][0] = s[y][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int x = 0; x < DP / 32; ++x) {
-                s[0] = mma(row_frag<T>(kc + c16 * LD + 32 * x + 8 * g), qf[x], s[0]);
-                s[1] = mma(row_frag<T>(kc + (16 + c16) * LD + 32 * x + 8 * g), qf[x], s[1]);
+                const Oct<T> k0 = row_frag<T>(kc + c16 * LD + 32 * x + 8 * g), k1 = row_frag<T>(kc + (16 + c16) * LD + 32 * x + 8 * g);
+#pragma unroll
+                for (int y = 0; y < NH; ++y) {
+                    s[y][0] = mma(k0, qf[y][x], s[y][0]);
+                    s[y][1] = mma(k1, qf[y][x], s[y][1]);
+                }
             }
             // a tile that all 16 queries see whole needs no mask
             const bool whole = t0 >= lo && t0 + WA_BK - 1 <= qw && qw >= lo && qw + 15 < hi && qw + 15 - t0 < a.W;
@@ -437,41 +449,54 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
                         for (int i = 0; i < 4; ++i) {
                             const int k = k0 + 16 * x + i;
                             const bool first = ((unsigned)(k - lo) < (unsigned)a.S) & (k <= qi) & q_ok;
-                            s[x][i] = ((unsigned)(k - k_first) < (unsigned)k_count) | first ? s[x][i] : -__builtin_inff();
+                            const bool seen = ((unsigned)(k - k_first) < (unsigned)k_count) | first;
+#pragma unroll
+                            for (int y = 0; y < NH; ++y) s[y][x][i] = seen ? s[y][x][i] : -__builtin_inff();
                         }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[x][i] = (unsigned)(k0 + 16 * x + i - k_first) < (unsigned)k_count ? s[x][i] : -__builtin_inff();
+                        for (int i = 0; i < 4; ++i) {
+                            const bool seen = (unsigned)(k0 + 16 * x + i - k_first) < (unsigned)k_count;
+#pragma unroll
+                            for (int y = 0; y < NH; ++y) s[y][x][i] = seen ? s[y][x][i] : -__builtin_inff();
+                        }
                 }
             }
-            float mt = s[0][0];
+            Oct<T> p[NH];
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int y = 0; y < NH; ++y) {
+                float mt = s[y][0][0];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[x][i]);
-            mt = groups_max(mt);
-            const float mn = fmaxf(m, mt * c), ms = mn == -__builtin_inff() ? 0.0f : mn;    // m: in units of log 2
-            const float alpha = __builtin_amdgcn_exp2f(m - ms);
-            m = mn;
-            float sum = 0.0f;
+                for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+                    for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[y][x][i]);
+                mt = groups_max(mt);
+                const float mn = fmaxf(m[y], mt * c), ms = mn == -__builtin_inff() ? 0.0f : mn;    // m: in units of log 2
+                const float alpha = __builtin_amdgcn_exp2f(m[y] - ms);
+                m[y] = mn;
+                float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[x][i] = __builtin_amdgcn_exp2f(fmaf(s[x][i], c, -ms));
-                    sum += s[x][i];
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[y][x][i] = __builtin_amdgcn_exp2f(fmaf(s[y][x][i], c, -ms));
+                        sum += s[y][x][i];
+                    }
+                l[y] = fmaf(l[y], alpha, sum);
+                if (__ballot(alpha != 1.0f) != 0) {
+#pragma unroll
+                    for (int t = 0; t < DP / 16; ++t) o[y][t] *= alpha;
                 }
-            l = fmaf(l, alpha, sum);
-            if (__ballot(alpha != 1.0f) != 0) {
-#pragma unroll
-                for (int t = 0; t < DP / 16; ++t) o[t] *= alpha;
+                p[y] = to_oct<T>(s[y][0], s[y][1]);
             }
-            const Oct<T> p = to_oct<T>(s[0], s[1]);
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) o[t] = mma(col_frag<T, LD>(vc, 16 * t), p, o[t]);
+            for (int t = 0; t < DP / 16; ++t) {
+                const Oct<T> vf = col_frag<T, LD>(vc, 16 * t);
+#pragma unroll
+                for (int y = 0; y < NH; ++y) o[y][t] = mma(vf, p[y], o[y][t]);
+            }
         }
         if (NB == 1) __syncthreads();
         if (n + 1 < kts.n) {
@@ -480,23 +505,27 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 3 : (DP * (int)si
         }
         __syncthreads();
     }
-    l = groups_sum(l);
+#pragma unroll
+    for (int y = 0; y < NH; ++y) l[y] = groups_sum(l[y]);
     if (qi >= a.L) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;                 // a NaN stays one
-    T* op = out + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-        const int d = 16 * t + 4 * g;
-        if (FAST || (d + 4 <= a.D && a.wide)) {
-            float r[4] = {o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv};
-            store_f32<T, 4>(op + d, r);
-        } else {
+    for (int y = 0; y < NH; ++y) {
+        const float inv = l[y] == 0.0f ? 0.0f : 1.0f / l[y];                   // a NaN stays one
+        T* op = out + (((int64_t)b * a.L + qi) * a.Hq + h + y) * a.D;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (d + i < a.D) op[d + i] = (T)(o[t][i] * inv);
+        for (int t = 0; t < DP / 16; ++t) {
+            const int d = 16 * t + 4 * g;
+            if (FAST || (d + 4 <= a.D && a.wide)) {
+                float r[4] = {o[y][t][0] * inv, o[y][t][1] * inv, o[y][t][2] * inv, o[y][t][3] * inv};
+                store_f32<T, 4>(op + d, r);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d + i < a.D) op[d + i] = (T)(o[y][t][i] * inv);
+            }
         }
+        if (g == 0) lse[((int64_t)b * a.Hq + h + y) * a.L + qi] = l[y] == 0.0f ? -__builtin_inff() : (m[y] + log2f(l[y])) * WA_LN2;
     }
-    if (g == 0) lse[((int64_t)b * a.Hq + h) * a.L + qi] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * WA_LN2;
 }
 
 // ---- backward: dQ ------------------------------------------------------------------------------------------------------------
@@ -1190,15 +1219,23 @@ static int64_t win_chunks(int64_t L, int64_t window, int32_t sinks, int group) {
     return (L + WA_CHUNK - 1) / WA_CHUNK;
 }
 
-template <class T, int DP, bool FAST>
-static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
+template <class T, int DP, bool FAST, int NH>
+static int win_fwd_heads(const WinArgs& a, void* out, hipStream_t st) {
     const size_t lds = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
-    int rc = win_lds(win_fwd_kernel<T, DP, FAST>, lds);
+    int rc = win_lds(win_fwd_kernel<T, DP, FAST, NH>, lds);
     if (rc != DR_OK) return rc;
-    DR_LAUNCH_NAMED("win_fwd_kernel", (win_fwd_kernel<T, DP, FAST>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), lds, st, a,
-                    (T*)out, a.lse);
+    DR_LAUNCH_NAMED("win_fwd_kernel", (win_fwd_kernel<T, DP, FAST, NH>), dim3((unsigned)a.tiles * (a.Hq / NH) * a.B), dim3(256), lds,
+                    st, a, (T*)out, a.lse);
     DR_CHECK_LAUNCH("win_fwd_kernel");
     return DR_OK;
+}
+template <class T, int DP, bool FAST>
+static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
+    // two heads at a time where that leaves 4 workgroups per CU and registers allow: 16 x 2048 x 8 / 2 heads x 64 bf16 48 us
+    // against 56; but D = 128 51 against 48, fp32 with D = 64 87 against 83, and at a quarter of the grid 10.5 against 8.3 us
+    if constexpr (FAST && DP * (int)sizeof(T) <= 128 && sizeof(T) == 2)
+        if (a.Hq / a.Hkv % 2 == 0 && (int64_t)a.tiles * a.Hq * a.B >= 2048) return win_fwd_heads<T, DP, FAST, 2>(a, out, st);
+    return win_fwd_heads<T, DP, FAST, 1>(a, out, st);
 }
 template <class T, int DP, bool FAST>
 static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStream_t st) {

@@ -413,3 +413,28 @@ def test_token_over_many_splits(dev, B, L, Hq, Hkv, D, dt):
     rel = 2 * ds + (L / 8 + 40) * U + (0.0 if dt == torch.float32 else e) + 4 * U * lse
     lim = rel * torch.einsum("bhl,blhd->bhd", p, V.abs()) * (1 + e) + e * ref.abs() + 1e-30 + torch.finfo(dt).smallest_normal * e
     _within("out", out, ref, lim)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_many_rows_with_shared_heads(dev, D, dt):
+    """Enough rows that the forward takes two heads of a group at a time (full tiles; B is cut for the 64-bit restatement,
+    whose rows are compared one by one)."""
+    from deeprec_amd import kernels as Kn
+    B, L, Hq, Hkv, W, S = 130, 200, 4, 1, 40, 3
+    q, k, v, go, begin, end = _inputs(B, L, Hq, Hkv, D, dt, D)
+    d = lambda t: t.to(dev)
+    mask = dict(window=W, sinks=S, begin=d(begin), end=d(end))
+    out, lse = Kn.window_attn_forward(d(q), d(k), d(v), **mask)
+    few = torch.tensor([0, 1, 2, 3, 70, 129])
+    vis = _visible(len(few), L, W, S, begin[few], end[few])
+    r = _ref(q[few], k[few], v[few], go[few], vis, D ** -0.5)
+    _within("out", out.cpu()[few], r["out"], _limits(r, dt, D, Hq // Hkv, D ** -0.5)[0])
+    got, none = lse.cpu().double()[few], ~vis.any(2)[:, None].expand(len(few), Hq, L)
+    assert bool((got[none] == -math.inf).all()) and bool(((got - r["lse"]).abs()[~none] < 1e-5 * (1 + r["lse"].abs()[~none])).all())
+    # the other rows: as each row alone (one head at a time) gives them, but for the order of no sum
+    for b in (5, 64, 128):
+        alone, ls = Kn.window_attn_forward(d(q[b:b + 1]), d(k[b:b + 1]), d(v[b:b + 1]), window=W, sinks=S, begin=d(begin[b:b + 1]),
+                                           end=d(end[b:b + 1]))
+        assert torch.equal(alone[0], out[b]) and torch.equal(ls[0], lse[b])
