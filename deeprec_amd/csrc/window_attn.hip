@@ -334,7 +334,8 @@ __device__ __forceinline__ void wave_stage(T* tile, const T* base, int64_t ld, i
 }
 // Workgroups go to the 8 XCDs in turn and each XCD has its own L2: dealt out one by one, neighbours along the sequence, which
 // read the same rows, would fetch them into 8 caches.  So runs of WA_RUN neighbours go to one XCD, the runs in turn (whole
-// eighths of the grid would leave an XCD with nothing but the short histories of a batch).
+// eighths of the grid would leave an XCD with nothing but the short histories of a batch).  dK / dV of 4 x 2047 x 8 / 2 heads x
+// 128 bf16: 56.5 us one by one, 54.0 in runs of 16, 53.6 in runs of 32; of 64 x 200 x 2 x 64 fp32: 35.3, 33.1, 32.6 us.
 constexpr int WA_RUN = 32;
 __device__ __forceinline__ unsigned win_block() {
     constexpr unsigned ROUND = 8 * WA_RUN;
@@ -366,6 +367,10 @@ struct KeyTiles {
 // A workgroup of 4 wavefronts takes 64 queries of one head; the key and value tiles it needs go through LDS, the next
 // tile's loads in flight while one is used (two buffers; one where two would not leave room for a second workgroup).
 // NH = 2: two heads of a group at once, which share the tiles, the key and value operands read from LDS and the masks.
+// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 28 us, 8.0 useful GFLOP = 285 TFLOP/s.  LDS reads (16 KB a wavefront and
+// tile), exponentials and matrix instructions take about a third each and overlap only across wavefronts: without its loads
+// from memory the kernel takes 24.6 us, without its products 19.4.  64 x 200 x 2 x 64 fp32, window 50: 18 us.
+// Tried: 64 keys in one buffer instead of 32 in two, 35.6 us.
 template <class T, int DP>
 constexpr int fwd_buffers() {
     return DP * (int)sizeof(T) <= 512 ? 2 : 1;
@@ -716,6 +721,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 
 // ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
 // S = Q K^T here, so a lane holds one KEY and four queries of each 16: the A operand of dV = P^T dO and dK = dS^T Q.
+// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 53 us (dQ: 48 us), 64 x 200 x 2 x 64 fp32: 33 us (25 us).  A step of 32 queries
+// x 16 keys reads 32 KB from LDS for 40 matrix instructions: LDS takes half of the time, and 32 keys a wavefront, which
+// would halve that, do not fit the registers at D = 128.
 // one (32 queries x 16 keys) step: adds to dk, dv what the queries [q_first, q_first + q_count) give the lane's key (whole:
 // all of them do)
 template <class T, int DP>
@@ -782,21 +790,18 @@ __device__ __forceinline__ float grad_scale(const WinArgs& a, int b, int h0, int
 // A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
 // head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
 // of the queries are added up at the end.  What the first items get from queries beyond the window is found here too
-// where that is at most 8 more steps (short rows: at 64 x 200 x 2 x 64 fp32 a launch of 11 us is saved); else it comes
-// from win_sink_kernel's partial sums, added last and in order.
-template <class T, int DP>
-constexpr int dkdv_buffers() {
-    return DP * (int)sizeof(T) <= 256 ? 2 : 1;
-}
+// where that is at most 8 more steps (backward of 64 x 200 x 2 x 64 fp32 with 2 first items, 3 steps: 62 us, 67 us with a launch
+// of its own; 32 x 600, 9 steps: 101 and 94 us); else it comes from win_sink_kernel's partial sums, added last and in order.
+// (One buffer: with two the two workgroups on the CU, which hide each other's barriers, gain nothing.)
 // a second workgroup on the CU is worth more than registers to spare (at D <= 128 in 16 bits, 64 in fp32)
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_dkdv_kernel(WinArgs a, T* __restrict__ dk_out, T* __restrict__ dv_out) {
-    constexpr int LD = lds_ld<T, DP>(), NB = dkdv_buffers<T, DP>(), R = 64, TILE = R * LD;
+    constexpr int LD = lds_ld<T, DP>(), R = 64, TILE = R * LD;
     constexpr bool AHEAD = DP * (int)sizeof(T) <= 512;       // else the next tile does not fit the registers
     extern __shared__ char smem[];
     T* qt = reinterpret_cast<T*>(smem);
-    T* gt = qt + NB * TILE;
-    float* st = reinterpret_cast<float*>(gt + NB * TILE);    // [NB][2][64]: lse2, delta
+    T* gt = qt + TILE;
+    float* st = reinterpret_cast<float*>(gt + TILE);         // [2][64]: lse2, delta
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const unsigned id = win_block();
     const int k0 = (int)(id % a.ktiles) * 32, hk = (int)(id / a.ktiles % a.Hkv);
@@ -834,10 +839,10 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             gs.base += a.D;
         }
     };
-    auto store = [&](int buf) {
-        qs.store(qt + buf * TILE);
-        gs.store(gt + buf * TILE);
-        if (threadIdx.x < 2 * R) st[buf * 2 * R + threadIdx.x] = stat;
+    auto store = [&]() {
+        qs.store(qt);
+        gs.store(gt);
+        if (threadIdx.x < 2 * R) st[threadIdx.x] = stat;
     };
     if (total > 0) load();
     Oct<T> kf[DP / 32], vf[DP / 32];
@@ -846,20 +851,20 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     f32x4 dk[DP / 16], dv[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
-    if (total > 0) store(0);
+    if (total > 0) store();
     __syncthreads();
     for (int n = 0, i = 0; n < total; ++n) {
-        const int t0 = tq0 + i * R + half, buf = NB == 2 ? n & 1 : 0;
+        const int t0 = tq0 + i * R + half;
         if (++i == nt) i = 0;
         if (AHEAD && n + 1 < total) load();
         if (kw <= t0 + 31 && (t0 - (kw + 15) < a.W || kw < first_end) && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
-            dkdv_step<T, DP>(a, qt + buf * TILE + half * LD, gt + buf * TILE + half * LD, st + buf * 2 * R + half,
-                             st + buf * 2 * R + R + half, kf, vf, t0, ki, q_count, whole, a.scale * up, dk, dv);
+            dkdv_step<T, DP>(a, qt + half * LD, gt + half * LD, st + half, st + R + half, kf, vf, t0, ki, q_count, whole,
+                             a.scale * up, dk, dv);
         }
-        if (NB == 1) __syncthreads();
+        __syncthreads();
         if (!AHEAD && n + 1 < total) load();
-        if (n + 1 < total) store(NB == 2 ? (n + 1) & 1 : 0);
+        if (n + 1 < total) store();
         __syncthreads();
     }
     // the second query half's sums join the first's over LDS: [key half][2][16][DP] fp32, which the tiles have room for
@@ -915,7 +920,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 
 // ---- backward: what the first items get from queries beyond the window ----------------------------------------------------------
 // Every query of a long history sees them, so their sums are split over chunks of 64 queries: NW wavefronts, each with its
-// own tiles of 32 queries in LDS, all on the same 16 first items, added up over LDS in order.
+// own tiles of 32 queries in LDS, all on the same 16 first items, added up over LDS in order.  4 x 2047 x 8 / 2 heads x 128 bf16:
+// 13 us, bound by the latency of a chunk's loads; every wavefront does one or two tiles.
 constexpr int WA_CHUNK = 64;
 template <class T, int DP>
 constexpr int sink_waves() {
@@ -1002,7 +1008,9 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
 // The query stands at position end - 1 and sees the first items and the window before it.  A workgroup takes one key head
 // (its up to 16 query heads are the 16 columns of the tile) and a share of the visible keys; its wavefronts take 32 keys
 // in turn, keys straight into registers, values through their own LDS tile, and are joined at the end.  With few sequences
-// the keys are split over workgroups and win_join_kernel adds up.
+// the keys are split over workgroups and win_join_kernel adds up.  64 x 260 keys x 8 / 2 heads x 64 bf16: 7 us, three round trips
+// to memory one after the other (8 wavefronts or loads a tile ahead: 6.5 us); 64 x 4096 keys: 28 us = 4.8 TB/s;
+// one sequence of 300000 keys: 36 us = 4.2 TB/s.
 struct TokenArgs {
     const void *q, *k, *v;
     int64_t qb, qh;
@@ -1240,7 +1248,7 @@ static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
 template <class T, int DP, bool FAST>
 static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStream_t st) {
     const size_t tiles = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
-    const size_t lds = (size_t)dkdv_buffers<T, DP>() * (2 * 64 * lds_ld<T, DP>() * sizeof(T) + 128 * sizeof(float));
+    const size_t lds = 2 * 64 * lds_ld<T, DP>() * sizeof(T) + 128 * sizeof(float);
     int rc = win_lds(win_dq_kernel<T, DP, FAST>, tiles);
     if (rc != DR_OK) return rc;
     DR_LAUNCH_NAMED("win_dq_kernel", (win_dq_kernel<T, DP, FAST>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), tiles, st, a,
@@ -1290,7 +1298,8 @@ static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int D, in
 }
 static int64_t token_keys(int64_t L, int64_t window, int32_t sinks) { return window >= L ? L : (window + sinks < L ? window + sinks : L); }
 
-// FAST: the head dim fills its tile and rows are read in 16-byte pieces (no column checks anywhere)
+// FAST: the head dim fills its tile and rows are read in 16-byte pieces: no column checks anywhere (forward + backward of
+// 4 x 2047 x 8 / 2 heads x 128 bf16: 31 + 115 us, 47 + 141 us without; 64 x 200 x 2 x 64 fp32: 18 + 62 and 19 + 68 us)
 #define WIN_BY_D(T, fast, launch, ...)                                                                        \
     return a.D <= 32    ? ((fast) && a.D == 32 ? launch<T, 32, true>(__VA_ARGS__) : launch<T, 32, false>(__VA_ARGS__))   \
            : a.D <= 64  ? ((fast) && a.D == 64 ? launch<T, 64, true>(__VA_ARGS__) : launch<T, 64, false>(__VA_ARGS__))   \
