@@ -291,7 +291,8 @@ constexpr uint8_t RUN_FILLS = 2;    // one run fills the chunk and goes on on bo
 // One group of LPR lanes per chunk.  A run (equal keys) that lies inside the chunk is finished here; the part of a run that
 // began in an earlier chunk goes to part[chunk][0], the part of one that goes on behind the chunk to part[chunk][1] (a run
 // that does both: [0]).  The chunk's keys and positions are fetched once, spread over the lanes, so that the only
-// dependent step left is position -> row, 16 rows in flight.
+// dependent step left is position -> row, up to 16 rows in flight.  204800 entries of 128 bf16: 16.6 us = 3.2 TB/s (joins 8 us);
+// 3668 entries of 95 fp32: 4.2 us.
 template <class T, int V, int LPR, int CH>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedArgs a, const T* __restrict__ gout, T* __restrict__ grad) {
     constexpr int E = CH / LPR > 0 ? CH / LPR : 1;                  // entries a lane keeps
