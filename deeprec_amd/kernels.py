@@ -1361,8 +1361,16 @@ _WIN_STRIDES = C.c_int64 * 3
 
 def _win_operands(q, k, v, q_dims, window, sinks, scale, begin, end):
     """Checks what the three calls share: strides as C arrays, sizes, mask arguments."""
-    sq = _win_tensor(q, "q", q_dims)
-    sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
+    try:                                                                    # the usual case in one expression of cheap calls
+        dev, dt = torch._C._cuda_getDevice(), q.dtype
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
+        good = (q.get_device() == dev and k.get_device() == dev and v.get_device() == dev and dt in DTYPES and k.dtype == dt
+                and v.dtype == dt and len(sq) == q_dims and len(sk) == 4 and len(sv) == 4 and sq[-1] == 1 and sk[3] == 1 and sv[3] == 1)
+    except (AttributeError, TypeError):
+        good = False
+    if not good:                                                            # names the fault, if there is one
+        sq = _win_tensor(q, "q", q_dims)
+        sk, sv = _win_tensor(k, "k", 4, q.dtype), _win_tensor(v, "v", 4, q.dtype)
     qs, ks = q.shape, k.shape
     B, L, Hkv, D = ks
     Hq = qs[-2]
