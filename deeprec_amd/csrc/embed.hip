@@ -381,9 +381,11 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedArgs a, T* __restr
     constexpr int GROUPS = 256 / LPR;
     __shared__ float red[GROUPS][LPR * V];
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, wl = threadIdx.x & 63;
+    // the four chunks' states in one load (the array is padded)
+    const uint32_t states = reinterpret_cast<const uint32_t*>(a.state)[blockIdx.x];
     for (int j = 0; j < 4; ++j) {
         const int64_t chunk = (int64_t)blockIdx.x * 4 + j;
-        if (chunk >= a.chunks || a.state[chunk] != RUN_BEGINS) continue;      // workgroup-uniform
+        if (chunk >= a.chunks || ((states >> (8 * j)) & 255u) != RUN_BEGINS) continue;   // workgroup-uniform
         int64_t last = chunk + 1;                                             // last chunk the run reaches
         for (;;) {
             const int64_t at = last + wl;

@@ -794,6 +794,8 @@ class _Embedding(torch.autograd.Function):
 def embedding(weight, ids, scale=1.0, padding_idx=None):
     """scale * weight[ids] with a dense gradient for `weight` [rows, d] (dr_embed_forward / dr_embed_backward); row
     padding_idx gets none.  The lookup of weights that autograd owns; Table.lookup serves the optimizer's sparse tables."""
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError("embedding: padding_idx %d is outside the table of %d rows" % (padding_idx, weight.shape[0]))
     return _Embedding.apply(weight, ids, float(scale), padding_idx)
 
 

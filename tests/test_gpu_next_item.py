@@ -233,3 +233,10 @@ def test_captured_training_step(dev):
         torch.cuda.synchronize()
         for a, b in zip(res, eager):
             assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * float(b.float().abs().max()))   # library products may differ in order
+
+
+def test_embedding_refuses_a_padding_row_outside_the_table():
+    from deeprec_amd.models import _common as M
+    for bad in (-1, 5):
+        with pytest.raises(ValueError, match="padding_idx"):
+            M.embedding(torch.zeros(5, 2), torch.zeros(3, dtype=torch.int32), padding_idx=bad)
