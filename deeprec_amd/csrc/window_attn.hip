@@ -478,15 +478,17 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[y][x][i]);
                 mt = groups_max(mt);
-                const float mn = fmaxf(m[y], mt * c), ms = mn == -__builtin_inff() ? 0.0f : mn;    // m: in units of log 2
-                const float alpha = __builtin_amdgcn_exp2f(m[y] - ms);
+                // m: the largest score itself.  Its weight is 2^0 whatever the scores' size: with m c rounded, and s c - m c
+                // in one fma, it would be 2 to the rounding error of m c, beyond any range from scores of 2^31 on
+                const float mn = fmaxf(m[y], mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f((m[y] - ms) * c);
                 m[y] = mn;
                 float sum = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[y][x][i] = __builtin_amdgcn_exp2f(fmaf(s[y][x][i], c, -ms));
+                        s[y][x][i] = __builtin_amdgcn_exp2f((s[y][x][i] - ms) * c);
                         sum += s[y][x][i];
                     }
                 l[y] = fmaf(l[y], alpha, sum);
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
                     if (d + i < a.D) op[d + i] = (T)(o[y][t][i] * inv);
             }
         }
-        if (g == 0) lse[((int64_t)b * a.Hq + h + y) * a.L + qi] = l[y] == 0.0f ? -__builtin_inff() : (m[y] + log2f(l[y])) * WA_LN2;
+        if (g == 0) lse[((int64_t)b * a.Hq + h + y) * a.L + qi] = l[y] == 0.0f ? -__builtin_inff() : fmaf(m[y], a.scale, log2f(l[y]) * WA_LN2);
     }
 }
 

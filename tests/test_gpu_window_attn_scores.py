@@ -1,0 +1,67 @@
+"""Windowed attention at scores, scales and values far from 1, against a 64-bit restatement.
+
+u = 2^-24, e = finfo(t).eps / 2 (0.. one rounding to the storage type).  Queries and keys are small integers times a power of
+two and scales are powers of two, so that every score is exact in fp32 and in 64 bits: what is left of the error is that of
+the softmax, not of the dot products.  With x = (s - max) c, c = scale log2 e (two roundings) and one more in the product,
+the weight w = 2^x is off by 3 u |ln w| + 2 u (the instruction's own error), the row's sum by the mean of that over the row:
+  rel p_ij <= u (3 |ln w_ij| + 3 sum_j p_ij |ln w_ij| + n / 8 + 40)."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_window_attn import DTYPES, U, _ref, _visible, _within
+
+gpu = pytest.mark.gpu
+
+
+def _integers(B, L, Hq, Hkv, D, dt, unit, top, seed):
+    """q, k: integers in [-top, top] times `unit`; v, dO normal; histories that begin and end inside the row, one empty."""
+    g = torch.Generator().manual_seed(seed)
+    whole = lambda *s: (torch.randint(-top, top + 1, s, generator=g).double() * unit).to(dt)
+    q, k = whole(B, L, Hq, D), whole(B, L, Hkv, D)
+    v, go = (torch.randn(s, generator=g).to(dt) for s in ((B, L, Hkv, D), (B, L, Hq, D)))
+    begin = torch.tensor([0, L // 3, 5, 0][:B], dtype=torch.int32)
+    end = torch.tensor([L, L - 3, 5, L][:B], dtype=torch.int32)
+    return q, k, v, go, begin, end
+
+
+def _relp(r, vis):
+    """The bound of rel p above, [B, H, L, L]; 0 where nothing is visible."""
+    top = r["p"].amax(-1, keepdim=True)
+    w = r["p"] / torch.where(top > 0, top, torch.ones_like(top))
+    ln = torch.where(w > 0, w, torch.ones_like(w)).log().abs()
+    return U * (3 * ln + 3 * (r["p"] * ln).sum(-1, keepdim=True) + r["n"] / 8 + 40) * vis[:, None]
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 150, 4, 2, 64, 40, 3), (130, 200, 4, 1, 32, 40, 3), (3, 70, 2, 2, 50, 70, 0)])
+@pytest.mark.parametrize("scale,unit", [(2.0 ** 27, 1.0), (2.0 ** 33, 1.0), (2.0 ** 99, 1.0), (2.0 ** -3, 2.0 ** 11), (2.0 ** -30, 2.0 ** 11)])
+def test_forward_at_large_scores(dev, shape, dt, scale, unit):
+    """Scores of 2^-30 to 2^110: only a query without keys gives zeros and lse -inf, and the single-token form agrees.
+    P is rounded to 16-bit types (e) or not; A = sum p |v|."""
+    from deeprec_amd import kernels as Kn
+    B, L, Hq, Hkv, D, W, S = shape
+    n = min(B, 3)                                                            # the rest repeats these
+    q, k, v, go, begin, end = _integers(n, L, Hq, Hkv, D, dt, unit, 4, L + D)
+    vis = _visible(n, L, W, S, begin, end)
+    r = _ref(q, k, v, go, vis, scale)
+    e = torch.finfo(dt).eps / 2
+    absV = r["V"].abs()
+    lim = ((r["p"] * (_relp(r, vis) + (0.0 if dt == torch.float32 else e))) @ absV).permute(0, 2, 1, 3)
+    lim = lim * (1 + e) + e * r["out"].abs() + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps + 1e-30
+    d = lambda t: t.repeat(-(-B // n), *[1] * (t.dim() - 1))[:B].to(dev)
+    mask = dict(window=W, sinks=S, scale=scale, begin=d(begin), end=d(end))
+    out, lse = Kn.window_attn_forward(d(q), d(k), d(v), **mask)
+    _within("out", out[:n], r["out"], lim)
+    none = ~vis.any(2)[:, None].expand(n, Hq, L)
+    got = lse[:n].cpu().double()
+    assert bool((got[none] == -math.inf).all())
+    assert bool(((got - r["lse"]).abs()[~none] <= 4 * U * r["lse"].abs()[~none] + 1e-5).all())
+    last = end.long().clamp(0, L) - 1
+    rows = torch.arange(n)
+    some = (end > begin) & (last >= 0)
+    tok = Kn.window_attn_token(q[rows, last.clamp_min(0)].to(dev), k.to(dev), v.to(dev), W, S, scale, begin.to(dev), end.to(dev))
+    want = torch.where(some[:, None, None], r["out"][rows, last.clamp_min(0)], torch.zeros((), dtype=torch.float64))
+    _within("token", tok, want, torch.where(some[:, None, None], lim[rows, last.clamp_min(0)], torch.full((), 1e-30, dtype=torch.float64)))
