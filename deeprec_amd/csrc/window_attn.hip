@@ -185,7 +185,8 @@ struct WinArgs {
     const int32_t *begin, *end;
     int mode, modeg;           // how rows of q, k, v / of out, gout are read
     int wide;                  // rows of out, dq take stores of four elements
-    float *lse, *delta;        // [B, Hq, L]
+    float *lse;                // [B, Hq, L]
+    float *delta, *ref, *norm; // [B, Hq, L]: -delta; p = exp2((s - ref) c - norm), see win_dq_kernel
     float* gmax;               // fp16: largest |dO| of every 16 queries [B, Hq, 4 tiles]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
     int chunks;                // far sinks: workgroups along the sequence; 0: none
@@ -544,6 +545,11 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
 // r being small, the second sum needs no more than P rounded to 16 bits.  The first one's weights are split into two halves
 // (hi + what hi misses), one more matrix instruction instead of another half step lost.  (Running the tiles twice, first
 // for delta, is as exact and took 77 us where this takes 48 at 4 x 2047 x 8 x 128.)
+// P from lse alone would be off by lse's rounding: 1e-3 of P at scores of 1e4.  So lse only gives a reference near the row's
+// maximum, ref = lse / scale; the kernel, which sees the whole row, sums the weights 2^((s - ref) c) itself, divides by the sum
+// l in the end and hands ref and norm = log2 l to the others.  Where |lse| reaches WA_FAR its rounding (half a unit of log 2 at
+// 2^23) could carry the weights out of range: there the workgroup takes the maximum itself in a first run over the keys.
+constexpr float WA_FAR = 65536.0f;
 template <class T>
 __device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>& hi, Oct<T>& lo) {
     hi = to_oct<T>(a, b);
@@ -593,7 +599,13 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     const int64_t irow = (((int64_t)b * a.L + qc) * a.Hq + h) * a.D, srow = ((int64_t)b * a.Hq + h) * a.L;
     load_frags<T, DP, FAST>(qf, (const T*)a.q + b * a.qs.b + (int64_t)qc * a.qs.l + h * a.qs.h, q_ok, a.D, a.mode);
     load_frags<T, DP, FAST>(gf, (const T*)a.gout + irow, q_ok, a.D, a.modeg);
-    const float lse2 = q_ok ? a.lse[srow + qc] * WA_LOG2E : 0.0f;            // in units of log 2
+    float ref = q_ok ? a.lse[srow + qc] / a.scale : 0.0f, l = 0.0f;
+    bool far;                                                                // the same in all four wavefronts
+    {
+        const int at = q0 + lane;
+        const float x = at >= lo && at < hi ? a.lse[srow + at] : 0.0f;
+        far = __ballot(!(fabsf(x) < WA_FAR)) != 0;
+    }
     float delta = 0.0f, fix = 0.0f;
     {
         Oct<T> of[DP / 32];
@@ -625,6 +637,35 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         if (FIX) pk[t] = f32x4{0, 0, 0, 0};
     }
     const float c = a.scale * WA_LOG2E;
+    // whether this wavefront's queries see anything of the tile
+    auto needs = [&](int t0) { return qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S); };
+    auto sees = [&](int k) {
+        return ((unsigned)(k - k_first) < (unsigned)k_count) | (((unsigned)(k - lo) < (unsigned)a.S) & (k <= qi) & q_ok);
+    };
+    if (far) {
+        float mx = -__builtin_inff();
+        for (int n = 0; n < kts.n; ++n) {
+            const int t0 = kts.row0(n);
+            ks.load(t0);
+            __syncthreads();
+            ks.store(kt);
+            __syncthreads();
+            if (!needs(t0)) continue;
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) s[y] = mma(row_frag<T>(kt + (16 * y + c16) * LD + 32 * x + 8 * g), qf[x], s[y]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sees(t0 + 16 * y + 4 * g + i) ? s[y][i] : -__builtin_inff());
+        }
+        mx = groups_max(mx);
+        ref = mx == -__builtin_inff() ? 0.0f : mx;
+        if (kts.n > 0) ks.load(kts.row0(0));                                 // the values' first tile is still held
+        __syncthreads();
+    }
     if (kts.n > 0) {
         ks.store(kt);
         vs.store(vt);
@@ -638,8 +679,9 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             ks.load(kts.row0(n + 1));
             vs.load(kts.row0(n + 1));
         }
-        if (qlo <= qhi && t0 <= qhi && (t0 + WA_BK - 1 > qlo - a.W || t0 < lo + a.S)) {
-            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+        if (needs(t0)) {
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+            f32x4 dp[2] = {f32x4{-delta, -delta, -delta, -delta}, f32x4{-delta, -delta, -delta, -delta}};   // dP - delta
 #pragma unroll
             for (int x = 0; x < DP / 32; ++x)
 #pragma unroll
@@ -651,15 +693,13 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[y][i] = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -lse2));
+                for (int i = 0; i < 4; ++i) s[y][i] = __builtin_amdgcn_exp2f((s[y][i] - ref) * c);
             if (!whole) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int k = t0 + 16 * y + 4 * g + i;
-                        const bool seen = ((unsigned)(k - k_first) < (unsigned)k_count) |
-                                          (((unsigned)(k - lo) < (unsigned)a.S) & (k <= qi) & q_ok);
+                        const bool seen = sees(t0 + 16 * y + 4 * g + i);
                         s[y][i] = seen ? s[y][i] : 0.0f;
                         dp[y][i] = seen ? dp[y][i] : 0.0f;     // whatever it was: 0 times a finite number
                     }
@@ -669,7 +709,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[y][i] *= (dp[y][i] - delta) * up;
+                    l += s[y][i];
+                    s[y][i] *= dp[y][i] * up;
                     fix += s[y][i];
                 }
             if constexpr (FIX) {
@@ -695,8 +736,10 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         }
         __syncthreads();
     }
+    l = groups_sum(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;                           // a NaN stays one
     if constexpr (FIX) {
-        fix = groups_sum(fix);
+        fix = groups_sum(fix) * inv;
         delta += fix * down;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t)
@@ -704,8 +747,12 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(-fix, pk[t][i], acc[t][i]);
     }
     if (qi >= a.L) return;
-    if (g == 0) a.delta[srow + qi] = delta;
-    down *= a.scale;
+    if (g == 0) {
+        a.delta[srow + qi] = -delta;
+        a.ref[srow + qi] = ref;
+        a.norm[srow + qi] = l == 0.0f ? 0.0f : log2f(l);
+    }
+    down *= inv * a.scale;
     T* op = dq + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
@@ -729,14 +776,19 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 // one (32 queries x 16 keys) step: adds to dk, dv what the queries [q_first, q_first + q_count) give the lane's key (whole:
 // all of them do)
 template <class T, int DP>
-__device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* lse2, const float* delta,
+__device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* ref, const float* norm, const float* delta,
                                           const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int q_first,
                                           int q_count, bool whole, float dscale, f32x4 (&dk)[DP / 16],
                                           f32x4 (&dv)[DP / 16]) {
     constexpr int LD = lds_ld<T, DP>();
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const float c = a.scale * WA_LOG2E;
-    f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, dp[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    f32x4 s[2], dp[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        s[y] = f32x4{0, 0, 0, 0};
+        dp[y] = *reinterpret_cast<const f32x4*>(delta + 16 * y + 4 * g);     // -delta: the sum becomes dP - delta
+    }
 #pragma unroll
     for (int x = 0; x < DP / 32; ++x)
 #pragma unroll
@@ -746,11 +798,11 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
         }
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(lse2 + 16 * y + 4 * g);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 16 * y + 4 * g);
+        const f32x4 rf = *reinterpret_cast<const f32x4*>(ref + 16 * y + 4 * g);
+        const f32x4 nm = *reinterpret_cast<const f32x4*>(norm + 16 * y + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i], c, -ls[i])), d = (dp[y][i] - de[i]) * dscale;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i] - rf[i], c, -nm[i])), d = dp[y][i] * dscale;
             if (!whole && (unsigned)(t0 + 16 * y + 4 * g + i - q_first) >= (unsigned)q_count) p = d = 0.0f;
             s[y][i] = p;
             dp[y][i] = p * d;
@@ -803,7 +855,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     extern __shared__ char smem[];
     T* qt = reinterpret_cast<T*>(smem);
     T* gt = qt + TILE;
-    float* st = reinterpret_cast<float*>(gt + TILE);         // [2][64]: lse2, delta
+    float* st = reinterpret_cast<float*>(gt + TILE);         // [4][64]: ref, norm, -delta twice (a branch costs 3 us)
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const unsigned id = win_block();
     const int k0 = (int)(id % a.ktiles) * 32, hk = (int)(id / a.ktiles % a.Hkv);
@@ -823,15 +875,16 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     qs.init((const T*)a.q + b * a.qs.b + hk * G * a.qs.h, a.qs.l, lo, hi, a.D, a.mode);
     gs.init((const T*)a.gout + ((int64_t)b * a.L * a.Hq + hk * G) * a.D, (int64_t)a.Hq * a.D, lo, hi, a.D, a.modeg);
     float stat = 0.0f;
+    const float* stats = wave == 0 ? a.ref : wave == 1 ? a.norm : a.delta;
     int h_next = 0, i_next = 0;                              // next tile: head of the group, place along the sequence
     auto load = [&]() {
         const int t0 = tq0 + i_next * R;
         qs.load(t0);
         gs.load(t0);
-        if (threadIdx.x < 2 * R) {
+        {
             const int qi = t0 + (int)(threadIdx.x & (R - 1));
             const int64_t row = ((int64_t)b * a.Hq + hk * G + h_next) * a.L + clamp_row(qi, lo, hi);
-            stat = threadIdx.x < R ? a.lse[row] * WA_LOG2E : a.delta[row];
+            stat = stats[row];
             if (qi < lo || qi >= hi) stat = 0.0f;
         }
         if (++i_next == nt) {
@@ -844,7 +897,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     auto store = [&]() {
         qs.store(qt);
         gs.store(gt);
-        if (threadIdx.x < 2 * R) st[threadIdx.x] = stat;
+        st[threadIdx.x] = stat;
     };
     if (total > 0) load();
     Oct<T> kf[DP / 32], vf[DP / 32];
@@ -861,7 +914,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         if (AHEAD && n + 1 < total) load();
         if (kw <= t0 + 31 && (t0 - (kw + 15) < a.W || kw < first_end) && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
-            dkdv_step<T, DP>(a, qt + half * LD, gt + half * LD, st + half, st + R + half, kf, vf, t0, ki, q_count, whole,
+            dkdv_step<T, DP>(a, qt + half * LD, gt + half * LD, st + half, st + R + half, st + 2 * R + half, kf, vf, t0, ki, q_count, whole,
                              a.scale * up, dk, dv);
         }
         __syncthreads();
@@ -936,7 +989,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     T* qt = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
     T* gt = qt + TILE;
-    float* st = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + NW * 2 * TILE) + wave * 64;
+    float* st = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + NW * 2 * TILE) + wave * 128;
     const int groups = (a.S + 15) / 16;
     int id = (int)blockIdx.x;
     const int grp = id % groups;
@@ -968,14 +1021,15 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         wave_stage<T, DP, FAST>(gt, gp, (int64_t)a.Hq * a.D, t0, lo, hi, a.D, a.modeg);
         {
             const int qi = t0 + (lane & 31);
-            const int64_t row = ((int64_t)b * a.Hq + h) * a.L + qi;
-            float x = 0.0f;
-            if (qi >= lo && qi < hi) x = lane < 32 ? a.lse[row] * WA_LOG2E : a.delta[row];
-            st[lane] = x;
+            const int64_t row = ((int64_t)b * a.Hq + h) * a.L + clamp_row(qi, lo, hi);
+            const bool in = qi >= lo && qi < hi;
+            const float x = (lane < 32 ? a.ref : a.norm)[row], y = a.delta[row];
+            st[lane] = in ? x : 0.0f;
+            st[64 + lane] = in ? y : 0.0f;                       // the upper half's copies are not read
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        dkdv_step<T, DP>(a, qt, gt, st, st + 32, kf, vf, t0, ki + a.W, q_count, false, a.scale * up, dk, dv);
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, st + 64, kf, vf, t0, ki + a.W, q_count, false, a.scale * up, dk, dv);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -1250,7 +1304,7 @@ static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
 template <class T, int DP, bool FAST>
 static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStream_t st) {
     const size_t tiles = (size_t)fwd_buffers<T, DP>() * 2 * WA_BK * lds_ld<T, DP>() * sizeof(T);
-    const size_t lds = 2 * 64 * lds_ld<T, DP>() * sizeof(T) + 128 * sizeof(float);
+    const size_t lds = 2 * 64 * lds_ld<T, DP>() * sizeof(T) + 256 * sizeof(float);
     int rc = win_lds(win_dq_kernel<T, DP, FAST>, tiles);
     if (rc != DR_OK) return rc;
     DR_LAUNCH_NAMED("win_dq_kernel", (win_dq_kernel<T, DP, FAST>), dim3((unsigned)a.tiles * a.Hq * a.B), dim3(256), tiles, st, a,
@@ -1258,7 +1312,7 @@ static int win_bwd_launch(const WinArgs& a, void* dq, void* dk, void* dv, hipStr
     DR_CHECK_LAUNCH("win_dq_kernel");
     if (a.chunks > 0) {
         constexpr int NW = sink_waves<T, DP>();
-        const size_t sl = (size_t)NW * (2 * WA_BK * lds_ld<T, DP>() * sizeof(T) + 64 * sizeof(float));
+        const size_t sl = (size_t)NW * (2 * WA_BK * lds_ld<T, DP>() * sizeof(T) + 128 * sizeof(float));
         rc = win_lds(win_sink_kernel<T, DP, FAST>, sl);
         if (rc != DR_OK) return rc;
         DR_LAUNCH_NAMED("win_sink_kernel", (win_sink_kernel<T, DP, FAST>), dim3((unsigned)((a.S + 15) / 16) * a.chunks * a.Hkv * a.B),
@@ -1357,7 +1411,7 @@ extern "C" int64_t dr_window_attn_backward_bytes(int64_t B, int64_t L, int32_t H
     using namespace dr;
     int rc = win_check("dr_window_attn_backward_bytes", B, L, Hq, Hkv, D, DR_F32, window, sinks, 1.0f);
     if (rc != DR_OK) return rc;
-    return align_up(B * Hq * L * 4, 256) + align_up(B * Hq * ((L + 63) / 64) * 16, 256) +
+    return 3 * align_up(B * Hq * L * 4, 256) + align_up(B * Hq * ((L + 63) / 64) * 16, 256) +
            align_up(B * Hkv * win_chunks(L, window, sinks, Hq / Hkv) * 2 * sinks * D * 4, 256) + 256;
 }
 
@@ -1400,7 +1454,10 @@ extern "C" int32_t dr_window_attn_backward(const void* q, const int64_t* q_strid
     a.end = end;
     a.lse = const_cast<float*>(lse);
     a.delta = (float*)ws;
-    a.gmax = (float*)((char*)ws + align_up(B * Hq * L * 4, 256));
+    const int64_t per_query = align_up(B * Hq * L * 4, 256);
+    a.ref = (float*)((char*)ws + per_query);
+    a.norm = (float*)((char*)ws + 2 * per_query);
+    a.gmax = (float*)((char*)ws + 3 * per_query);
     a.part = (float*)((char*)a.gmax + align_up(B * Hq * ((L + 63) / 64) * 16, 256));
     a.chunks = (int)win_chunks(L, window, sinks, Hq / Hkv);
     a.here = sinks > 0 && a.chunks == 0;

@@ -65,3 +65,81 @@ def test_forward_at_large_scores(dev, shape, dt, scale, unit):
     tok = Kn.window_attn_token(q[rows, last.clamp_min(0)].to(dev), k.to(dev), v.to(dev), W, S, scale, begin.to(dev), end.to(dev))
     want = torch.where(some[:, None, None], r["out"][rows, last.clamp_min(0)], torch.zeros((), dtype=torch.float64))
     _within("token", tok, want, torch.where(some[:, None, None], lim[rows, last.clamp_min(0)], torch.full((), 1e-30, dtype=torch.float64)))
+
+
+def _limits(r, vis, dt, D, G, scale, e16, eP):
+    """Bounds of out, dq, dk, dv [in the outputs' layout].  P enters its product with a relative error eP beside _relp's, dS with
+    e16.  delta is as exact as P: <dO, O> with O in fp32, or from the rounded O (delta_0) and corrected by
+    r = sum p (dP - delta_0), which is off by p's errors on |dP - delta_0| and fp32 sums; r P K, taken off dQ at the end, has P
+    rounded once to a 16-bit type (e).  With |x|_1 the absolute sum of a dot product's terms:
+      |ddS| <= p scale [(relp + e16) |dP - delta| + (2 D + 8) u (|dO v|_1 + |delta|) + err delta]
+    (the D terms of dP are added to -delta: no partial sum exceeds |dO v|_1 + |delta|), and fp32 sums of m terms add
+    (m / 8 + 8) u of their absolute sum."""
+    e = torch.finfo(dt).eps / 2
+    p, relp = r["p"], _relp(r, vis)
+    absV, absK, absGO = r["V"].abs(), r["K"].abs(), r["GO"].abs()
+    t = lambda x: x.transpose(2, 3)
+    out = (p * (relp + eP)) @ absV
+    dot = absGO @ t(absV) + r["delta"].abs()
+    diff = (r["dp"] - r["delta"]).abs()
+    err0 = (absGO * (out + e * r["o"].abs())).sum(-1, keepdim=True)          # delta_0 - delta: O off by its rounding
+    err = (p * (relp * (diff + err0) + (2 * D + 8) * U * dot)).sum(-1, keepdim=True) + (r["n"] / 8 + 8) * U * (p * (diff + err0)).sum(-1, keepdim=True)
+    if dt == torch.float32:
+        err = err0 + (2 * D + 8) * U * (absGO * r["o"].abs()).sum(-1, keepdim=True)
+    dS = p * scale * ((relp + e16) * (diff + (err0 if e16 else 0.0)) + (2 * D + 8) * U * dot + err)
+    absS = p * scale * (diff + err0)
+    dq = dS @ absK + (r["n"] / 8 + 8) * U * (absS @ absK) + (scale * e * err0 * (p @ absK) if dt != torch.float32 else 0.0)
+    dk = t(dS) @ r["Q"].abs() + (r["nk"] * G / 8 + 8) * U * (t(absS) @ r["Q"].abs())
+    dv = t(p * (relp + eP)) @ absGO + (r["nk"] * G / 8 + 8) * U * (t(p) @ absGO)
+    fin = lambda lim, ref: lim * (1 + e) + e * ref.abs() + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2 + 1e-30
+    return (fin(out.permute(0, 2, 1, 3), r["out"]), fin(dq.permute(0, 2, 1, 3), r["dq"]), fin(r["group"](dk), r["dk"]),
+            fin(r["group"](dv), r["dv"]))
+
+
+def _check(dev, q, k, v, go, W, S, scale, begin, end, limits):
+    from deeprec_amd import kernels as Kn
+    d = lambda t: t.to(dev)
+    mask = dict(window=W, sinks=S, scale=scale, begin=d(begin), end=d(end))
+    out, lse = Kn.window_attn_forward(d(q), d(k), d(v), **mask)
+    grads = Kn.window_attn_backward(d(q), d(k), d(v), out, lse, d(go), **mask)
+    B, L, Hq, D = q.shape
+    vis = _visible(B, L, W, S, begin, end)
+    r = _ref(q, k, v, go, vis, scale)
+    lims = limits(r, vis)
+    for name, x, lim in zip(("out", "dq", "dk", "dv"), (out,) + grads, lims):
+        _within(name, x, r[name], lim)
+    return out, lse, grads
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 150, 4, 2, 64, 40, 3), (2, 400, 2, 1, 50, 40, 3), (3, 90, 2, 2, 150, 90, 0)])
+@pytest.mark.parametrize("shift", [0, 256, -256, 2048, -2048])
+def test_backward_far_from_zero(dev, shape, shift):
+    """Scores of about shift^2 / 8 (8192, 524288) that differ by a few: P has fp32's digits all the same, in every product."""
+    B, L, Hq, Hkv, D, W, S = shape
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, torch.float32, 1.0, 2, L + D)
+    q[..., 0], k[..., 0] = float(shift), float(abs(shift))
+    _check(dev, q, k, v, go, W, S, 0.125, begin, end, lambda r, vis: _limits(r, vis, torch.float32, D, Hq // Hkv, 0.125, 0.0, 0.0))
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("scale", [2.0 ** 33, 2.0 ** 99])
+def test_backward_at_large_scores(dev, dt, scale):
+    """One key, or several with equal scores, carries a row: dV is the sum of dO over the rows that chose it, dQ and dK stay
+    within the rounding of dP - delta times scale (fp16 cannot hold that: its dQ and dK are not compared)."""
+    from deeprec_amd import kernels as Kn
+    B, L, Hq, Hkv, D, W, S = 3, 150, 4, 2, 64, 40, 3
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, dt, 1.0, 4, 7)
+    d = lambda t: t.to(dev)
+    mask = dict(window=W, sinks=S, scale=scale, begin=d(begin), end=d(end))
+    out, lse = Kn.window_attn_forward(d(q), d(k), d(v), **mask)
+    dq, dk, dv = Kn.window_attn_backward(d(q), d(k), d(v), out, lse, d(go), **mask)
+    vis = _visible(B, L, W, S, begin, end)
+    r = _ref(q, k, v, go, vis, scale)
+    e = torch.finfo(dt).eps / 2
+    lim = _limits(r, vis, dt, D, Hq // Hkv, scale, e, 0.0 if dt == torch.float32 else e)
+    _within("dv", dv, r["dv"], lim[3])
+    if dt != torch.float16:
+        _within("dq", dq, r["dq"], lim[1])
+        _within("dk", dk, r["dk"], lim[2])
