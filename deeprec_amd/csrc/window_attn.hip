@@ -778,7 +778,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 template <class T, int DP>
 __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T* gc, const float* ref, const float* norm, const float* delta,
                                           const Oct<T> (&kf)[DP / 32], const Oct<T> (&vf)[DP / 32], int t0, int q_first,
-                                          int q_count, bool whole, float dscale, f32x4 (&dk)[DP / 16],
+                                          int q_count, bool whole, float up, f32x4 (&dk)[DP / 16],
                                           f32x4 (&dv)[DP / 16]) {
     constexpr int LD = lds_ld<T, DP>();
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
@@ -802,7 +802,7 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
         const f32x4 nm = *reinterpret_cast<const f32x4*>(norm + 16 * y + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i] - rf[i], c, -nm[i])), d = dp[y][i] * dscale;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i] - rf[i], c, -nm[i])), d = dp[y][i] * up;
             if (!whole && (unsigned)(t0 + 16 * y + 4 * g + i - q_first) >= (unsigned)q_count) p = d = 0.0f;
             s[y][i] = p;
             dp[y][i] = p * d;
@@ -915,15 +915,16 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         if (kw <= t0 + 31 && (t0 - (kw + 15) < a.W || kw < first_end) && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
             dkdv_step<T, DP>(a, qt + half * LD, gt + half * LD, st + half, st + R + half, st + 2 * R + half, kf, vf, t0, ki, q_count, whole,
-                             a.scale * up, dk, dv);
+                             up, dk, dv);
         }
         __syncthreads();
         if (!AHEAD && n + 1 < total) load();
         if (n + 1 < total) store();
         __syncthreads();
     }
-    // the second query half's sums join the first's over LDS: [key half][2][16][DP] fp32, which the tiles have room for
-    const float down = 1.0f / up;
+    // the second query half's sums join the first's over LDS: [key half][2][16][DP] fp32, which the tiles have room for.
+    // dK gets its scale here, in fp32: before, it could carry dS out of fp16's range
+    const float down = a.scale / up;
     float* red = reinterpret_cast<float*>(smem) + (wave & 1) * 32 * DP;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
@@ -932,7 +933,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] : dk[t][i];
+                    red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] : dk[t][i] * down;
         }
     __syncthreads();
     const int far = a.chunks > 0 && klo <= khi && k0 < lo + a.S ? (lo + a.S < khi + 1 ? lo + a.S : khi + 1) - klo : 0;
@@ -950,7 +951,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 #pragma unroll
                 for (int q = 0; q < 16; ++q) x += q0 + q < a.chunks ? v[q] : 0.0f;
             }
-            reinterpret_cast<float*>(smem)[(key >> 4) * 32 * DP + which * 16 * DP + (key & 15) * DP + d] += which ? x : x * up;
+            reinterpret_cast<float*>(smem)[(key >> 4) * 32 * DP + which * 16 * DP + (key & 15) * DP + d] += x;
         }
         __syncthreads();
     }
@@ -966,7 +967,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         for (int t = 0; t < DP / 16; ++t) {
             const int d = 16 * t + c16;
             if (!FAST && d >= a.D) continue;
-            const float x = (dk[t][i] + red[(4 * g + i) * DP + d]) * down, y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
+            const float x = fmaf(dk[t][i], down, red[(4 * g + i) * DP + d]), y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
             ko[d] = (T)x;
             vo[d] = (T)y;
         }
@@ -1010,7 +1011,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
     const int first = chunk * WA_CHUNK, per = WA_CHUNK / WA_BK;
     const float up = grad_scale<T>(a, b, hk * G, G, first, first + WA_CHUNK <= a.L ? first + WA_CHUNK - 1 : a.L - 1);
-    const float down = 1.0f / up;
+    const float down = a.scale / up;
     for (int n = wave; n < per * G; n += NW) {
         const int h = hk * G + n / per, t0 = first + n % per * WA_BK;
         // wavefront-uniform: no query of the tile is both in the history and beyond the window of the group's first key
@@ -1029,7 +1030,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        dkdv_step<T, DP>(a, qt, gt, st, st + 32, st + 64, kf, vf, t0, ki + a.W, q_count, false, a.scale * up, dk, dv);
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, st + 64, kf, vf, t0, ki + a.W, q_count, false, up, dk, dv);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }

@@ -143,3 +143,15 @@ def test_backward_at_large_scores(dev, dt, scale):
     if dt != torch.float16:
         _within("dq", dq, r["dq"], lim[1])
         _within("dk", dk, r["dk"], lim[2])
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 150, 4, 2, 64, 40, 3), (1, 700, 2, 1, 64, 100, 33)])
+@pytest.mark.parametrize("scale,unit", [(2.0 ** -13, 8.0), (2.0 ** -19, 64.0), (2.0 ** 13, 2.0 ** -9)])
+def test_fp16_gradients_at_any_scale(dev, shape, scale, unit):
+    """A scale far from D^-0.5 with queries and keys that make up for it: dS is an ordinary number before the scale, which must
+    not meet it in fp16.  The second shape's first items get their far gradients from a launch of their own."""
+    B, L, Hq, Hkv, D, W, S = shape
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, torch.float16, unit, 4, 17)
+    e = 2.0 ** -11
+    _check(dev, q, k, v, go, W, S, scale, begin, end, lambda r, vis: _limits(r, vis, torch.float16, D, Hq // Hkv, scale, e, e))
