@@ -187,7 +187,7 @@ struct WinArgs {
     int wide;                  // rows of out, dq take stores of four elements
     float *lse;                // [B, Hq, L]
     float *delta, *ref, *norm; // [B, Hq, L]: -delta; p = exp2((s - ref) c - norm), see win_dq_kernel
-    float* gmax;               // fp16: largest |dO| of every 16 queries [B, Hq, 4 tiles]
+    float* gmax;               // fp16: largest |dS| (before the scale) of every 16 queries [B, Hq, 4 tiles]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
     int chunks;                // far sinks: workgroups along the sequence; 0: none
     int here;                  // far sinks: taken by win_dkdv_kernel itself
@@ -561,10 +561,12 @@ __device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>
     }
     lo = to_oct<T>(x, y);
 }
-// power of two that brings x into [1, 2); 1 for 0 and what is not finite
+// fp16 holds dS of no gradient, value or scale by itself: it is multiplied by a power of two that brings the largest |dS| to
+// [2^13, 2^14), so that nothing overflows and the two halves keep 2^-38 of the largest.  Here that power, at most 2^100
+// (dS = 0); 1 for what is not finite.
 __device__ __forceinline__ float grad_up(float x) {
     const int e = (int)((__float_as_uint(x) >> 23) & 255u);
-    return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t)(254 - e) << 23);
+    return e == 255 ? 1.0f : __uint_as_float((uint32_t)(e > 40 ? 267 - e : 227) << 23);
 }
 template <class T, int DP, bool FAST>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_dq_kernel(WinArgs a, T* __restrict__ dq) {
@@ -616,19 +618,18 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int e = 0; e < 8; ++e) delta = fmaf((float)gf[s][e], (float)of[s][e], delta);
         delta = groups_sum(delta);
     }
-    // fp16 has no range for dS of every gradient scale: the rows are brought to dO of about 1 first
-    float up = 1.0f, down = 1.0f;
-    if constexpr (std::is_same<T, f16>::value) {
-        float big = 0.0f;
+    // fp16: the power of two starts from a guess (|dP| of about 8 |dO|) and follows the query's largest |dS| down as the tiles
+    // come, as the forward's maximum goes up: no |dS| up beyond 2^15
+    constexpr bool RANGE = std::is_same<T, f16>::value;
+    float up = 1.0f, most = 0.0f, big = 0.0f;
+    if constexpr (RANGE) {
+        float x = 0.0f;
 #pragma unroll
         for (int s = 0; s < DP / 32; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf((float)gf[s][e]));
-        big = groups_max(big);
-        up = grad_up(big);
-        down = 1.0f / up;
-        for (int off = 8; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
-        if (lane == 0) a.gmax[(((int64_t)b * a.Hq + h) * a.tiles + q0 / 64) * 4 + wave] = big;   // of these 16 queries
+            for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf((float)gf[s][e]));
+        up = grad_up(8.0f * groups_max(x));
+        most = 32768.0f / up;
     }
     f32x4 acc[DP / 16], pk[FIX ? DP / 16 : 1];                               // sums of p (dP - delta) K and of p K
 #pragma unroll
@@ -710,9 +711,27 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     l += s[y][i];
-                    s[y][i] *= dp[y][i] * up;
+                    s[y][i] *= dp[y][i];
                     fix += s[y][i];
                 }
+            if constexpr (RANGE) {
+                float t = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t = fmaxf(t, fabsf(s[y][i]));
+                big = fmaxf(big, t);
+                if (__ballot(t > most) != 0) {
+                    t = groups_max(t);
+                    const float next = t > most ? grad_up(t) : up, f = next / up;
+                    up = next;
+                    most = 32768.0f / up;
+#pragma unroll
+                    for (int x = 0; x < DP / 16; ++x) acc[x] *= f;
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) s[y] *= up;
+            }
             if constexpr (FIX) {
                 Oct<T> dh, dl;
                 split_oct<T>(s[0], s[1], dh, dl);
@@ -740,11 +759,19 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;                           // a NaN stays one
     if constexpr (FIX) {
         fix = groups_sum(fix) * inv;
-        delta += fix * down;
+        delta += fix;
+        const float f = -fix * up;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(-fix, pk[t][i], acc[t][i]);
+            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(f, pk[t][i], acc[t][i]);
+    }
+    if constexpr (RANGE) {
+        // no |dS| of these 16 queries is larger: p (dP - delta) = p (dP - delta_0) - p fix
+        big = groups_max(big) * inv + fabsf(fix);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
+        if (lane == 0) a.gmax[(((int64_t)b * a.Hq + h) * a.tiles + q0 / 64) * 4 + wave] = big;
     }
     if (qi >= a.L) return;
     if (g == 0) {
@@ -752,7 +779,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         a.ref[srow + qi] = ref;
         a.norm[srow + qi] = l == 0.0f ? 0.0f : log2f(l);
     }
-    down *= inv * a.scale;
+    const float down = inv * a.scale / up;
     T* op = dq + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
@@ -802,10 +829,10 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
         const f32x4 nm = *reinterpret_cast<const f32x4*>(norm + 16 * y + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i] - rf[i], c, -nm[i])), d = dp[y][i] * up;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[y][i] - rf[i], c, -nm[i])), d = dp[y][i];
             if (!whole && (unsigned)(t0 + 16 * y + 4 * g + i - q_first) >= (unsigned)q_count) p = d = 0.0f;
             s[y][i] = p;
-            dp[y][i] = p * d;
+            dp[y][i] = p * d * up;                               // in this order: only p d is known to be in range
         }
     }
     const Oct<T> pf = to_oct<T>(s[0], s[1]);
@@ -829,18 +856,38 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
     }
 }
 
-// The factor that brings the gradients of the queries [q0, q1] of a group's heads to about 1 (fp16; see win_dq_kernel)
+// The power of two for dS of the queries [q0, q1] of a group's heads (fp16: grad_up of the largest |dS| that win_dq_kernel met;
+// queries whose dS is not finite make NaN what they see, whatever it is)
+// In two steps, with loads of the caller's own between them: first() requests a lane's first value, scale() the rest and
+// gives the answer.
 template <class T>
-__device__ __forceinline__ float grad_scale(const WinArgs& a, int b, int h0, int heads, int q0, int q1) {
-    if constexpr (!std::is_same<T, f16>::value) return 1.0f;
-    float big = 0.0f;
-    const int r0 = q0 / 16, n = q1 / 16 - r0 + 1;
-    for (int i = threadIdx.x & 63; i < n * heads; i += 64)
-        big = fmaxf(big, a.gmax[((int64_t)b * a.Hq + h0 + i / n) * a.tiles * 4 + r0 + i % n]);
+struct GradScale {
+    const float* rows;                                       // [heads, 4 tiles] of the group
+    int r0, n, total, tiles;
+    float x;
+    __device__ __forceinline__ float at(int i) const { return rows[(int64_t)(i / n) * tiles * 4 + r0 + i % n]; }
+    __device__ __forceinline__ void first(const WinArgs& a, int b, int h0, int heads, int q0, int q1) {
+        if constexpr (!std::is_same<T, f16>::value) return;
+        rows = a.gmax + ((int64_t)b * a.Hq + h0) * a.tiles * 4;
+        tiles = a.tiles;
+        r0 = q0 / 16;
+        n = q1 / 16 - r0 + 1;
+        total = n * heads;
+        const int i = threadIdx.x & 63;
+        x = at(i < total ? i : 0);
+    }
+    __device__ __forceinline__ float scale() const {
+        if constexpr (!std::is_same<T, f16>::value) return 1.0f;
+        float big = x < __builtin_inff() ? x : 0.0f;
+        for (int i = (int)(threadIdx.x & 63) + 64; i < total; i += 64) {
+            const float y = at(i);
+            big = fmaxf(big, y < __builtin_inff() ? y : 0.0f);
+        }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
-    return grad_up(big);
-}
+        for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off, 64));
+        return grad_up(big);
+    }
+};
 // A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
 // head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
 // of the queries are added up at the end.  What the first items get from queries beyond the window is found here too
@@ -870,7 +917,6 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     const int klo = k0 > lo ? k0 : lo, khi = k0 + 31 < hi - 1 ? k0 + 31 : hi - 1;
     const int qend = klo > khi ? -1 : (klo >= first_end && khi + (int64_t)a.W - 1 < hi - 1 ? khi + a.W - 1 : hi - 1);
     const int tq0 = klo / 32 * 32, nt = klo <= khi ? (qend - tq0) / R + 1 : 0, total = nt * G;
-    const float up = total > 0 ? grad_scale<T>(a, b, hk * G, G, tq0, qend) : 1.0f;
     Stage<T, DP, R, FAST> qs, gs;
     qs.init((const T*)a.q + b * a.qs.b + hk * G * a.qs.h, a.qs.l, lo, hi, a.D, a.mode);
     gs.init((const T*)a.gout + ((int64_t)b * a.L * a.Hq + hk * G) * a.D, (int64_t)a.Hq * a.D, lo, hi, a.D, a.modeg);
@@ -899,13 +945,18 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         gs.store(gt);
         st[threadIdx.x] = stat;
     };
-    if (total > 0) load();
+    GradScale<T> ds_up;
+    if (total > 0) {
+        ds_up.first(a, b, hk * G, G, tq0, qend);
+        load();
+    }
     Oct<T> kf[DP / 32], vf[DP / 32];
     load_frags<T, DP, FAST>(kf, (const T*)a.k + b * a.ks.b + (int64_t)clamp_row(ki, lo, hi) * a.ks.l + hk * a.ks.h, k_ok, a.D, a.mode);
     load_frags<T, DP, FAST>(vf, (const T*)a.v + b * a.vs.b + (int64_t)clamp_row(ki, lo, hi) * a.vs.l + hk * a.vs.h, k_ok, a.D, a.mode);
     f32x4 dk[DP / 16], dv[DP / 16];
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
+    const float up = total > 0 ? ds_up.scale() : 1.0f;
     if (total > 0) store();
     __syncthreads();
     for (int n = 0, i = 0; n < total; ++n) {
@@ -1010,7 +1061,9 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0, 0, 0, 0};
     const int first = chunk * WA_CHUNK, per = WA_CHUNK / WA_BK;
-    const float up = grad_scale<T>(a, b, hk * G, G, first, first + WA_CHUNK <= a.L ? first + WA_CHUNK - 1 : a.L - 1);
+    GradScale<T> ds_up;
+    ds_up.first(a, b, hk * G, G, first, first + WA_CHUNK <= a.L ? first + WA_CHUNK - 1 : a.L - 1);
+    const float up = ds_up.scale();
     const float down = a.scale / up;
     for (int n = wave; n < per * G; n += NW) {
         const int h = hk * G + n / per, t0 = first + n % per * WA_BK;

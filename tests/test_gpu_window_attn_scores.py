@@ -155,3 +155,20 @@ def test_fp16_gradients_at_any_scale(dev, shape, scale, unit):
     q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, torch.float16, unit, 4, 17)
     e = 2.0 ** -11
     _check(dev, q, k, v, go, W, S, scale, begin, end, lambda r, vis: _limits(r, vis, torch.float16, D, Hq // Hkv, scale, e, e))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 150, 4, 2, 64, 40, 3), (1, 700, 2, 1, 64, 100, 33), (2, 90, 2, 1, 80, 90, 0)])
+@pytest.mark.parametrize("size", [4096.0])
+def test_fp16_values_of_any_size(dev, shape, size):
+    """Values that line up with dO: |dP| = D size, 262144, where dQ and dK are ordinary fp16 numbers."""
+    B, L, Hq, Hkv, D, W, S = shape
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, torch.float16, 2.0 ** -4 if size > 1 else 4.0, 4, 23)
+    g = torch.Generator().manual_seed(5)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g).double() * 2 - 1
+    pattern = sign(D)
+    v = (sign(B, L, Hkv, 1) * pattern * size).half()
+    go = (pattern.expand(B, L, Hq, D) * 1.0).half()
+    scale = 0.125 if size > 1 else 2.0 ** -6
+    e = 2.0 ** -11
+    _check(dev, q, k, v, go, W, S, scale, begin, end, lambda r, vis: _limits(r, vis, torch.float16, D, Hq // Hkv, scale, e, e))
