@@ -41,6 +41,23 @@ __device__ __forceinline__ f32x4 mma(const Oct<float>& a, const Oct<float>& b, f
     return c;
 }
 
+// Probabilities go into their products times 2^p_bits, undone in fp32: without, fp16 loses what lies below 2^-14 and drops what
+// lies below 2^-25, and with it the whole gradient of keys that no query weighs strongly.  (The 15 is added to the exponent:
+// its last bit there costs p 2^-21 ln 2, five units of fp32's rounding.)
+template <class T>
+constexpr float p_bits() {
+    return std::is_same<T, f16>::value ? 15.0f : 0.0f;
+}
+template <class T>
+constexpr float p_down() {
+    return std::is_same<T, f16>::value ? 0x1p-15f : 1.0f;
+}
+// 2^x of a weight that goes into a product
+template <class T>
+__device__ __forceinline__ float weight(float d, float c) {
+    return __builtin_amdgcn_exp2f(p_bits<T>() == 0.0f ? d * c : fmaf(d, c, p_bits<T>()));
+}
+
 // LDS row length: rows of a 16-lane read start 4 banks apart
 template <class T, int DP>
 constexpr int lds_ld() {
@@ -186,7 +203,7 @@ struct WinArgs {
     int mode, modeg;           // how rows of q, k, v / of out, gout are read
     int wide;                  // rows of out, dq take stores of four elements
     float *lse;                // [B, Hq, L]
-    float *delta, *ref, *norm; // [B, Hq, L]: -delta; p = exp2((s - ref) c - norm), see win_dq_kernel
+    float *delta, *ref, *norm; // [B, Hq, L]: -delta; p 2^p_bits = exp2((s - ref) c - norm), see win_dq_kernel
     float* gmax;               // fp16: largest |dS| (before the scale) of every 16 queries [B, Hq, 4 tiles]
     float* part;               // far sinks: [B, Hkv, chunks, 2, S, D]
     int chunks;                // far sinks: workgroups along the sequence; 0: none
@@ -489,7 +506,7 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[y][x][i] = __builtin_amdgcn_exp2f((s[y][x][i] - ms) * c);
+                        s[y][x][i] = weight<T>(s[y][x][i] - ms, c);
                         sum += s[y][x][i];
                     }
                 l[y] = fmaf(l[y], alpha, sum);
@@ -532,7 +549,7 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
                     if (d + i < a.D) op[d + i] = (T)(o[y][t][i] * inv);
             }
         }
-        if (g == 0) lse[((int64_t)b * a.Hq + h + y) * a.L + qi] = l[y] == 0.0f ? -__builtin_inff() : fmaf(m[y], a.scale, log2f(l[y]) * WA_LN2);
+        if (g == 0) lse[((int64_t)b * a.Hq + h + y) * a.L + qi] = l[y] == 0.0f ? -__builtin_inff() : fmaf(m[y], a.scale, (log2f(l[y]) - p_bits<T>()) * WA_LN2);
     }
 }
 
@@ -628,7 +645,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         for (int s = 0; s < DP / 32; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf((float)gf[s][e]));
-        up = grad_up(8.0f * groups_max(x));
+        up = grad_up(8.0f / p_down<T>() * groups_max(x));
         most = 32768.0f / up;
     }
     f32x4 acc[DP / 16], pk[FIX ? DP / 16 : 1];                               // sums of p (dP - delta) K and of p K
@@ -694,7 +711,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[y][i] = __builtin_amdgcn_exp2f((s[y][i] - ref) * c);
+                for (int i = 0; i < 4; ++i) s[y][i] = weight<T>(s[y][i] - ref, c);
             if (!whole) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
@@ -777,7 +794,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
     if (g == 0) {
         a.delta[srow + qi] = -delta;
         a.ref[srow + qi] = ref;
-        a.norm[srow + qi] = l == 0.0f ? 0.0f : log2f(l);
+        a.norm[srow + qi] = l == 0.0f ? 0.0f : log2f(l * p_down<T>()) - p_bits<T>();
     }
     const float down = inv * a.scale / up;
     T* op = dq + (((int64_t)b * a.L + qi) * a.Hq + h) * a.D;
@@ -966,7 +983,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         if (kw <= t0 + 31 && (t0 - (kw + 15) < a.W || kw < first_end) && t0 < hi && kw < hi && kw + 15 >= lo) {
             const bool whole = kw >= lo && kw + 15 <= t0 && t0 + 31 < hi && t0 + 31 - kw < a.W;
             dkdv_step<T, DP>(a, qt + half * LD, gt + half * LD, st + half, st + R + half, st + 2 * R + half, kf, vf, t0, ki, q_count, whole,
-                             up, dk, dv);
+                             up * p_down<T>(), dk, dv);
         }
         __syncthreads();
         if (!AHEAD && n + 1 < total) load();
@@ -984,7 +1001,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
             for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] : dk[t][i] * down;
+                    red[which * 16 * DP + (4 * g + i) * DP + 16 * t + c16] = which ? dv[t][i] * p_down<T>() : dk[t][i] * down;
         }
     __syncthreads();
     const int far = a.chunks > 0 && klo <= khi && k0 < lo + a.S ? (lo + a.S < khi + 1 ? lo + a.S : khi + 1) - klo : 0;
@@ -1018,7 +1035,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
         for (int t = 0; t < DP / 16; ++t) {
             const int d = 16 * t + c16;
             if (!FAST && d >= a.D) continue;
-            const float x = fmaf(dk[t][i], down, red[(4 * g + i) * DP + d]), y = dv[t][i] + red[16 * DP + (4 * g + i) * DP + d];
+            const float x = fmaf(dk[t][i], down, red[(4 * g + i) * DP + d]);
+            const float y = fmaf(dv[t][i], p_down<T>(), red[16 * DP + (4 * g + i) * DP + d]);
             ko[d] = (T)x;
             vo[d] = (T)y;
         }
@@ -1083,7 +1101,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        dkdv_step<T, DP>(a, qt, gt, st, st + 32, st + 64, kf, vf, t0, ki + a.W, q_count, false, up, dk, dv);
+        dkdv_step<T, DP>(a, qt, gt, st, st + 32, st + 64, kf, vf, t0, ki + a.W, q_count, false, up * p_down<T>(), dk, dv);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -1101,7 +1119,7 @@ __global__ __launch_bounds__(256) void win_sink_kernel(WinArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float* r = red + (4 * g + i) * DP + 16 * t + c16;
-                        const float x = which ? dv[t][i] : dk[t][i] * down;
+                        const float x = which ? dv[t][i] * p_down<T>() : dk[t][i] * down;
                         *r = w == 0 ? x : *r + x;
                     }
             }
@@ -1201,7 +1219,7 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
         for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[y][i] = __builtin_amdgcn_exp2f((s[y][i] - ms) * c);
+                s[y][i] = weight<T>(s[y][i] - ms, c);
                 sum += s[y][i];
             }
         l = fmaf(l, alpha, sum);

@@ -172,3 +172,26 @@ def test_fp16_values_of_any_size(dev, shape, size):
     scale = 0.125 if size > 1 else 2.0 ** -6
     e = 2.0 ** -11
     _check(dev, q, k, v, go, W, S, scale, begin, end, lambda r, vis: _limits(r, vis, torch.float16, D, Hq // Hkv, scale, e, e))
+
+
+@gpu
+@pytest.mark.parametrize("W,S", [(1000, 0), (250, 20)])
+def test_fp16_small_probabilities(dev, W, S):
+    """A sharp softmax with a loss scale: keys that no query weighs strongly still get their gradient, key by key.
+    P goes into its products times 2^15, its last bit 2^-24 2^-15: half of it is 2^-40.  dS goes in as two halves, its largest
+    brought to 2^13 or more: 2^-25 / 2^13 = 2^-38 of the largest |dS|."""
+    L, D, dt = 1000, 64, torch.float16
+    q, k, v, go, begin, end = _integers(1, L, 2, 1, D, dt, 1.0, 7, 29)
+    go = (go.float() * 256).half()
+    e = 2.0 ** -11
+
+    def limits(r, vis):
+        out, dq, dk, dv = _limits(r, vis, dt, D, 2, 0.125, e * e, e)
+        seen = vis[:, None].double()
+        big = (r["p"] * (r["dp"] - r["delta"])).abs().amax()
+        dv = dv + r["group"](2.0 ** -40 * seen.transpose(2, 3) @ r["GO"].abs())
+        dk = dk + r["group"](2.0 ** -38 * big * 0.125 * seen.transpose(2, 3) @ r["Q"].abs())
+        dq = dq + (2.0 ** -38 * big * 0.125 * seen @ r["K"].abs()).permute(0, 2, 1, 3)
+        out = out + (2.0 ** -40 * seen @ r["V"].abs()).permute(0, 2, 1, 3)
+        return out, dq, dk, dv
+    _check(dev, q, k, v, go, W, S, 0.125, begin, end, limits)
