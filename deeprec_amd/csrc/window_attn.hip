@@ -10,8 +10,10 @@
 // the order of a sum is free as long as A uses the same one, and A = V^T is read from LDS by that rule (two transposing
 // 8-byte reads for 16-bit types, eight 4-byte reads for fp32).  Running maximum and sum are one scalar per lane.
 // fp32 runs the same code: a 16x16x32 step is eight v_mfma_f32_16x16x4_f32, element e of every lane's eight in step e.
-// Scores, statistics and sums are fp32; P and dS are rounded to the storage type for the second product, as its operands
-// are (fp32: not at all).
+// Scores, statistics and sums are fp32.  The second product's operands are of the storage type; P and dS, of 16-bit types, go
+// in as two halves (hi + what hi misses): rounded once, P alone put as much error into out and dV as their own rounding, and
+// where terms cancel far more.  The second half costs 9 % of the forward at D = 128 (28.5 -> 30.6 us at 4 x 2047 x 8 / 2 heads,
+// window 256), 20 % at D = 64 on a large grid, 3 % of dK / dV, nothing for one token.
 #include <initializer_list>
 #include <type_traits>
 
@@ -178,6 +180,18 @@ __device__ __forceinline__ Oct<T> to_oct(const f32x4& a, const f32x4& b) {
     return r;
 }
 
+// 16-bit operands in two halves: the rounded value and what it misses, e^2 left of it (e: half a step)
+template <class T>
+__device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>& hi, Oct<T>& lo) {
+    hi = to_oct<T>(a, b);
+    f32x4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = a[e] - (float)hi[e];
+        y[e] = b[e] - (float)hi[4 + e];
+    }
+    lo = to_oct<T>(x, y);
+}
 // over the four lane groups that share a query: every lane gets the maximum / the sum
 __device__ __forceinline__ float groups_max(float x) {
     const int lane = threadIdx.x & 63;
@@ -487,7 +501,7 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
                         }
                 }
             }
-            Oct<T> p[NH];
+            Oct<T> p[NH], pl[NH];                              // 16-bit types: the halves of P
 #pragma unroll
             for (int y = 0; y < NH; ++y) {
                 float mt = s[y][0][0];
@@ -514,13 +528,19 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
 #pragma unroll
                     for (int t = 0; t < DP / 16; ++t) o[y][t] *= alpha;
                 }
-                p[y] = to_oct<T>(s[y][0], s[y][1]);
+                if constexpr (sizeof(T) == 2)
+                    split_oct<T>(s[y][0], s[y][1], p[y], pl[y]);
+                else
+                    p[y] = to_oct<T>(s[y][0], s[y][1]);
             }
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
                 const Oct<T> vf = col_frag<T, LD>(vc, 16 * t);
 #pragma unroll
-                for (int y = 0; y < NH; ++y) o[y][t] = mma(vf, p[y], o[y][t]);
+                for (int y = 0; y < NH; ++y) {
+                    o[y][t] = mma(vf, p[y], o[y][t]);
+                    if constexpr (sizeof(T) == 2) o[y][t] = mma(vf, pl[y], o[y][t]);
+                }
             }
         }
         if (NB == 1) __syncthreads();
@@ -567,17 +587,6 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
 // l in the end and hands ref and norm = log2 l to the others.  Where |lse| reaches WA_FAR its rounding (half a unit of log 2 at
 // 2^23) could carry the weights out of range: there the workgroup takes the maximum itself in a first run over the keys.
 constexpr float WA_FAR = 65536.0f;
-template <class T>
-__device__ __forceinline__ void split_oct(const f32x4& a, const f32x4& b, Oct<T>& hi, Oct<T>& lo) {
-    hi = to_oct<T>(a, b);
-    f32x4 x, y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[e] = a[e] - (float)hi[e];
-        y[e] = b[e] - (float)hi[4 + e];
-    }
-    lo = to_oct<T>(x, y);
-}
 // fp16 holds dS of no gradient, value or scale by itself: it is multiplied by a power of two that brings the largest |dS| to
 // [2^13, 2^14), so that nothing overflows and the two halves keep 2^-38 of the largest.  Here that power, at most 2^100
 // (dS = 0); 1 for what is not finite.
@@ -852,19 +861,21 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
             dp[y][i] = p * d * up;                               // in this order: only p d is known to be in range
         }
     }
-    const Oct<T> pf = to_oct<T>(s[0], s[1]);
     if constexpr (sizeof(T) == 2) {
-        Oct<T> dh, dl;
+        Oct<T> ph, pl, dh, dl;
+        split_oct<T>(s[0], s[1], ph, pl);
         split_oct<T>(dp[0], dp[1], dh, dl);
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
-            dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
+            const Oct<T> gf = col_frag<T, LD>(gc, 16 * t);
+            dv[t] = mma(ph, gf, dv[t]);
+            dv[t] = mma(pl, gf, dv[t]);
             const Oct<T> qf = col_frag<T, LD>(qc, 16 * t);
             dk[t] = mma(dh, qf, dk[t]);
             dk[t] = mma(dl, qf, dk[t]);
         }
     } else {
-        const Oct<T> df = to_oct<T>(dp[0], dp[1]);
+        const Oct<T> pf = to_oct<T>(s[0], s[1]), df = to_oct<T>(dp[0], dp[1]);
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             dv[t] = mma(pf, col_frag<T, LD>(gc, 16 * t), dv[t]);
@@ -1225,11 +1236,19 @@ __global__ __launch_bounds__(256) void win_token_kernel(TokenArgs a) {
         l = fmaf(l, alpha, sum);
 #pragma unroll
         for (int x = 0; x < DP / 16; ++x) o[x] *= alpha;
-        const Oct<T> p = to_oct<T>(s[0], s[1]);
+        Oct<T> p, pl;                                          // 16-bit types: the halves of P
+        if constexpr (sizeof(T) == 2)
+            split_oct<T>(s[0], s[1], p, pl);
+        else
+            p = to_oct<T>(s[0], s[1]);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int x = 0; x < DP / 16; ++x) o[x] = mma(col_frag<T, LD>(vt, 16 * x), p, o[x]);
+        for (int x = 0; x < DP / 16; ++x) {
+            const Oct<T> vf = col_frag<T, LD>(vt, 16 * x);
+            o[x] = mma(vf, p, o[x]);
+            if constexpr (sizeof(T) == 2) o[x] = mma(vf, pl, o[x]);
+        }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -1367,8 +1386,8 @@ static int win_fwd_heads(const WinArgs& a, void* out, hipStream_t st) {
 }
 template <class T, int DP, bool FAST>
 static int win_fwd_launch(const WinArgs& a, void* out, hipStream_t st) {
-    // two heads at a time where that leaves 4 workgroups per CU and registers allow: 16 x 2048 x 8 / 2 heads x 64 bf16 48 us
-    // against 56; but D = 128 51 against 48, fp32 with D = 64 87 against 83, and at a quarter of the grid 10.5 against 8.3 us
+    // two heads at a time where that leaves 4 workgroups per CU and registers allow: 16 x 2048 x 8 / 2 heads x 64 bf16 58 us
+    // against 61, x 32 50 against 52; but x 128 106 against 97, x 64 fp32 209 against 203, and a quarter of the grid 22 against 21
     if constexpr (FAST && DP * (int)sizeof(T) <= 128 && sizeof(T) == 2)
         if (a.Hq / a.Hkv % 2 == 0 && (int64_t)a.tiles * a.Hq * a.B >= 2048) return win_fwd_heads<T, DP, FAST, 2>(a, out, st);
     return win_fwd_heads<T, DP, FAST, 1>(a, out, st);

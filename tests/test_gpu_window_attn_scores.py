@@ -195,3 +195,56 @@ def test_fp16_small_probabilities(dev, W, S):
         out = out + (2.0 ** -40 * seen @ r["V"].abs()).permute(0, 2, 1, 3)
         return out, dq, dk, dv
     _check(dev, q, k, v, go, W, S, 0.125, begin, end, limits)
+
+
+FAR = [(1, 400, 2, 1, D, 24, 5) for D in (7, 24, 32, 50, 80, 128, 150, 256)] + [(3, 330, 8, 2, 64, 16, 33), (2, 620, 1, 1, 16, 40, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,L,Hq,Hkv,D,W,S", [(3, 150, 4, 2, 64, 40, 3), (2, 100, 2, 2, 128, 100, 0)] + FAR)
+def test_errors_are_those_of_one_rounding(dev, B, L, Hq, Hkv, D, W, S, dt):
+    """16-bit types: P and dS enter their products as two halves (e^2 left of them), delta is corrected, so beside the one
+    rounding of the result there is nothing of the order e.  FAR: shapes whose first items get the gradients of far queries
+    from a launch of their own, at every tile width.  Outside the history stands NaN.
+    fp16: P times 2^15 and dS brought to 2^13 or more lose 2^-40 and 2^-38 of the largest."""
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, dt, 0.25, 4, B + L + D)
+    pos = torch.arange(L)[None]
+    pad = (pos < begin[:, None]) | (pos >= end[:, None])
+    for t in (q, k, v, go):
+        t[pad] = math.nan
+    scale = 0.25
+    e = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+
+    def limits(r, vis):
+        lims = _limits(r, vis, dt, D, Hq // Hkv, scale, e * e, e * e)
+        if dt != torch.float16:
+            return lims
+        seen, big = vis[:, None].double(), (r["p"] * (r["dp"] - r["delta"])).abs().amax() * scale
+        back = lambda t: t.permute(0, 2, 1, 3)
+        return (lims[0] + back(2.0 ** -40 * seen @ r["V"].abs()), lims[1] + back(2.0 ** -38 * big * seen @ r["K"].abs()),
+                lims[2] + r["group"](2.0 ** -38 * big * seen.transpose(2, 3) @ r["Q"].abs()),
+                lims[3] + r["group"](2.0 ** -40 * seen.transpose(2, 3) @ r["GO"].abs()))
+    _check(dev, q, k, v, go, W, S, scale, begin, end, limits)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("L,D", [(100, 64), (3000, 64), (700, 80)])
+def test_token_errors_are_those_of_one_rounding(dev, L, D, dt):
+    """The single-token form, in one workgroup and split over several."""
+    from deeprec_amd import kernels as Kn
+    B, Hq, Hkv = 3, 4, 2
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, dt, 0.25, 4, L + D)
+    out = Kn.window_attn_token(q[:, 0].to(dev), k.to(dev), v.to(dev), L, 0, 0.25, begin.to(dev), end.to(dev))
+    lo, hi = begin.long()[:, None, None], end.long()[:, None, None]
+    j = torch.arange(L)[None, None]
+    vis = ((j >= lo) & (j < hi))                                             # [B, 1, L]: one query
+    Q, K, V = q[:, 0].double()[:, :, None], *(t.double().permute(0, 2, 1, 3).repeat_interleave(Hq // Hkv, 1) for t in (k, v))
+    s = (Q @ K.transpose(2, 3) * 0.25).masked_fill(~vis[:, None], -math.inf)
+    p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+    r = dict(p=p, n=vis.sum(2)[:, None, :, None].double())
+    e = torch.finfo(dt).eps / 2
+    ref = (p @ V)[:, :, 0]
+    lim = ((p * (_relp(r, vis) + e * e) + 2.0 ** -40 * vis[:, None]) @ V.abs())[:, :, 0]
+    _within("out", out, ref, lim * (1 + e) + e * ref.abs() + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2 + 1e-30)
