@@ -204,6 +204,18 @@ class GraphedStep:
 SPARSE_DENSE_MIN = 1 << 22     # elements: below this a table's dense-L2 step keeps the dense-gradient form
 
 
+def clip_norm_of(clip_norm, shard=None):
+    """A model's or optimizer's clip_norm argument, refused where no step could apply it: not a positive float32 number, or
+    row-sharded tables, whose rows are spread over ranks."""
+    if clip_norm is None:
+        return None
+    if not 0 < np.float32(clip_norm) < np.inf:
+        raise ValueError("clip_norm must be positive and finite, got %s" % (clip_norm,))
+    if active_shard(shard) is not None:
+        raise ValueError("clip_norm with sharded tables: their rows are spread over ranks; their global norm is not offered")
+    return float(clip_norm)
+
+
 class TFOptimizer:
     """kind: 'adam' (TF1 eps 1e-8 / Keras 1e-7), 'adagrad' (initial accumulator 0.1), 'rmsprop', 'sgd'."""
     KIND = {"sgd": K.OPT_SGD, "adam": K.OPT_ADAM, "adagrad": K.OPT_ADAGRAD, "rmsprop": K.OPT_RMSPROP}
@@ -213,7 +225,7 @@ class TFOptimizer:
                  rho=0.9, momentum=0.0, clip_norm=None):
         """clip_norm: the global norm that clip() holds a step's gradients to (None: clip() does nothing)."""
         self.kind, self.lr = kind, float(learning_rate)
-        self.clip_norm = None if clip_norm is None else float(clip_norm)
+        self.clip_norm = clip_norm_of(clip_norm)
         self.eps = float(eps if eps is not None else (1e-8 if kind == "adam" else 1e-10))
         self.beta1, self.beta2, self.acc0, self.rho, self.momentum = beta1, beta2, initial_accumulator_value, rho, momentum
         self.step_count = 0

@@ -14,7 +14,7 @@ import torch
 
 from ... import kernels as K
 from ...utils.evaluation.SeqRecMetrics import evaluate_caser
-from .._common import (TFOptimizer, Table, active_shard, seq_dot_loss, device_of, normal_, shift_sess, to_dev, load_checkpoint, save_checkpoint)
+from .._common import (TFOptimizer, Table, active_shard, clip_norm_of, seq_dot_loss, device_of, normal_, shift_sess, to_dev, load_checkpoint, save_checkpoint)
 from ._seq_common import SeqBase
 
 
@@ -91,7 +91,7 @@ class Caser(SeqBase):
     def __init__(self, sess, num_user=None, num_item=None, learning_rate=0.001, reg_rate=1e-6, epoch=500, batch_size=1000,
                  show_time=False, T=1, display_step=1000, verbose=False, device=None, shard=None, sampler="reference", clip_norm=None):
         # clip_norm: global norm that a step's gradients are held to (TFOptimizer.clip); None: the reference's behaviour
-        self.clip_norm = clip_norm
+        self.clip_norm = clip_norm_of(clip_norm, shard)
         self.sess, self.num_user, self.num_item = shift_sess(sess, num_user, num_item)
         self.shard = active_shard(shard)                    # _common.Shard: data-parallel over ranks, tables row-sharded
         self.learning_rate = learning_rate

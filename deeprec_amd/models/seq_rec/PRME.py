@@ -10,7 +10,7 @@ import torch
 
 from ... import kernels as K
 from ...utils.evaluation import SeqRecMetrics
-from .._common import (TFOptimizer, Table, seq_dist_loss, device_of, normal_, shift_sess, to_dev, load_checkpoint, save_checkpoint)
+from .._common import (TFOptimizer, Table, clip_norm_of, seq_dist_loss, device_of, normal_, shift_sess, to_dev, load_checkpoint, save_checkpoint)
 from ._seq_common import SeqBase
 
 
@@ -18,7 +18,7 @@ class PRME(SeqBase):
     def __init__(self, sess, num_user=None, num_item=None, learning_rate=0.001, reg_rate=1e-2, epoch=5000, batch_size=1000,
                  show_time=False, T=1, display_step=1000, verbose=False, device=None, sampler="reference", clip_norm=None):
         # clip_norm: global norm that a step's gradients are held to (TFOptimizer.clip); None: the reference's behaviour
-        self.clip_norm = clip_norm
+        self.clip_norm = clip_norm_of(clip_norm)
         self.sess, self.num_user, self.num_item = shift_sess(sess, num_user, num_item)
         self.learning_rate = learning_rate
         self.epochs = epoch
