@@ -248,3 +248,60 @@ def test_token_errors_are_those_of_one_rounding(dev, L, D, dt):
     ref = (p @ V)[:, :, 0]
     lim = ((p * (_relp(r, vis) + e * e) + 2.0 ** -40 * vis[:, None]) @ V.abs())[:, :, 0]
     _within("out", out, ref, lim * (1 + e) + e * ref.abs() + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2 + 1e-30)
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_far_first_items_in_graphs(dev, dt):
+    """Forward and backward captured twice, far first items by their own launch; replayed with eager calls between, once on
+    scores beyond 65536, where the backward takes the rows' maxima itself: the same bits as the eager call every time."""
+    from deeprec_amd import kernels as Kn
+    B, L, Hq, Hkv, D, W, S = 3, 400, 4, 2, 64, 24, 5
+    q, k, v, go, begin, end = (t.to(dev) for t in _integers(B, L, Hq, Hkv, D, dt, 0.25, 4, 3))
+    mask = dict(window=W, sinks=S, begin=begin, end=end)
+
+    def call():
+        o, s = Kn.window_attn_forward(q, k, v, **mask)
+        return (o, s) + Kn.window_attn_backward(q, k, v, o, s, go, **mask)
+    call()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = call()
+        graphs.append((gr, res))
+    for size in (1.0, 4096.0, 0.5, 1.0):
+        for t in (q, k, v, go):
+            t.normal_()
+        q.mul_(size)
+        k.mul_(size if size < 2 else 64.0)
+        mine = call()
+        assert (float(mine[1][mine[1] > -math.inf].abs().max()) > 65536) == (size > 2)
+        for gr, res in graphs:
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(res, mine))
+        assert all(torch.equal(a, b) for a, b in zip(call(), mine))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** 10])
+def test_loss_scale_with_far_first_items(dev, dt, size):
+    """dO far from 1 where the first items' far gradients join those of the window (fp16: each with a power of two of its own)."""
+    B, L, Hq, Hkv, D, W, S = 2, 500, 4, 2, 64, 40, 20
+    q, k, v, go, begin, end = _integers(B, L, Hq, Hkv, D, dt, 0.25, 4, 19)
+    go = (go.float() * size).to(dt)
+    e = torch.finfo(dt).eps / 2
+
+    def limits(r, vis):
+        lims = _limits(r, vis, dt, D, Hq // Hkv, 0.25, e * e, e * e)
+        if dt != torch.float16:
+            return lims
+        seen, big = vis[:, None].double(), (r["p"] * (r["dp"] - r["delta"])).abs().amax() * 0.25
+        back = lambda t: t.permute(0, 2, 1, 3)
+        return (lims[0] + back(2.0 ** -40 * seen @ r["V"].abs()), lims[1] + back(2.0 ** -38 * big * seen @ r["K"].abs()),
+                lims[2] + r["group"](2.0 ** -38 * big * seen.transpose(2, 3) @ r["Q"].abs()),
+                lims[3] + r["group"](2.0 ** -40 * seen.transpose(2, 3) @ r["GO"].abs()))
+    _check(dev, q, k, v, go, W, S, 0.25, begin, end, limits)
