@@ -2,7 +2,7 @@
 //   key j is visible to query i iff begin <= j <= i < end and (i - j < window or j - begin < sinks)
 //   out_i = sum_j p_ij v_j,  p_i = softmax_j(scale <q_i, k_j>) over the visible j;   lse_i = log sum_j exp(scale <q_i, k_j>)
 // [begin, end) is the part of the row that holds the history (padding on either side); a query outside it gets zeros and
-// lse = -inf, keys and values outside it are never read.  Hq query heads share Hkv key / value heads in groups.
+// lse = -inf, and what stands outside reaches no result.  Hq query heads share Hkv key / value heads in groups.
 //
 // Tiles of 16 queries x 16 keys on the matrix cores.  The contraction is laid out so that nothing moves between lanes: with
 // S^T = K Q^T a lane holds, for ONE query, four keys of each 16-key tile (rows 4 g + i of lane group g), and that is already
@@ -367,7 +367,7 @@ __device__ __forceinline__ void wave_stage(T* tile, const T* base, int64_t ld, i
 // Workgroups go to the 8 XCDs in turn and each XCD has its own L2: dealt out one by one, neighbours along the sequence, which
 // read the same rows, would fetch them into 8 caches.  So runs of WA_RUN neighbours go to one XCD, the runs in turn (whole
 // eighths of the grid would leave an XCD with nothing but the short histories of a batch).  dK / dV of 4 x 2047 x 8 / 2 heads x
-// 128 bf16: 56.5 us one by one, 54.0 in runs of 16, 53.6 in runs of 32; of 64 x 200 x 2 x 64 fp32: 35.3, 33.1, 32.6 us.
+// 128 bf16 (P in one half): 56.5 us one by one, 54.0 in runs of 16, 53.6 in runs of 32; of 64 x 200 x 2 x 64 fp32: 35.3, 33.1, 32.6 us.
 constexpr int WA_RUN = 32;
 __device__ __forceinline__ unsigned win_block() {
     constexpr unsigned ROUND = 8 * WA_RUN;
@@ -399,10 +399,10 @@ struct KeyTiles {
 // A workgroup of 4 wavefronts takes 64 queries of one head; the key and value tiles it needs go through LDS, the next
 // tile's loads in flight while one is used (two buffers; one where two would not leave room for a second workgroup).
 // NH = 2: two heads of a group at once, which share the tiles, the key and value operands read from LDS and the masks.
-// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 28 us, 8.0 useful GFLOP = 285 TFLOP/s.  LDS reads (16 KB a wavefront and
-// tile), exponentials and matrix instructions take about a third each and overlap only across wavefronts: without its loads
-// from memory the kernel takes 24.6 us, without its products 19.4.  64 x 200 x 2 x 64 fp32, window 50: 18 us.
-// Tried: 64 keys in one buffer instead of 32 in two, 35.6 us.
+// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 30.5 us, 8.0 useful GFLOP = 262 TFLOP/s.  LDS reads (16 KB a wavefront and
+// tile), exponentials and matrix instructions take about a third each and overlap only across wavefronts (with P in one half,
+// 28 us: 24.6 without its loads from memory, 19.4 without its products).  64 x 200 x 2 x 64 fp32, window 50: 18 us.
+// Tried: 64 keys in one buffer instead of 32 in two, 35.6 us against 29.6.
 template <class T, int DP>
 constexpr int fwd_buffers() {
     return DP * (int)sizeof(T) <= 512 ? 2 : 1;
@@ -576,16 +576,17 @@ __global__ __launch_bounds__(256, NH == 1 && DP * (int)sizeof(T) <= 256 ? 3 : (D
 // ---- backward: dQ ------------------------------------------------------------------------------------------------------------
 // dS = P (dP - delta) scale with delta_i = sum_j p_ij dP_ij;  dQ^T = K^T dS^T in the forward's layout.  Writes delta for the
 // others.  dP - delta cancels where one key carries a row, so delta has to be as exact as dP.  For fp32 it is <dO_i, O_i>;
-// a 16-bit O is off by half a step and its P was rounded too (measured: dQ, dK 1.8 times as far from 64 bits as the rounding
-// of the result alone).  16-bit types start from that delta_0 and correct it: with r = sum p (dP - delta_0) = delta - delta_0,
+// a 16-bit O is off by half a step (uncorrected, dQ and dK were 1.8 times as far from 64 bits as the rounding of the result
+// alone).  16-bit types start from that delta_0 and correct it: with r = sum p (dP - delta_0) = delta - delta_0,
 //   dQ = scale (sum p (dP - delta_0) K - r sum p K),
 // r being small, the second sum needs no more than P rounded to 16 bits.  The first one's weights are split into two halves
 // (hi + what hi misses), one more matrix instruction instead of another half step lost.  (Running the tiles twice, first
-// for delta, is as exact and took 77 us where this takes 48 at 4 x 2047 x 8 x 128.)
+// for delta, is as exact and took 77 us where this took 48 at 4 x 2047 x 8 x 128.)
 // P from lse alone would be off by lse's rounding: 1e-3 of P at scores of 1e4.  So lse only gives a reference near the row's
 // maximum, ref = lse / scale; the kernel, which sees the whole row, sums the weights 2^((s - ref) c) itself, divides by the sum
 // l in the end and hands ref and norm = log2 l to the others.  Where |lse| reaches WA_FAR its rounding (half a unit of log 2 at
-// 2^23) could carry the weights out of range: there the workgroup takes the maximum itself in a first run over the keys.
+// 2^23) could carry the weights out of range: there the workgroup takes the maximum itself in a first run over the keys
+// (backward of 4 x 2047 x 8 / 2 x 128 bf16: 137 us, 121 without).
 constexpr float WA_FAR = 65536.0f;
 // fp16 holds dS of no gradient, value or scale by itself: it is multiplied by a power of two that brings the largest |dS| to
 // [2^13, 2^14), so that nothing overflows and the two halves keep 2^-38 of the largest.  Here that power, at most 2^100
@@ -823,8 +824,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 
 // ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
 // S = Q K^T here, so a lane holds one KEY and four queries of each 16: the A operand of dV = P^T dO and dK = dS^T Q.
-// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 53 us (dQ: 48 us), 64 x 200 x 2 x 64 fp32: 33 us (25 us).  A step of 32 queries
-// x 16 keys reads 32 KB from LDS for 40 matrix instructions: LDS takes half of the time, and 32 keys a wavefront, which
+// 4 x 2047 x 8 / 2 heads x 128 bf16, window 256: 58 us (dQ: 51 us), 64 x 200 x 2 x 64 fp32: 33 us (26 us).  A step of 32 queries
+// x 16 keys reads 33 KB from LDS for 48 matrix instructions: LDS takes half of the time, and 32 keys a wavefront, which
 // would halve that, do not fit the registers at D = 128.
 // one (32 queries x 16 keys) step: adds to dk, dv what the queries [q_first, q_first + q_count) give the lane's key (whole:
 // all of them do)
@@ -885,7 +886,7 @@ __device__ __forceinline__ void dkdv_step(const WinArgs& a, const T* qc, const T
 }
 
 // The power of two for dS of the queries [q0, q1] of a group's heads (fp16: grad_up of the largest |dS| that win_dq_kernel met;
-// queries whose dS is not finite make NaN what they see, whatever it is)
+// queries whose dS is not finite give what they see no finite gradient, whatever it is)
 // In two steps, with loads of the caller's own between them: first() requests a lane's first value, scale() the rest and
 // gives the answer.
 template <class T>
@@ -919,8 +920,8 @@ struct GradScale {
 // A workgroup takes 32 keys of one key head and walks the queries that see them through the window, 64 at a time, head by
 // head of the group (so the group's sum needs no atomics): wavefront (w, x) takes key half w and query half x, the halves
 // of the queries are added up at the end.  What the first items get from queries beyond the window is found here too
-// where that is at most 8 more steps (backward of 64 x 200 x 2 x 64 fp32 with 2 first items, 3 steps: 62 us, 67 us with a launch
-// of its own; 32 x 600, 9 steps: 101 and 94 us); else it comes from win_sink_kernel's partial sums, added last and in order.
+// where that is at most 8 more steps (backward of 64 x 200 x 2 x 64 fp32 with 2 first items, 3 steps: 62 us, 65 us with a launch
+// of its own; 32 x 600, 9 steps: 101 and 93 us); else it comes from win_sink_kernel's partial sums, added last and in order.
 // (One buffer: with two the two workgroups on the CU, which hide each other's barriers, gain nothing.)
 // a second workgroup on the CU is worth more than registers to spare (at D <= 128 in 16 bits, 64 in fp32)
 template <class T, int DP, bool FAST>
@@ -1057,7 +1058,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 256 ? 2 : 1) void win_d
 // ---- backward: what the first items get from queries beyond the window ----------------------------------------------------------
 // Every query of a long history sees them, so their sums are split over chunks of 64 queries: NW wavefronts, each with its
 // own tiles of 32 queries in LDS, all on the same 16 first items, added up over LDS in order.  4 x 2047 x 8 / 2 heads x 128 bf16:
-// 13 us, bound by the latency of a chunk's loads; every wavefront does one or two tiles.
+// 12 us, bound by the latency of a chunk's loads; every wavefront does one or two tiles.
 constexpr int WA_CHUNK = 64;
 template <class T, int DP>
 constexpr int sink_waves() {
@@ -1446,7 +1447,7 @@ static void token_split(int64_t B, int Hkv, int hgroups, int64_t keys, int D, in
 static int64_t token_keys(int64_t L, int64_t window, int32_t sinks) { return window >= L ? L : (window + sinks < L ? window + sinks : L); }
 
 // FAST: the head dim fills its tile and rows are read in 16-byte pieces: no column checks anywhere (forward + backward of
-// 4 x 2047 x 8 / 2 heads x 128 bf16: 31 + 115 us, 47 + 141 us without; 64 x 200 x 2 x 64 fp32: 18 + 62 and 19 + 68 us)
+// 4 x 2047 x 8 / 2 heads x 128 bf16: 31 + 114 us, 47 + 142 us without; 64 x 200 x 2 x 64 fp32: 18 + 62 and 19 + 66 us)
 #define WIN_BY_D(T, fast, launch, ...)                                                                        \
     return a.D <= 32    ? ((fast) && a.D == 32 ? launch<T, 32, true>(__VA_ARGS__) : launch<T, 32, false>(__VA_ARGS__))   \
            : a.D <= 64  ? ((fast) && a.D == 64 ? launch<T, 64, true>(__VA_ARGS__) : launch<T, 64, false>(__VA_ARGS__))   \

@@ -1408,9 +1408,9 @@ def window_attn_forward(q, k, v, window, sinks=0, scale=None, begin=None, end=No
     """Causal attention over the last `window` positions and the first `sinks` items of each history.  q [B, L, Hq, D],
     k, v [B, L, Hkv, D] (float32 / float16 / bfloat16, any strides with the last dim contiguous), Hq a multiple of Hkv.
     Key j is visible to query i iff begin <= j <= i < end and (i - j < window or j - begin < sinks); begin / end: int32 [B]
-    (None: the whole row), so padding may stand on either side; padded positions are never read and give zero rows.
-    A value inside the history that is not finite makes NaN whatever sees it, and may do so to what shares a tile of 32
-    positions with it.  scale (1e-30 .. 1e30) None: D ** -0.5.  Returns (out [B, L, Hq, D], lse float32 [B, Hq, L])."""
+    (None: the whole row), so padding may stand on either side; padded positions reach no result and give zero rows.
+    A value inside the history that is not finite makes NaN whatever sees it (but a score of -inf just weighs nothing), and
+    may do so to what shares a tile of 32 positions with it.  scale (1e-30 .. 1e30) None: D ** -0.5.  Returns (out [B, L, Hq, D], lse float32 [B, Hq, L])."""
     sq, sk, sv, B, L, Hq, Hkv, D, dt, window, sinks, scale = _win_operands(q, k, v, 4, window, sinks, scale, begin, end)
     out = _like(q)
     lse = torch.empty((B, Hq, L), dtype=torch.float32, device=q.device)

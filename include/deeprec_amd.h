@@ -550,9 +550,9 @@ int32_t dr_shard_bpr_finish(float* P, float* Pslot0, float* Pslot1, float* Q, fl
 /* ---- global gradient norm over many tensors, and clipping -----------------------------------------------------------
  * tf.clip_by_global_norm (the reference clips rows only, cml.py:80-81): norm = sqrt(sum over the n tensors of the sum of
  * their squared elements), out[i] = in[i] * clip_norm / max(norm, clip_norm); a norm that is not finite makes every output
- * NaN.  in / out / count / dtype are HOST arrays of n device pointers, element counts and DR_F32 / DR_F16 / DR_BF16; every
- * tensor is contiguous, out[i] has in[i]'s type.  out[i] == in[i] clips in place; any other overlap of an output is
- * refused.  out NULL: only the norm.  norm_out: fp32 device scalar (NULL: not wanted).  Sums in fp64, in a fixed order.
+ * NaN (where a finite norm passes fp32's range, norm_out is inf and the outputs are as the formula says).
+ * in / out / count / dtype are HOST arrays of n device pointers, element counts and DR_F32 / DR_F16 / DR_BF16; every tensor
+ * is contiguous, out[i] has in[i]'s type.  out[i] == in[i] clips in place; any other overlap of an output is refused.  out NULL: only the norm.  norm_out: fp32 device scalar (NULL: not wanted).  Sums in fp64, in a fixed order.
  * Recorded gradient rows of a table count row by row, duplicates not combined, as TensorFlow's IndexedSlices do. */
 int64_t dr_global_norm_bytes(int32_t n);
 int32_t dr_clip_global_norm(const void* const* in, void* const* out, const int64_t* count, const int32_t* dtype, int32_t n,
@@ -577,12 +577,13 @@ int32_t dr_embed_backward(const void* gout, int64_t n, int32_t d, int32_t dtype,
  * Key j is visible to query i iff begin[b] <= j <= i < end[b] and (i - j < window or j - begin[b] < sinks); window >= 1,
  * 0 <= sinks <= 64; begin / end int32 [B] on the device (NULL: 0 / L), cut to [0, L].  1e-30 <= scale <= 1e30.
  * forward: out [B, L, Hq, D] contiguous, lse [B, Hq, L] fp32 = log sum exp(scale <q, k>).  A position outside [begin, end)
- * gives a zero row (lse -inf, gradients 0) and is never read.  backward: out, lse as written, gout [B, L, Hq, D]
- * contiguous -> dq [B, L, Hq, D], dk, dv [B, L, Hkv, D] contiguous, overwritten; sums over a group's heads included; no
+ * gives a zero row (lse -inf, gradients 0) and what it holds reaches no result.  backward: out, lse as written, gout
+ * [B, L, Hq, D] contiguous -> dq [B, L, Hq, D], dk, dv [B, L, Hkv, D] contiguous, overwritten; sums over a group's heads included; no
  * atomics, bit-repeatable.  ws: dr_window_attn_backward_bytes(...), 256-byte aligned.
- * A position that is not finite inside the history makes NaN what sees it, and may make NaN what shares a tile of 32
- * positions with it without seeing it (the products run over whole tiles); outside the history it may be anything.  Outputs
- * and workspace must not overlap the inputs.
+ * Any score that fp32 holds keeps fp32's digits; 16-bit results are off by their own rounding and by what fp32 sums leave.
+ * A position that is not finite inside the history makes NaN what sees it (but a score of -inf just weighs nothing), and may
+ * make NaN what shares a tile of 32 positions with it without seeing it (the products run over whole tiles); outside the
+ * history it may be anything.  Outputs and workspace must not overlap the inputs.
  * token: ONE query per sequence, q [B, Hq, D] (strides {batch, head}), at position end[b] - 1 of a cache k, v [B, L, Hkv, D]
  * that already holds its own key and value -> out [B, Hq, D] contiguous.  ws: dr_window_attn_token_bytes(...), 256-byte
  * aligned (0 bytes: NULL). */
